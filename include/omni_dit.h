@@ -77,6 +77,56 @@ int odit_attn_fwd(const void* q, const void* k, const void* v, void* o, const ui
                   const int64_t v_strides[3], const int64_t o_strides[3], float scale, int dtype,
                   void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * A text stage beside the transformer: what a query sees, and what its scores become.
+ *   s = scale * q.k;  cap > 0: s = cap * tanh(s / cap);  then one of
+ *   slopes [H]:                 s -= slopes[h] * |away|
+ *   distance [H][2 radius + 1]: s += distance[h][clamp(away, -radius, radius) + radius]
+ * with away = key's position - query's position. The last of a document's queries is at the place of its last key.
+ *   docs > 0: query rows [q_starts[n], q_starts[n+1]) and key rows [k_starts[n], k_starts[n+1]) are document n, and a query sees keys of its
+ *     own document alone (int32 [docs + 1], on the device, in rising order; rows of no document see nothing). docs == 0: each batch row is one.
+ *   causal: no key behind the query; window > 0: keys with |away| < window; prefix (int32, per document, on the device): the first prefix[n]
+ *     keys of the document are seen in any case.
+ */
+typedef struct odit_attn_rules {
+  int causal, window, docs, radius;
+  float cap; /* 0 (none) or up to 8192 */
+  const int *q_starts, *k_starts, *prefix;
+  const float *slopes, *distance;
+} odit_attn_rules;
+
+/* o = softmax(rules(q k^T)) v over whole prompts: q [B,Sq,H,D], k, v [B,Sk,Hkv,D], o [B,Sq,H,D] with strides as in odit_attn_fwd, bf16 or
+ * fp16, D 64 or 128. Documents cut every batch row alike. A query that sees nothing gets zeros; what keys and values hold that a query does
+ * not see (NaN and infinities too) does not reach it. */
+int odit_attn_ruled(const void* q, const void* k, const void* v, void* o, int B, int Sq, int Sk, int H, int Hkv, int D,
+                    const int64_t q_strides[3], const int64_t k_strides[3], const int64_t v_strides[3], const int64_t o_strides[3],
+                    float scale, const odit_attn_rules* rules, int dtype, void* stream);
+
+/* The same for one new token per sequence, q and o [B,H,D] (strides for batch and head), over a paged cache: key and value caches
+ * [pages,page_size,Hkv,D] (strides for page, row and head, multiples of 8), table int32 [B,max_pages] (row stride table_stride) of pages,
+ * lengths int32 [B]. Key j of a sequence is row j % page_size of page table[b][j / page_size]; the query is at the place of key
+ * lengths[b] - 1. Lengths past max_pages * page_size count as that, below 0 as 0; a length of 0 gives zeros; keys whose page number lies
+ * outside [0, pages) are not seen. Of the rules, docs and prefix do not apply (0 and NULL).
+ * `workspace`: odit_attn_paged_workspace_bytes for the same shape and window (may be 0), contents irrelevant before and after. */
+size_t odit_attn_paged_workspace_bytes(int B, int H, int Hkv, int D, int max_pages, int page_size, int window);
+int odit_attn_paged(const void* q, const void* key_cache, const void* value_cache, const int* table, const int* lengths, void* o, int B,
+                    int H, int Hkv, int D, int pages, int page_size, int max_pages, const int64_t q_strides[2],
+                    const int64_t key_cache_strides[3], const int64_t value_cache_strides[3], int64_t table_stride,
+                    const int64_t o_strides[2], float scale, const odit_attn_rules* rules, int dtype, void* workspace,
+                    size_t workspace_bytes, void* stream);
+
+/* Rotary positions of T packed tokens, and their keys and values into such a cache. Pair i < rot/2 of each head of q [T,H,D] and k [T,Hkv,D]
+ * (strides for token and head, multiples of 8; D a multiple of 8 up to 1024) is turned by positions[t] * turns[i] whole turns (fp64, so far
+ * positions keep their angle) and scaled by `magnitude`; features from rot on pass through. ODIT_FLAG_NEOX: pairs (i, i+rot/2), otherwise
+ * (2i, 2i+1). q_out [T,H,D] is dense. slots == NULL: rotated keys go to k_out [T,Hkv,D], dense; v and the caches are NULL.
+ * slots int64 [T]: rotated keys and the values v [T,Hkv,D] go to row slots[t] % page_size of page slots[t] / page_size, k_out is NULL;
+ * tokens whose slot lies outside the cache are not stored. Slots are distinct: of two tokens with one slot, either's features are left there. */
+int odit_rope_append(const void* q, const void* k, const void* v, const int64_t* positions, const double* turns, void* q_out, void* k_out,
+                     const int64_t* slots, void* key_cache, void* value_cache, int64_t T, int H, int Hkv, int D, int rot, int64_t pages,
+                     int page_size, const int64_t q_strides[2], const int64_t k_strides[2], const int64_t v_strides[2],
+                     const int64_t key_cache_strides[3], const int64_t value_cache_strides[3], float magnitude, int dtype, unsigned flags,
+                     void* stream);
+
 /* Extended form of odit_attn_fwd with three optional additions.
  *
  * Values in two tensors: with v_tail != NULL, key rows [0, k_split) take their values from `v` and rows

@@ -42,6 +42,19 @@ _SIGNATURES = {
          C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
          _i64p, _i64p, _i64p, _i64p, _i64p, _i64p, C.c_float, C.c_int, C.c_void_p, C.c_size_t, C.c_void_p],
     ),
+    "odit_attn_ruled": (
+        C.c_int,
+        [C.c_void_p] * 4 + [C.c_int] * 6 + [_i64p] * 4 + [C.c_float, C.c_void_p, C.c_int, C.c_void_p],
+    ),
+    "odit_attn_paged_workspace_bytes": (C.c_size_t, [C.c_int] * 7),
+    "odit_attn_paged": (
+        C.c_int,
+        [C.c_void_p] * 6 + [C.c_int] * 7 + [_i64p] * 3 + [C.c_int64, _i64p, C.c_float, C.c_void_p, C.c_int, C.c_void_p, C.c_size_t, C.c_void_p],
+    ),
+    "odit_rope_append": (
+        C.c_int,
+        [C.c_void_p] * 10 + [C.c_int64] + [C.c_int] * 4 + [C.c_int64, C.c_int] + [_i64p] * 5 + [C.c_float, C.c_int, C.c_uint, C.c_void_p],
+    ),
     "odit_attn_fwd_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int]),
     "odit_attn_fwd_plan": (
         C.c_int,
@@ -181,6 +194,13 @@ class LinearProblem(C.Structure):
 
     _fields_ = [(n, C.c_void_p) for n in ("x", "w", "bias", "residual", "gate", "out")] + [("M", C.c_int), ("rows_per_gate", C.c_int)] + [
         (n, C.c_int64) for n in ("ldx", "ldw", "ldo", "ldr", "gate_stride")]
+
+
+class AttnRules(C.Structure):
+    """``odit_attn_rules``."""
+
+    _fields_ = [(n, C.c_int) for n in ("causal", "window", "docs", "radius")] + [("cap", C.c_float)] + [
+        (n, C.c_void_p) for n in ("q_starts", "k_starts", "prefix", "slopes", "distance")]
 
 
 class Embedder(C.Structure):

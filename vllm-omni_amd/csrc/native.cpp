@@ -20,6 +20,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/hip/EmptyTensor.h>
+#include <c10/core/GradMode.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
@@ -578,6 +579,180 @@ PyObject* py_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
   PyTuple_SET_ITEM(r, 1, wrap(std::move(ot)));
   PyTuple_SET_ITEM(r, 2, wrap(std::move(lse)));
   return r;
+  NATIVE_END
+}
+
+// ------------------------------------------------------------------------------------- a text stage's operators
+// whether a gradient would be asked of the result: kernels.py refuses that
+bool wants_grad(std::initializer_list<const Tensor*> ts) {
+  if (!c10::GradMode::is_enabled()) return false;
+  for (const Tensor* t : ts)
+    if (t && t->requires_grad()) return true;
+  return false;
+}
+
+// a dense tensor of this type and shape (shape[i] < 0: any), or none at all
+bool dense(const Tensor* t, at::ScalarType type, std::initializer_list<int64_t> shape) {
+  if (!t) return true;
+  if (t->scalar_type() != type || t->dim() != static_cast<int64_t>(shape.size()) || !t->is_contiguous()) return false;
+  int64_t i = 0;
+  for (const int64_t n : shape)
+    if (const int64_t at = i++; n >= 0 && t->size(at) != n) return false;
+  return true;
+}
+
+// causal, window (None or a number), cap, slopes, distance: the rules that both attentions have. -1: an error is set, 0: not of the usual form
+int score_rules(PyObject* causal, PyObject* window, PyObject* cap, PyObject* slopes, PyObject* distance, int64_t H, const Where& w, odit_attn_rules* r) {
+  const Tensor *sl, *di;
+  if (!optional_tensor(slopes, &sl) || !optional_tensor(distance, &di)) return 0;
+  *r = odit_attn_rules{};
+  r->causal = causal ? PyObject_IsTrue(causal) : 1;
+  if (r->causal < 0) return -1;
+  if (window != Py_None) {
+    if (!PyLong_Check(window)) return 0;
+    int over = 0;
+    const long n = PyLong_AsLongAndOverflow(window, &over);
+    if (over || n <= 0 || n > (1l << 30)) return 0;
+    r->window = static_cast<int>(n);
+  }
+  const double c = PyFloat_AsDouble(cap);
+  if (c == -1.0 && PyErr_Occurred()) return -1;
+  r->cap = static_cast<float>(c);
+  if ((sl && di) || !w.holds(sl) || !w.holds(di) || !dense(sl, at::kFloat, {H}) || !dense(di, at::kFloat, {H, -1}) || wants_grad({sl, di})) return 0;
+  r->slopes = static_cast<const float*>(ptr(sl));
+  r->distance = static_cast<const float*>(ptr(di));
+  if (di) {
+    if (di->size(1) % 2 == 0 || di->size(1) > 65535) return 0;
+    r->radius = static_cast<int>(di->size(1) / 2);
+  }
+  return 1;
+}
+
+// (q, k, v, scale, causal, window, prefix, q_starts, k_starts, cap, slopes, distance)
+PyObject* py_attn_ruled(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  NATIVE_BEGIN
+  const Tensor *q, *k, *v, *prefix, *qst, *kst;
+  if (n != 12 || !(q = tensor_of(a[0])) || !(k = tensor_of(a[1])) || !(v = tensor_of(a[2])) || !optional_tensor(a[6], &prefix) ||
+      !optional_tensor(a[7], &qst) || !optional_tensor(a[8], &kst))
+    return none();
+  const double scale = PyFloat_AsDouble(a[3]);
+  if (PyErr_Occurred()) return nullptr;
+  const Where w;
+  for (const Tensor* t : {q, k, v, prefix, qst, kst})
+    if (!w.holds(t)) return none();
+  if (!attn_operand(*q) || !attn_operand(*k) || !attn_operand(*v) || wants_grad({q, k, v})) return none();
+  const int dt = code_of(*q);
+  if ((dt != ODIT_BF16 && dt != ODIT_F16) || k->scalar_type() != q->scalar_type() || v->scalar_type() != q->scalar_type()) return none();
+  const int64_t B = q->size(0), Sq = q->size(1), H = q->size(2), D = q->size(3), Sk = k->size(1), Hkv = k->size(2), most = 1 << 30;
+  if (k->size(0) != B || k->size(3) != D || v->sizes() != k->sizes() || B == 0 || Sq == 0 || Sk == 0 || B > most || Sq > most || Sk > most) return none();
+  if (!qst != !kst || !dense(qst, at::kInt, {-1}) || (qst && (qst->size(0) < 2 || qst->size(0) > most)) || !dense(kst, at::kInt, {qst ? qst->size(0) : -1}) ||
+      !dense(prefix, at::kInt, {qst ? qst->size(0) - 1 : B}))
+    return none();
+  odit_attn_rules r;
+  const int ok = score_rules(a[4], a[5], a[9], a[10], a[11], H, w, &r);
+  if (ok <= 0) return ok < 0 ? nullptr : none();
+  r.docs = qst ? static_cast<int>(qst->size(0) - 1) : 0;
+  r.q_starts = static_cast<const int*>(ptr(qst));
+  r.k_starts = static_cast<const int*>(ptr(kst));
+  r.prefix = static_cast<const int*>(ptr(prefix));
+  Tensor o = fresh({B, Sq, H, D}, q->options());
+  const int64_t qs[3] = {q->stride(0), q->stride(1), q->stride(2)}, ks[3] = {k->stride(0), k->stride(1), k->stride(2)},
+                vs[3] = {v->stride(0), v->stride(1), v->stride(2)}, os[3] = {Sq * H * D, H * D, D};
+  if (unlocked([&] { return odit_attn_ruled(ptr(q), ptr(k), ptr(v), o.data_ptr(), B, Sq, Sk, H, Hkv, D, qs, ks, vs, os, static_cast<float>(scale), &r, dt,
+                                            w.stream); }) != 0)
+    return none();
+  return wrap(std::move(o));
+  NATIVE_END
+}
+
+// a paged cache's part: [pages, page, heads, D] with strides that the kernels take
+bool cache_operand(const Tensor& t) { return attn_operand(t) && t.size(0) < (1ll << 31) && t.size(1) > 0 && t.size(1) < (1ll << 30); }
+
+// (q, key_cache, value_cache, table, lengths, scale, window, cap, slopes, distance)
+PyObject* py_attn_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  NATIVE_BEGIN
+  const Tensor *q, *k, *v, *table, *len;
+  if (n != 10 || !(q = tensor_of(a[0])) || !(k = tensor_of(a[1])) || !(v = tensor_of(a[2])) || !(table = tensor_of(a[3])) || !(len = tensor_of(a[4])))
+    return none();
+  const double scale = PyFloat_AsDouble(a[5]);
+  if (PyErr_Occurred()) return nullptr;
+  const Where w;
+  for (const Tensor* t : {q, k, v, table, len})
+    if (!w.holds(t)) return none();
+  if (q->dim() != 3 || q->stride(2) != 1 || q->stride(0) % 8 != 0 || q->stride(1) % 8 != 0 || !aligned16(q->data_ptr()) || wants_grad({q, k, v})) return none();
+  const int dt = code_of(*q);
+  if ((dt != ODIT_BF16 && dt != ODIT_F16) || k->scalar_type() != q->scalar_type() || v->scalar_type() != q->scalar_type() || k->dim() != 4 ||
+      v->sizes() != k->sizes() || !cache_operand(*k) || !cache_operand(*v))
+    return none();
+  const int64_t B = q->size(0), H = q->size(1), D = q->size(2), pages = k->size(0), page = k->size(1), Hkv = k->size(2);
+  if (k->size(3) != D || B == 0 || pages == 0 || Hkv == 0 || table->scalar_type() != at::kInt || table->dim() != 2 || table->size(0) != B || table->size(1) == 0 ||
+      table->stride(1) != 1 || table->size(1) * page > (1ll << 30) || !dense(len, at::kInt, {B}) || B * H > (1ll << 30))
+    return none();
+  odit_attn_rules r;
+  const int ok = score_rules(nullptr, a[6], a[7], a[8], a[9], H, w, &r);
+  if (ok <= 0) return ok < 0 ? nullptr : none();
+  Tensor o = fresh({B, H, D}, q->options()), ws;
+  // (memory of the call's own, from the allocator: a captured graph then has its own too, and two of them can run side by side)
+  const size_t need = odit_attn_paged_workspace_bytes(B, H, Hkv, D, table->size(1), page, r.window);
+  if (need > 0) ws = fresh({static_cast<int64_t>(need)}, q->options().dtype(at::kByte));
+  const int64_t qs[2] = {q->stride(0), q->stride(1)}, ks[3] = {k->stride(0), k->stride(1), k->stride(2)}, vs[3] = {v->stride(0), v->stride(1), v->stride(2)},
+                os[2] = {H * D, D};
+  if (unlocked([&] { return odit_attn_paged(ptr(q), ptr(k), ptr(v), static_cast<const int*>(ptr(table)), static_cast<const int*>(ptr(len)), o.data_ptr(), B, H, Hkv, D,
+                                            pages, page, table->size(1), qs, ks, vs, table->stride(0), os, static_cast<float>(scale), &r, dt,
+                                            need > 0 ? ws.data_ptr() : nullptr, need, w.stream); }) != 0)
+    return none();
+  return wrap(std::move(o));
+  NATIVE_END
+}
+
+// (q, k, v, positions, turns, magnitude, flags, slots, key_cache, value_cache) -> (q, k or None)
+PyObject* py_rope_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  NATIVE_BEGIN
+  const Tensor *q, *k, *v, *pos, *turns, *slots, *kc, *vc;
+  if (n != 10 || !(q = tensor_of(a[0])) || !(k = tensor_of(a[1])) || !optional_tensor(a[2], &v) || !(pos = tensor_of(a[3])) || !(turns = tensor_of(a[4])) ||
+      !optional_tensor(a[7], &slots) || !optional_tensor(a[8], &kc) || !optional_tensor(a[9], &vc))
+    return none();
+  const double magnitude = PyFloat_AsDouble(a[5]);
+  const long flags = PyLong_AsLong(a[6]);
+  if (PyErr_Occurred()) return nullptr;
+  const Where w;
+  for (const Tensor* t : {q, k, v, pos, turns, slots, kc, vc})
+    if (!w.holds(t)) return none();
+  const bool cached = slots != nullptr;
+  if (cached != (v != nullptr) || cached != (kc != nullptr) || cached != (vc != nullptr) || wants_grad({q, k, v, turns, kc, vc})) return none();
+  const int dt = code_of(*q);
+  if (dt != ODIT_BF16 && dt != ODIT_F16) return none();
+  for (const Tensor* t : {q, k, v}) {
+    if (t && (t->dim() != 3 || t->scalar_type() != q->scalar_type() || t->size(0) != q->size(0) || t->size(2) != q->size(2) || t->stride(2) != 1 ||
+              t->stride(0) % 8 != 0 || t->stride(1) % 8 != 0 || !aligned16(t->data_ptr())))
+      return none();
+  }
+  const int64_t T = q->size(0), H = q->size(1), Hkv = k->size(1), D = q->size(2);
+  if (T == 0 || H == 0 || Hkv == 0 || H > 65536 || Hkv > 65536 || D > 1024 || !dense(pos, at::kLong, {T}) || !dense(turns, at::kDouble, {-1}) || turns->size(0) > 512 ||
+      !dense(slots, at::kLong, {T}) || (v && v->size(1) != Hkv))
+    return none();
+  if (cached && (kc->dim() != 4 || vc->sizes() != kc->sizes() || !cache_operand(*kc) || !cache_operand(*vc) || kc->scalar_type() != q->scalar_type() ||
+                 vc->scalar_type() != q->scalar_type() || kc->size(2) != Hkv || kc->size(3) != D))
+    return none();
+  Tensor qo = fresh({T, H, D}, q->options()), ko;
+  if (!cached) ko = fresh({T, Hkv, D}, q->options());
+  const int64_t qs[2] = {q->stride(0), q->stride(1)}, ks[2] = {k->stride(0), k->stride(1)};
+  int64_t vs[2] = {0, 0}, kcs[3] = {0, 0, 0}, vcs[3] = {0, 0, 0};
+  if (cached) {
+    vs[0] = v->stride(0); vs[1] = v->stride(1);
+    for (int i = 0; i < 3; ++i) { kcs[i] = kc->stride(i); vcs[i] = vc->stride(i); }
+  }
+  if (unlocked([&] { return odit_rope_append(ptr(q), ptr(k), ptr(v), static_cast<const int64_t*>(ptr(pos)), static_cast<const double*>(ptr(turns)), qo.data_ptr(),
+                                             cached ? nullptr : ko.data_ptr(), static_cast<const int64_t*>(ptr(slots)), ptr(kc), ptr(vc), T, H, Hkv, D,
+                                             2 * turns->size(0), cached ? kc->size(0) : 0, cached ? kc->size(1) : 1, qs, ks, vs, kcs, vcs,
+                                             static_cast<float>(magnitude), dt, static_cast<unsigned>(flags), w.stream); }) != 0)
+    return none();
+  if (!cached) return wrap2(std::move(qo), std::move(ko));
+  PyObject* out = PyTuple_New(2);
+  PyTuple_SET_ITEM(out, 0, wrap(std::move(qo)));
+  Py_INCREF(Py_None);
+  PyTuple_SET_ITEM(out, 1, Py_None);
+  return out;
   NATIVE_END
 }
 
@@ -2306,6 +2481,9 @@ PyMethodDef kMethods[] = {
     NATIVE_FN("own_tree", &py_own_tree),
     NATIVE_FN("rotary", &py_rotary),
     NATIVE_FN("attn", &py_attn),
+    NATIVE_FN("attn_ruled", &py_attn_ruled),
+    NATIVE_FN("attn_paged", &py_attn_paged),
+    NATIVE_FN("rope_append", &py_rope_append),
     NATIVE_FN("linear", &py_linear),
     NATIVE_FN("pair_is_small", &py_pair_is_small),
     NATIVE_FN("linear_few", &py_linear_few),

@@ -312,6 +312,222 @@ def _attn_scratch(device: int, stream: int, need: int) -> torch.Tensor:
     return _ATTN_SCRATCH.get(device, stream, need)
 
 
+# ------------------------------------------------------------------------- a text stage: prompts, and one token at a time
+def _inference_only(name: str, *tensors: torch.Tensor | None) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{name} has no backward pass: call it under torch.inference_mode() or torch.no_grad()")
+
+
+def _strided8(t: torch.Tensor) -> torch.Tensor:
+    """``t`` with a contiguous last axis, 16-byte alignment and strides that are multiples of 8: itself, or a copy."""
+    if t.stride(-1) == 1 and all(s % 8 == 0 for s in t.stride()[:-1]) and t.data_ptr() % 16 == 0:
+        return t
+    HIDDEN_COPIES["made_contiguous"] += 1
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _vector(name: str, t: torch.Tensor | None, dtype: torch.dtype, *shape: int) -> torch.Tensor | None:
+    """A small operand of this type and shape (-1: any size), made dense."""
+    if t is None:
+        return None
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.dim() != len(shape) or any(n >= 0 and n != m for n, m in zip(shape, t.shape)):
+        raise ValueError(f"{name}: expected shape {tuple('any' if n < 0 else n for n in shape)}, got {tuple(t.shape)}")
+    return t.contiguous()
+
+
+def _score_rules(causal, window, cap, slopes, distance, H: int):
+    """The ``odit_attn_rules`` that both attentions have, and the tensors that it points into."""
+    if window is not None and not 0 < int(window) <= 1 << 30:
+        raise ValueError(f"window={window} must be None or in [1, {1 << 30}]")
+    if not 0.0 <= float(cap) <= 8192.0:
+        raise ValueError(f"cap={cap} must be 0 (none) or up to 8192")
+    if slopes is not None and distance is not None:
+        raise ValueError("slopes and distance exclude each other")
+    slopes, distance = _vector("slopes", slopes, torch.float32, H), _vector("distance", distance, torch.float32, H, -1)
+    if distance is not None and (distance.shape[1] % 2 == 0 or distance.shape[1] > 2049):
+        raise ValueError(f"distance: expected [H, 2 R + 1] with R up to 1024, got {tuple(distance.shape)}")
+    return _lib.AttnRules(causal=int(bool(causal)), window=0 if window is None else int(window), cap=float(cap), slopes=_ptr(slopes),
+                          distance=_ptr(distance), radius=0 if distance is None else distance.shape[1] // 2), (slopes, distance)
+
+
+def _float16_pair(name: str, *tensors: torch.Tensor) -> None:
+    if any(t.dtype != tensors[0].dtype for t in tensors):
+        raise TypeError(f"{name}: tensors must share a dtype")
+    if tensors[0].dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"{name} takes bfloat16 and float16, got {tensors[0].dtype}")
+
+
+def attn_ruled(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    scale: float,
+    *,
+    causal: bool = False,
+    window: int | None = None,
+    prefix: torch.Tensor | None = None,
+    q_starts: torch.Tensor | None = None,
+    k_starts: torch.Tensor | None = None,
+    cap: float = 0.0,
+    slopes: torch.Tensor | None = None,
+    distance: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Attention of whole prompts, q [B,Sq,H,D] on k/v [B,Sk,Hkv,D] (bf16/fp16, D 64 or 128), under rules for scores and visibility.
+
+    A score is ``s = scale q.k``; with ``cap``, ``cap tanh(s / cap)``; then ``- slopes[h] |away|`` (``slopes`` float32 [H]) or
+    ``+ distance[h, clamp(away, -R, R) + R]`` (``distance`` float32 [H, 2 R + 1], R up to 1024), ``away`` being the key's position less the
+    query's. Each batch row is one document, or rows ``q_starts[n]:q_starts[n + 1]`` and keys ``k_starts[n]:k_starts[n + 1]`` are (int32
+    [N + 1], rising, on the GPU; every batch row is cut alike). A document's last query is at the place of its last key. ``causal`` hides the keys
+    behind the query, ``window`` those with ``|away| >= window``; the first ``prefix[n]`` keys of document n (int32 [N], or [B] without
+    documents) are seen in any case. A query that sees nothing, or is of no document, gets zeros; NaN and infinities in keys and values that
+    a query does not see do not reach it. Inference only."""
+    out = (_nat or _load_native()).attn_ruled(q, k, v, scale, causal, window, prefix, q_starts, k_starts, cap, slopes, distance)
+    if out is not None:
+        return out
+    _dev(q, k, v, prefix, q_starts, k_starts, slopes, distance)
+    _inference_only("attn_ruled", q, k, v, slopes, distance)
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+        raise ValueError("attn_ruled expects 4-D [B,S,H,D] tensors")
+    _float16_pair("attn_ruled", q, k, v)
+    B, Sq, H, D = q.shape
+    _, Sk, Hkv, _ = k.shape
+    if (k.shape[0], k.shape[3]) != (B, D) or v.shape != k.shape:
+        raise ValueError(f"shape mismatch: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
+    if (q_starts is None) != (k_starts is None):
+        raise ValueError("q_starts and k_starts come together")
+    q_starts = _vector("q_starts", q_starts, torch.int32, -1)
+    if q_starts is not None and q_starts.numel() < 2:
+        raise ValueError("q_starts and k_starts need a begin and an end for one document at least")
+    docs = 0 if q_starts is None else q_starts.numel() - 1
+    k_starts = _vector("k_starts", k_starts, torch.int32, docs + 1)
+    prefix = _vector("prefix", prefix, torch.int32, docs or B)
+    rules, held = _score_rules(causal, window, cap, slopes, distance, H)
+    rules.docs, rules.q_starts, rules.k_starts, rules.prefix = docs, _ptr(q_starts), _ptr(k_starts), _ptr(prefix)
+    q, k, v = _strided8(q), _strided8(k), _strided8(v)
+    o = torch.empty((B, Sq, H, D), dtype=q.dtype, device=q.device)
+    with torch.cuda.device(q.device):
+        rc = _lib.load().odit_attn_ruled(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), B, Sq, Sk, H, Hkv, D, _lib.i64_array(q.stride()[:3]),
+            _lib.i64_array(k.stride()[:3]), _lib.i64_array(v.stride()[:3]), _lib.i64_array((Sq * H * D, H * D, D)), float(scale),
+            _lib.C.byref(rules), _code(q), _stream())
+    _lib.check(rc, "odit_attn_ruled")
+    return o
+
+
+def _cache(name: str, t: torch.Tensor, Hkv: int | None, D: int, like: torch.Tensor) -> None:
+    """Checks of one part of a paged cache (which is never copied)."""
+    if t.dim() != 4 or (Hkv is not None and t.shape[2] != Hkv) or t.shape[3] != D or t.shape[1] == 0:
+        raise ValueError(f"{name}: expected [pages, page size, {'kv heads' if Hkv is None else Hkv}, {D}], got {tuple(t.shape)}")
+    if t.dtype != like.dtype:
+        raise TypeError(f"{name} must be {like.dtype}, got {t.dtype}")
+    if t.stride(3) != 1 or any(s % 8 for s in t.stride()[:3]) or t.data_ptr() % 16:
+        raise ValueError(f"{name}: the last axis must be contiguous, other strides multiples of 8, the memory 16-byte aligned")
+
+
+def attn_paged(
+    q: torch.Tensor,
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    table: torch.Tensor,
+    lengths: torch.Tensor,
+    scale: float,
+    *,
+    window: int | None = None,
+    cap: float = 0.0,
+    slopes: torch.Tensor | None = None,
+    distance: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Attention of one new token per sequence, q [B,H,D], over caches [pages, page size, Hkv, D] (bf16/fp16, D 64 or 128).
+
+    Key j of sequence b is row ``j % page size`` of page ``table[b, j // page size]``; the query stands at key ``lengths[b] - 1`` and sees
+    that one and all before it, or the last ``window`` of them. ``table`` int32 [B, most pages] and ``lengths`` int32 [B] are read on the GPU: lengths
+    are cut to what the table holds, a length of 0 gives zeros, keys on pages outside the cache are not seen, and cache rows that a sequence does
+    not have are not read. ``cap``, ``slopes`` and ``distance`` as in :func:`attn_ruled`. Inference only."""
+    out = (_nat or _load_native()).attn_paged(q, key_cache, value_cache, table, lengths, scale, window, cap, slopes, distance)
+    if out is not None:
+        return out
+    _dev(q, key_cache, value_cache, table, lengths, slopes, distance)
+    _inference_only("attn_paged", q, key_cache, value_cache, slopes, distance)
+    if q.dim() != 3:
+        raise ValueError(f"attn_paged expects q [B,H,D], got {tuple(q.shape)}")
+    _float16_pair("attn_paged", q)
+    B, H, D = q.shape
+    _cache("key_cache", key_cache, None, D, q)
+    pages, page, Hkv, _ = key_cache.shape
+    _cache("value_cache", value_cache, Hkv, D, q)
+    if value_cache.shape != key_cache.shape:
+        raise ValueError(f"shape mismatch: key_cache {tuple(key_cache.shape)}, value_cache {tuple(value_cache.shape)}")
+    table, lengths = _vector("table", table, torch.int32, B, -1), _vector("lengths", lengths, torch.int32, B)
+    rules, held = _score_rules(True, window, cap, slopes, distance, H)
+    q, n = _strided8(q), table.shape[1]
+    o = torch.empty((B, H, D), dtype=q.dtype, device=q.device)
+    lib = _lib.load()
+    need = int(lib.odit_attn_paged_workspace_bytes(B, H, Hkv, D, n, page, rules.window))
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    with torch.cuda.device(q.device):
+        rc = lib.odit_attn_paged(
+            q.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), table.data_ptr(), lengths.data_ptr(), o.data_ptr(), B, H, Hkv, D,
+            pages, page, n, _lib.i64_array(q.stride()[:2]), _lib.i64_array(key_cache.stride()[:3]), _lib.i64_array(value_cache.stride()[:3]),
+            n, _lib.i64_array((H * D, D)), float(scale), _lib.C.byref(rules), _code(q), _ptr(ws), need, _stream())
+    _lib.check(rc, "odit_attn_paged")
+    return o
+
+
+def rope_append(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor | None,
+    positions: torch.Tensor,
+    turns: torch.Tensor,
+    *,
+    neox: bool = True,
+    magnitude: float = 1.0,
+    slots: torch.Tensor | None = None,
+    key_cache: torch.Tensor | None = None,
+    value_cache: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """Rotary positions of packed tokens q [T,H,D], k [T,Hkv,D] (bf16/fp16), keys and values going into a paged cache.
+
+    Feature pair i of ``2 * len(turns)`` rotated features of each head is turned by ``positions[t] * turns[i]`` whole turns (``positions`` int64 [T],
+    ``turns`` float64: a frequency over 2 pi, stretched for long contexts as the model has it) and scaled by ``magnitude``; pairs are (i, i + rot / 2)
+    with ``neox``, else (2 i, 2 i + 1). Further features pass through. Returns the rotated (q, k), dense. With ``slots`` (int64 [T]) the rotated
+    keys and ``v`` [T,Hkv,D] go to row ``slots[t] % page size`` of page ``slots[t] // page size`` of the caches [pages, page size, Hkv, D] and
+    None comes back for k; a token whose slot lies outside the cache (-1: a padded one) is not stored. Slots are distinct. Inference only."""
+    out = (_nat or _load_native()).rope_append(q, k, v, positions, turns, magnitude, ODIT_FLAG_NEOX if neox else 0, slots, key_cache, value_cache)
+    if out is not None:
+        return out
+    _dev(q, k, v, positions, turns, slots, key_cache, value_cache)
+    _inference_only("rope_append", q, k, v, turns, key_cache, value_cache)
+    if len({t is None for t in (v, slots, key_cache, value_cache)}) != 1:
+        raise ValueError("rope_append takes v, slots, key_cache and value_cache together, or none of them")
+    if q.dim() != 3 or k.dim() != 3 or (k.shape[0], k.shape[2]) != (q.shape[0], q.shape[2]) or (v is not None and v.shape != k.shape):
+        raise ValueError(f"expected q [T,H,D] and k, v [T,Hkv,D], got {[None if t is None else tuple(t.shape) for t in (q, k, v)]}")
+    _float16_pair("rope_append", *(t for t in (q, k, v) if t is not None))
+    T, H, D = q.shape
+    Hkv = k.shape[1]
+    positions, turns = _vector("positions", positions, torch.int64, T), _vector("turns", turns, torch.float64, -1)
+    slots = _vector("slots", slots, torch.int64, T)
+    cached = slots is not None
+    if cached:
+        _cache("key_cache", key_cache, Hkv, D, q)
+        _cache("value_cache", value_cache, Hkv, D, q)
+        if value_cache.shape != key_cache.shape:
+            raise ValueError(f"shape mismatch: key_cache {tuple(key_cache.shape)}, value_cache {tuple(value_cache.shape)}")
+    q, k, v = _strided8(q), _strided8(k), None if v is None else _strided8(v)
+    q_out = torch.empty((T, H, D), dtype=q.dtype, device=q.device)
+    k_out = None if cached else torch.empty((T, Hkv, D), dtype=q.dtype, device=q.device)
+    strides = [_lib.i64_array(t.stride()[:n]) if t is not None else None for t, n in ((q, 2), (k, 2), (v, 2), (key_cache, 3), (value_cache, 3))]
+    with torch.cuda.device(q.device):
+        rc = _lib.load().odit_rope_append(
+            q.data_ptr(), k.data_ptr(), _ptr(v), positions.data_ptr(), turns.data_ptr(), q_out.data_ptr(), _ptr(k_out), _ptr(slots),
+            _ptr(key_cache), _ptr(value_cache), T, H, Hkv, D, 2 * turns.numel(), key_cache.shape[0] if cached else 0,
+            key_cache.shape[1] if cached else 1, *strides, float(magnitude), _code(q), ODIT_FLAG_NEOX if neox else 0, _stream())
+    _lib.check(rc, "odit_rope_append")
+    return q_out, k_out
+
+
 # --------------------------------------------------------------------------------------------- K2
 def qknorm_rope(
     q: torch.Tensor,
