@@ -417,8 +417,7 @@ extern "C" int odit_attn_paged(const void* q, const void* key_cache, const void*
   p.kc_p = key_cache_strides[0]; p.kc_r = key_cache_strides[1]; p.kc_h = key_cache_strides[2];
   p.vc_p = value_cache_strides[0]; p.vc_r = value_cache_strides[1]; p.vc_h = value_cache_strides[2];
   p.scale_log2 = scale * kLog2e;
-  p.cap.in = r.cap > 0.f ? 2.f * kLog2e * scale / r.cap : 0.f;
-  p.cap.out = r.cap * kLog2e;
+  p.cap = make_cap(r.cap, scale);
   p.group = H / Hkv; p.head_blocks = paged_head_blocks(H, Hkv);
   const int64_t units = static_cast<int64_t>(B) * Hkv * p.head_blocks;
   p.units = static_cast<int>(units);

@@ -28,20 +28,53 @@ struct RuledParams {
   int docs, causal, window, radius;  // docs 0: one document per batch row; window 0: none
   int B, Sq, Sk, H, Hkv;
   int64_t qs_b, qs_s, qs_h, ks_b, ks_s, ks_h, vs_b, vs_s, vs_h, os_b, os_s, os_h;
-  float scale_log2;
+  float scale_log2, bias_scale;  // scale log2(e) and 1 / scale
   Cap cap;
   int n_qblocks, units;  // units: heads of all batch rows
 };
 
-// the document of row r: the last one that starts at or before it (the search ends whatever the starts hold)
-__device__ __forceinline__ int doc_of(const int* starts, int docs, int r) {
-  int lo = 0, hi = docs;  // starts[lo] <= r < starts[hi], if anywhere
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (starts[mid] <= r) lo = mid; else hi = mid;
+// Among 64 documents from `base` on, whose starts the lanes hold: the last one that starts at or before the lane's row, one of the 32 from
+// row0 on; `doc` where there is none. *past: whether a later start lies behind all the rows.
+__device__ __forceinline__ int doc_among(int mine, int base, int row0, int row, int doc, bool* past) {
+  const uint64_t before = __ballot(mine <= row0);
+  bool end = false;
+  for (int i = before == 0 ? 0 : __popcll(before) - 1; i < 64 && !end; ++i) {
+    const int start = __builtin_amdgcn_readlane(mine, i);
+    end = start > row0 + 31;
+    if (start <= row) doc = base + i;
   }
-  return lo;
+  if (past != nullptr) *past = end;
+  return doc;
 }
+// The documents of 32 rows from row0 on, lane l's row being row0 + l % 32: the last one that starts at or before it. The wavefront reads 64
+// starts at a time: searches by halves would be log2(docs) dependent trips to memory.
+// (Whatever the starts hold, the search ends and stays inside them.)
+__device__ __forceinline__ int doc_of(const int* starts, int docs, int row0, int row) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, n = docs;  // the first row's document is one of [lo, lo + n)
+  while (n > 64) {
+    const int step = (n + 63) / 64, at = lane * step;
+    const uint64_t before = __ballot(at < n && starts[lo + (at < n ? at : 0)] <= row0);
+    const int skip = (before == 0 ? 0 : __popcll(before) - 1) * step;
+    lo += skip;
+    n = n - skip < step ? n - skip : step;
+  }
+  int doc = lo;
+  for (int base = lo; base < docs; base += 64) {
+    bool past;
+    doc = doc_among(base + lane < docs ? starts[base + lane] : 0x7fffffff, base, row0, row, doc, &past);
+    if (past) break;
+  }
+  return doc;
+}
+
+// of the 32 lanes of each half of a wavefront, which hold the same
+template <int CTRL> __device__ __forceinline__ int dpp_int(int v) { return __builtin_amdgcn_update_dpp(v, v, CTRL, 0xf, 0xf, false); }
+__device__ __forceinline__ int half_min(int v) {
+  v = min(v, dpp_int<0xB1>(v)); v = min(v, dpp_int<0x4E>(v)); v = min(v, dpp_int<0x141>(v)); v = min(v, dpp_int<0x140>(v));
+  return min(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16));
+}
+__device__ __forceinline__ int half_max(int v) { return ~half_min(~v); }
 
 __device__ __forceinline__ int clampi(int x, int lo, int hi) { return x < lo ? lo : x > hi ? hi : x; }
 
@@ -55,7 +88,7 @@ __device__ __forceinline__ uint64_t range_bits(int lo, int hi, int t0) {
 
 // BIAS 0: none, 1: slopes, 2: table
 template <typename T, int D, bool CAP, int BIAS>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 3 : 2, D == 64 ? 3 : 2)))
 void attn_ruled_kernel(const RuledParams p) {
   using M = Mma<T>;
   using frag = typename M::frag;
@@ -66,13 +99,17 @@ void attn_ruled_kernel(const RuledParams p) {
 
   __shared__ __attribute__((aligned(1024))) char lds[4 * TILEB];  // K0 K1 V0 V1
   __shared__ int bounds[NW][4];
-  __shared__ float table[BIAS == 2 ? 2 * kMaxRadius + 1 : 1];  // the head's biases in units of log2
+  __shared__ int places[BIAS != 0 ? BM : 1];  // pos of each lane's query
+  __shared__ int4 ranges[BM];  // blo, bhi, plo, phi of each lane's query: read again at each tile, which has no registers to hold them
+  // BIAS 2: the head's biases, with the outermost ones once more for each further key of a tile that some distance inside begins or ends
+  constexpr int kPad = BN - 1;
+  __shared__ float table[BIAS == 2 ? 2 * kMaxRadius + 1 + 2 * kPad : 1];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, hh = lane >> 5;
   // the last query blocks, which see most under a causal order, begin first; where the heads divide over the XCDs, an XCD keeps its heads
   int unit, qb;
-  if (p.units % kNumXcd == 0) {
+  if (BIAS != 1 && p.units % kNumXcd == 0) {
     const int per = p.units / kNumXcd, local = blockIdx.x / kNumXcd;
     unit = blockIdx.x % kNumXcd * per + local % per;
     qb = p.n_qblocks - 1 - local / per;
@@ -84,18 +121,58 @@ void attn_ruled_kernel(const RuledParams p) {
   const int q0 = qb * BM + wave * 32;
   const int row = q0 + l32 < p.Sq ? q0 + l32 : p.Sq - 1;
 
+  const T* const qrow = static_cast<const T*>(p.q) + b * p.qs_b + h * p.qs_h + row * p.qs_s;
+  frag qf[KS];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) qf[ks] = __builtin_bit_cast(frag, *reinterpret_cast<const u32x4_v*>(qrow + hh * 8 + ks * 16));
+  // (three workgroups to a compute unit: some fragments are read again at each tile, for want of a few registers)
+  constexpr int QL = D != 64 ? 0 : CAP && BIAS != 2 ? 4 : 2;
+  __shared__ u32x4_v q_lds[QL > 0 ? QL * NW * 64 : 1];
+  auto q_at = [&](int ks) __attribute__((always_inline)) {
+    if (ks >= QL) return qf[ks];
+    uint32_t from = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void_rp)(q_lds + ks * NW * 64 + tid)));
+    asm volatile("" : "+v"(from) : : "memory");  // (opaque, or the compiler keeps what was stored there in registers after all)
+    return __builtin_bit_cast(frag, *(__attribute__((address_space(3))) const u32x4_v*)(from));
+  };
+
+  // Biases join a product at its first addition, as the accumulator's first value, where a zero would stand otherwise: they cost nothing
+  // and are kept in units of products (x / scale). Behind a cap they are in units of log2.
+  const float bias_unit = CAP ? kLog2e : p.bias_scale;
+  if constexpr (BIAS == 2) {
+    const float* from = p.distance + static_cast<int64_t>(h) * (2 * p.radius + 1);
+    for (int i = tid; i <= 2 * p.radius + 2 * kPad; i += 256) table[i] = from[clampi(i - kPad, 0, 2 * p.radius)] * bias_unit;
+  }
+
   // ---- what this lane's query sees ----
+  constexpr int kNone = 0x7fffffff;
   int blo, bhi, plo = 0, phi = 0, pos;  // pos: the key at the query's own place
   {
-    int ks = 0, kn = p.Sk, qs = 0, qe = p.Sq, doc = b;
+    int ks = 0, kn = p.Sk, qs = 0, qe = p.Sq, doc = 0, prefix = 0;
     bool in = true;
     if (p.docs > 0) {
-      doc = doc_of(p.q_starts, p.docs, row);
-      qs = p.q_starts[doc];
-      qe = p.q_starts[doc + 1];
+      const int row0 = q0 < p.Sq ? q0 : p.Sq - 1;
+      if (p.docs < 64) {  // the lanes hold all starts: one trip to memory
+        const int at = lane <= p.docs ? lane : p.docs;
+        const int q_start = p.q_starts[at], k_start = p.k_starts[at], seen = p.prefix != nullptr ? p.prefix[min(at, p.docs - 1)] : 0;
+        doc = doc_among(lane < p.docs ? q_start : kNone, 0, row0, row, 0, nullptr);
+        qs = __shfl(q_start, doc, 64);
+        qe = __shfl(q_start, doc + 1, 64);
+        ks = __shfl(k_start, doc, 64);
+        kn = __shfl(k_start, doc + 1, 64);
+        prefix = __shfl(seen, doc, 64);
+      } else {
+        doc = doc_of(p.q_starts, p.docs, row0, row);
+        qs = p.q_starts[doc];
+        qe = p.q_starts[doc + 1];
+        ks = p.k_starts[doc];
+        kn = p.k_starts[doc + 1];
+        prefix = p.prefix != nullptr ? p.prefix[doc] : 0;
+      }
       in = row >= qs && row < qe;
-      ks = clampi(p.k_starts[doc], 0, p.Sk);
-      kn = clampi(p.k_starts[doc + 1], ks, p.Sk) - ks;
+      ks = clampi(ks, 0, p.Sk);
+      kn = clampi(kn, ks, p.Sk) - ks;
+    } else if (p.prefix != nullptr) {
+      prefix = p.prefix[b];
     }
     // the query's place from the document's first key (cut to what sums with a window keep in 32 bits, whatever the starts hold)
     constexpr int64_t kFar = (1 << 30) - 1;
@@ -104,25 +181,21 @@ void attn_ruled_kernel(const RuledParams p) {
     const int lo = p.window > 0 ? clampi(at - p.window + 1, 0, kn) : 0;
     const int hi = p.causal ? clampi(at + 1, 0, kn) : p.window > 0 ? clampi(at + p.window, 0, kn) : kn;
     pos = ks + at;
-    blo = ks + lo;
-    bhi = in && hi > lo ? ks + hi : blo;
-    if (p.prefix != nullptr && in) {
+    blo = in && hi > lo ? ks + lo : 0;  // (nothing: [0, 0))
+    bhi = in && hi > lo ? ks + hi : 0;
+    if (in && prefix > 0 && kn > 0) {
       plo = ks;
-      phi = ks + clampi(p.prefix[doc], 0, kn);
+      phi = ks + min(prefix, kn);
     }
   }
-  // the wavefront's ranges: from the smallest begin to the largest end, and what all of its queries see
-  auto wave_min = [](int x) { for (int s = 1; s < 64; s <<= 1) { const int y = __shfl_xor(x, s, 64); x = y < x ? y : x; } return __builtin_amdgcn_readfirstlane(x); };
-  auto wave_max = [](int x) { for (int s = 1; s < 64; s <<= 1) { const int y = __shfl_xor(x, s, 64); x = y > x ? y : x; } return __builtin_amdgcn_readfirstlane(x); };
-  constexpr int kNone = 0x7fffffff;
-  const int b_first = wave_min(bhi > blo ? blo : kNone), b_end = wave_max(bhi > blo ? bhi : 0);
-  const int p_first = wave_min(phi > plo ? plo : kNone), p_end = wave_max(phi > plo ? phi : 0);
-  const int b_all0 = wave_max(blo), b_all1 = wave_min(bhi), p_all0 = wave_max(plo), p_all1 = wave_min(phi);
-  const int pos_min = wave_min(pos), pos_max = wave_max(pos);
-  if (lane == 0) { bounds[wave][0] = b_first; bounds[wave][1] = b_end; bounds[wave][2] = p_first; bounds[wave][3] = p_end; }
-  if constexpr (BIAS == 2) {
-    const float* from = p.distance + static_cast<int64_t>(h) * (2 * p.radius + 1);
-    for (int i = tid; i <= 2 * p.radius; i += 256) table[i] = from[i] * kLog2e;
+  int all0, all1;  // the keys that all queries of the wavefront have in their bands (none: all1 <= all0)
+  {
+    const int b0 = half_min(bhi > 0 ? blo : kNone), b1 = half_max(bhi), p0 = half_min(phi > 0 ? plo : kNone), p1 = half_max(phi);
+    all0 = half_max(blo);
+    all1 = half_min(bhi);
+    if (hh == 0) ranges[wave * 32 + l32] = make_int4(blo, bhi, plo, phi);
+    if (BIAS != 0 && hh == 0) places[wave * 32 + l32] = pos;
+    if (lane == 0) { bounds[wave][0] = b0; bounds[wave][1] = b1; bounds[wave][2] = p0; bounds[wave][3] = p1; }
   }
   __syncthreads();
   // the workgroup's tiles: up to two runs
@@ -143,46 +216,43 @@ void attn_ruled_kernel(const RuledParams p) {
     s2 = __builtin_amdgcn_readfirstlane(c0); n2 = __builtin_amdgcn_readfirstlane(c1 - c0);
   }
   const int n_tiles = n1 + n2;
-  auto tile_at = [&](int i) { return i < n1 ? s1 + i : s2 + i - n1; };
+  // From the last key back: under a causal order the nearest keys come first. Where distance takes from the scores, the running maximum is
+  // then near its end from the first tile on (slopes at 16384 tokens, 16 heads: 1203 us forwards, @@ backwards).
+  auto tile_at = [&](int i) { return n_tiles - 1 - i < n1 ? s1 + n_tiles - 1 - i : s2 + n_tiles - 1 - i - n1; };
 
   // ---- tile loads: as in attn_fwd_dma.hip, but with a buffer descriptor for each tile, so that offsets stay small in any tensor ----
   const T* const kbase = static_cast<const T*>(p.k) + b * p.ks_b + hkv * p.ks_h;
   const T* const vbase = static_cast<const T*>(p.v) + b * p.vs_b + hkv * p.vs_h;
   const int r0 = wave * IPW * RPI + lane / CPR, pc0 = lane % CPR;
-  uint32_t kvoff[IPW], vvoff[IPW];
-#pragma unroll
-  for (int i = 0; i < IPW; ++i) {
-    const int r = r0 + RPI * i;
-    kvoff[i] = static_cast<uint32_t>(r * p.ks_s * 2) + static_cast<uint32_t>(((pc0 ^ (r % 16)) % CPR) * 16);
-    vvoff[i] = static_cast<uint32_t>(r * p.vs_s * 2) + static_cast<uint32_t>(((pc0 ^ (4 * (r % 4))) % CPR) * 16);
-  }
+  // Byte offsets of the lane's first instruction; the others' rows lie a whole number of rows further down, which is the load's scalar
+  // offset. Their swizzle is the same, but for keys of head size 128, where it differs by a constant.
+  const uint32_t krow = static_cast<uint32_t>(r0 * p.ks_s * 2), kswz = static_cast<uint32_t>(((pc0 ^ (r0 % 16)) % CPR) * 16);
+  const uint32_t vvoff = static_cast<uint32_t>(r0 * p.vs_s * 2) + static_cast<uint32_t>(((pc0 ^ (4 * (r0 % 4))) % CPR) * 16);
   const uint32_t lds_base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void_rp)lds));
-  auto load_tile = [&](const T* base, int64_t stride, const uint32_t(&off)[IPW], int t, int dst) {
+  auto load_tile = [&](const T* base, int64_t stride, bool keys, int t, int dst) __attribute__((always_inline)) {
     const uint64_t a = reinterpret_cast<uint64_t>(base + static_cast<int64_t>(t) * BN * stride);
     const int rows = min(BN, p.Sk - t * BN);  // rows behind the last key read as zeros
     u32x4_v r;
     r.x = static_cast<uint32_t>(a); r.y = static_cast<uint32_t>(a >> 32) & 0xffffu;
     r.z = static_cast<uint32_t>(((rows - 1) * stride + D) * 2); r.w = 0x00020000u;
+    uint32_t row = keys ? krow : vvoff, swz = keys ? kswz : 0;
+    asm volatile("" : "+v"(swz));  // (the sums are formed here, not held in registers across the loop)
 #pragma unroll
-    for (int i = 0; i < IPW; ++i) load_lds16(lds_base + dst + (wave * IPW + i) * 1024, off[i], r, 0);
+    for (int i = 0; i < IPW; ++i)
+      load_lds16(lds_base + dst + (wave * IPW + i) * 1024, row + (keys ? swz ^ static_cast<uint32_t>((RPI * i) % 16 % CPR * 16) : 0), r,
+                 static_cast<uint32_t>(RPI * i * stride * 2));
   };
-  auto load_k = [&](int i) { load_tile(kbase, p.ks_s, kvoff, tile_at(i), (i & 1) * TILEB); };
-  auto load_v = [&](int i) { load_tile(vbase, p.vs_s, vvoff, tile_at(i), (2 + (i & 1)) * TILEB); };
-
-  const T* const qrow = static_cast<const T*>(p.q) + b * p.qs_b + h * p.qs_h + row * p.qs_s;
-  frag qf[KS];
-#pragma unroll
-  for (int ks = 0; ks < KS; ++ks) qf[ks] = __builtin_bit_cast(frag, *reinterpret_cast<const u32x4_v*>(qrow + hh * 8 + ks * 16));
+  auto load_k = [&](int i, const int buf) { load_tile(kbase, p.ks_s, true, tile_at(i), buf * TILEB); };
+  auto load_v = [&](int i, const int buf) { load_tile(vbase, p.vs_s, false, tile_at(i), (2 + buf) * TILEB); };
 
   f32x16_v o[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[dt][e] = 0.f;
-  constexpr bool MADE = CAP || BIAS != 0;  // scores are turned into units of log2 before their maximum is taken
-  const float c = MADE ? 1.f : p.scale_log2;
+  const float c = CAP ? 1.f : p.scale_log2;  // from what m_run is in to units of log2
   float m_run = -INFINITY, l_run = 0.f, mc = 0.f;
-  const float slope = BIAS == 1 ? p.slopes[h] * kLog2e : 0.f;
+  const float slope = BIAS == 1 ? p.slopes[h] * bias_unit : 0.f;
 
   const int k_lane = l32 * ROWB + (((hh ^ (l32 % 16)) % CPR) << 4);
   const int sq = (lane & 15) >> 2, dh = (lane >> 4) & 1;
@@ -192,96 +262,242 @@ void attn_ruled_kernel(const RuledParams p) {
     return __uint_as_float(hh ? r[0] : r[1]);
   };
 
-  // bias of key `key` for this lane's query, and the whole way from a product to units of log2
-  auto made = [&](float s, int key) __attribute__((always_inline)) {
-    float x = CAP ? p.cap(s) : s * p.scale_log2;
-    if constexpr (BIAS == 1) x = fmaf(-slope, fabsf(static_cast<float>(key - pos)), x);
-    if constexpr (BIAS == 2) x += table[clampi(key - pos, -p.radius, p.radius) + p.radius];
-    return x;
+  constexpr bool POLY = CAP && BIAS == 0;
+  // the score of a key that is not seen (POLY: finite, as are all capped ones, for the polynomial 1 + 0 s^2 + ..; its exp2 is zero all the same)
+  const float kOut = POLY ? -1e18f : -INFINITY;
+  // whether some query of the wavefront sees a key of the tile from t0 on, and whether all of them see all
+  auto own = [&]() __attribute__((always_inline)) { return ranges[wave * 32 + l32]; };
+  auto some_see = [&](int t0) {
+    if (t0 >= all0 && t0 + BN <= all1) return true;  // (most tiles of a long prompt)
+    const int4 r = own();
+    return __any((t0 < r.y && t0 + BN > r.x) || (t0 < r.w && t0 + BN > r.z)) != 0;
+  };
+  auto all_see = [&](int t0) {
+    if (t0 >= all0 && t0 + BN <= all1) return true;
+    const int4 r = own();
+    return __all((t0 >= r.x && t0 + BN <= r.y) || (t0 >= r.z && t0 + BN <= r.w)) != 0;
+  };
+  constexpr auto key_of = [](int e) { return (e >> 4) * 32 + ((e & 15) >> 2) * 8 + (e & 3); };  // of the lane's score e: t0 + key_of(e) + 4 hh
+
+  // biases of the lane's keys of the tile from t0 on
+  auto biases = [&](int t0, f32x16_v(&s)[2]) __attribute__((always_inline)) {
+    const int pos = places[wave * 32 + l32], first = t0 + 4 * hh - pos;
+    if constexpr (BIAS == 1) {
+      const float at = static_cast<float>(first);
+      const bool before = __all(t0 + BN - 1 <= pos), behind = __all(t0 >= pos);
+      if (before || behind) {  // (linear: one instruction each)
+        const float sl = before ? slope : -slope, b0 = sl * at;
+#pragma unroll
+        for (int e = 0; e < 32; ++e) s[e >> 4][e & 15] = fmaf(sl, static_cast<float>(key_of(e)), b0);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          s[e >> 4][e & 15] = -slope * fabsf(at + static_cast<float>(key_of(e)));
+          if (e % 8 == 7) __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+    } else {
+      const bool before = __all(t0 + BN - 1 - pos <= -p.radius), behind = __all(t0 - pos >= p.radius);
+      if (before || behind) {
+        const float far = table[before ? 0 : 2 * p.radius + 2 * kPad];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) s[e >> 4][e & 15] = far;
+      } else {
+        const float* const from = table + clampi(first, -p.radius - kPad, p.radius) + p.radius + kPad;
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          s[e >> 4][e & 15] = from[key_of(e)];
+          if (e % 8 == 7) __builtin_amdgcn_sched_barrier(0);  // (not all at once: there are no registers for it)
+        }
+      }
+    }
+  };
+  auto first_values = [&](int t0, f32x16_v(&s)[2]) __attribute__((always_inline)) {
+    if constexpr (BIAS != 0 && !CAP) {
+      biases(t0, s);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 32; ++e) s[e >> 4][e & 15] = 0.f;
+    }
+  };
+  auto lane_max = [&](const f32x16_v(&s)[2]) __attribute__((always_inline)) {
+    float mx = s[0][0];
+#pragma unroll
+    for (int e = 1; e < 32; ++e) mx = __builtin_elementwise_maximum(mx, s[e >> 4][e & 15]);
+    return mx;
+  };
+  // Behind the products: the cap by its own formula and the biases behind it (CAP, unless the tile's scores stay as they are: see below),
+  // keys that some query does not see; returns the lane's maximum
+  auto finish_scores = [&](int t0, bool all, f32x16_v(&s)[2]) {
+    if constexpr (CAP) {
+      f32x16_v add[2];
+      if constexpr (BIAS != 0) biases(t0, add);
+#pragma unroll
+      for (int e = 0; e < 32; ++e) {
+        s[e >> 4][e & 15] = p.cap(s[e >> 4][e & 15]) + (BIAS != 0 ? add[e >> 4][e & 15] : 0.f);
+        if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    if (!all) {
+      const int4 r = own();
+      const uint64_t w = range_bits(r.x, r.y, t0) | range_bits(r.z, r.w, t0);
+      const uint32_t half[2] = {static_cast<uint32_t>(w) >> (4 * hh), static_cast<uint32_t>(w >> 32) >> (4 * hh)};
+#pragma unroll
+      for (int e = 0; e < 32; ++e) s[e >> 4][e & 15] = (half[e >> 4] & (1u << (key_of(e) & 31))) ? s[e >> 4][e & 15] : kOut;
+    }
+    const float mx = lane_max(s);
+    return POLY && mx == kOut ? -INFINITY : mx;
+  };
+  auto settle_max = [&](float mx) __attribute__((always_inline)) {
+    if (__any((mx - m_run) * c > 8.f)) {
+      const float m_new = fmaxf(m_run, fmaxf(mx, swapped(mx)));
+      const float m_safe = m_new == -INFINITY ? 0.f : m_new;
+      const float alpha = __builtin_amdgcn_exp2f((m_run - m_safe) * c);
+      l_run *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[dt][e] *= alpha;
+      m_run = m_new;
+      mc = m_safe * c;
+    }
+  };
+
+  // Tile i of the workgroup: its probabilities from s_cur while the next tile's products are formed (stage A), then its part of the output
+  // while the next scores' maximum is taken (stage B). `buf` is i % 2, a literal at every call.
+  // With a cap and no bias, scores that all queries see and that are small against the cap stay products until stage A, where the cap's
+  // polynomial is part of the exponent: the tanh rises, so their maximum is the capped ones'. Other tiles' scores are made at once
+  // (finish_scores), and their polynomial is the score itself.
+  bool seen = false, live = false;  // tile i: seen by some query of this wavefront (s_cur holds its scores), with some weight
+  float c0 = 1.f, c1 = 0.f, c2 = 0.f, c3 = 0.f;  // POLY: of s_cur
+  auto k_at = [&](const char* kb, int i) { return *reinterpret_cast<const u32x4_v*>(kb + (i & 1) * 32 * ROWB + (k_lane ^ ((i >> 1) * 32))); };
+  auto tile = [&](int i, const int buf, f32x16_v(&s_cur)[2], f32x16_v(&s_next)[2]) {
+    const bool has_next = i + 1 < n_tiles;
+    if (i + 2 < n_tiles) load_k(i + 2, buf);
+    if (has_next) load_v(i + 1, buf ^ 1);
+    const int tn = has_next ? tile_at(i + 1) * BN : 0;
+    const bool seen_next = has_next && some_see(tn);
+    float mx = -INFINITY, most = 0.f;  // the next scores' maximum and their sizes', of this lane
+    if (seen || seen_next) {
+      // Everything of a tile in one piece: branches around its parts would have the scores of both their ways brought together by copies
+      // (32 at every tile, 10 % of a long prompt). So the next products are formed where nothing of them is seen, and probabilities of
+      // scores that do not count (`live` says so), once each at the ends of a run of tiles.
+      uint32_t pf[2][2][4];
+      float sum = 0.f;
+      auto exponent = [&](float s) __attribute__((always_inline)) {
+        if constexpr (!POLY) return fmaf(s, c, -mc);
+        const float z = s * s;
+        return fmaf(s, fmaf(z, fmaf(z, fmaf(z, c3, c2), c1), c0), -mc);
+      };
+      auto probabilities = [&](int pi) __attribute__((always_inline)) {
+        const int kt = pi >> 3, e = (pi & 7) * 2;
+        const float p0 = __builtin_amdgcn_exp2f(exponent(s_cur[kt][e])), p1 = __builtin_amdgcn_exp2f(exponent(s_cur[kt][e + 1]));
+        sum += p0 + p1;
+        pf[kt][(pi & 7) >> 2][pi & 3] = M::pack2(p0, p1);
+      };
+      __builtin_amdgcn_s_setprio(2);
+      const char* const kb = lds + (buf ^ 1) * TILEB;
+      first_values(tn, s_next);
+      constexpr int KPF = CAP || D == 64 ? 2 : 3;  // fragments on their way ahead of the instruction that takes them
+      u32x4_v kfr[KPF + 1];
+#pragma unroll
+      for (int n = 0; n < KPF; ++n) kfr[n] = k_at(kb, n);
+      frag qn = q_at(0);
+#pragma unroll
+      for (int n = 0; n < 2 * KS; ++n) {
+        if (n + KPF < 2 * KS) kfr[(n + KPF) % (KPF + 1)] = k_at(kb, n + KPF);
+        s_next[n & 1] = M::run(__builtin_bit_cast(frag, kfr[n % (KPF + 1)]), qn, s_next[n & 1]);
+        if ((n & 1) && n + 1 < 2 * KS) qn = q_at((n + 1) >> 1);
+        constexpr int EACH = 16 / (2 * KS);
+#pragma unroll
+        for (int m = 0; m < EACH; ++m) probabilities(n * EACH + m);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      __builtin_amdgcn_s_setprio(0);
+      auto max_step = [&](int e) __attribute__((always_inline)) {
+        const float x0 = s_next[e >> 4][e & 15], x1 = s_next[e >> 4][(e + 1) & 15];
+        mx = __builtin_elementwise_maximum(__builtin_elementwise_maximum(mx, x0), x1);
+        if constexpr (CAP) most = __builtin_elementwise_maximum(__builtin_elementwise_maximum(most, fabsf(x0)), fabsf(x1));
+      };
+      if (live) {
+        l_run += sum;
+        const char* const vb = lds + (2 + buf) * TILEB;
+        constexpr int NSTEP = 4 * DT, VPF = CAP || D == 64 ? 2 : 3, EACH = 32 / NSTEP;
+        s16x4_r vlo[VPF + 1], vhi[VPF + 1];
+        auto v_fetch = [&](int st) {
+          const char* const vp = vb + (st / DT) * 16 * ROWB + (v_lane ^ ((st % DT * 64) % ROWB));
+          vlo[st % (VPF + 1)] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_rp)(vp));
+          vhi[st % (VPF + 1)] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_rp)(vp + 8 * ROWB));
+        };
+#pragma unroll
+        for (int st = 0; st < VPF; ++st) v_fetch(st);
+#pragma unroll
+        for (int st = 0; st < NSTEP; ++st) {
+          if (st + VPF < NSTEP) v_fetch(st + VPF);
+          const int dt = st % DT, kt = (st / DT) >> 1, g = (st / DT) & 1;
+          u32x4_v pb;
+          pb.x = pf[kt][g][0]; pb.y = pf[kt][g][1]; pb.z = pf[kt][g][2]; pb.w = pf[kt][g][3];
+          o[dt] = M::run(__builtin_bit_cast(frag, __builtin_shufflevector(vlo[st % (VPF + 1)], vhi[st % (VPF + 1)], 0, 1, 2, 3, 4, 5, 6, 7)),
+                         __builtin_bit_cast(frag, pb), o[dt]);
+          if constexpr (!CAP || BIAS == 0) {
+#pragma unroll
+            for (int e = st * EACH; e < st * EACH + EACH; e += 2) max_step(e);
+            asm volatile("" : "+v"(mx));  // (where it is: it would sink below the test behind the loop otherwise)
+            if constexpr (CAP) asm volatile("" : "+v"(most));
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      } else if constexpr (!CAP || BIAS == 0) {
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) max_step(e);
+      }
+      if (seen_next) {  // the next scores made ready, as far as they are not
+        const bool all = all_see(tn);
+        if constexpr (POLY) {
+          const bool small = all && __all(most < p.cap.few);
+          if (small) mx = p.cap(mx);
+          else mx = finish_scores(tn, all, s_next);
+          c0 = small ? p.cap.c0 : 1.f;
+          c1 = small ? p.cap.c1 : 0.f;
+          c2 = small ? p.cap.c2 : 0.f;
+          c3 = small ? p.cap.c3 : 0.f;
+        } else if (CAP || !all) {
+          mx = finish_scores(tn, all, s_next);
+        }
+      }
+    }
+    if (!seen_next) mx = -INFINITY;
+    __builtin_amdgcn_s_waitcnt(0);  // this wavefront's tile loads have landed
+    __syncthreads();
+    settle_max(mx);
+    seen = seen_next;
+    // (with biases, scores may lie so far below that all of a tile's probabilities are zero in 32 bits: nothing to add)
+    live = seen_next && (BIAS == 0 || __any(!((mx - m_run) * c < -150.f)));
   };
 
   if (n_tiles > 0) {
-    load_k(0);
-    load_v(0);
-  }
-  __builtin_amdgcn_s_waitcnt(0);
-  __syncthreads();
-  for (int i = 0; i < n_tiles; ++i) {
-    const int buf = i & 1, t0 = tile_at(i) * BN;
-    if (i + 1 < n_tiles) {
-      load_k(i + 1);
-      load_v(i + 1);
-    }
-    if ((t0 < b_end && t0 + BN > b_first) || (t0 < p_end && t0 + BN > p_first)) {  // (wave-uniform) some query sees some key
-      f32x16_v s[2];
+    load_k(0, 0);
+    load_v(0, 0);
+    if (n_tiles > 1) load_k(1, 1);
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) s[kt][e] = 0.f;
-      const char* kb = lds + buf * TILEB;
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-          s[kt] = M::run(__builtin_bit_cast(frag, *reinterpret_cast<const u32x4_v*>(kb + kt * 32 * ROWB + (k_lane ^ (ks * 32)))), qf[ks], s[kt]);
-      if constexpr (MADE) {
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) s[kt][e] = made(s[kt][e], t0 + kt * 32 + (e >> 2) * 8 + hh * 4 + (e & 3));
-      }
-      if (!((t0 >= b_all0 && t0 + BN <= b_all1) || (t0 >= p_all0 && t0 + BN <= p_all1))) {
-        const uint64_t w = range_bits(blo, bhi, t0) | range_bits(plo, phi, t0);
-        const uint32_t half[2] = {static_cast<uint32_t>(w) >> (4 * hh), static_cast<uint32_t>(w >> 32) >> (4 * hh)};
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) s[kt][e] = (half[kt] & (1u << ((e >> 2) * 8 + (e & 3)))) ? s[kt][e] : -INFINITY;
-      }
-      float mx = s[0][0];
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) mx = __builtin_elementwise_maximum(mx, s[kt][e]);
-      if (__any((mx - m_run) * c > 8.f)) {
-        const float m_new = fmaxf(m_run, fmaxf(mx, swapped(mx)));
-        const float m_safe = m_new == -INFINITY ? 0.f : m_new;
-        const float alpha = __builtin_amdgcn_exp2f((m_run - m_safe) * c);
-        l_run *= alpha;
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) o[dt][e] *= alpha;
-        m_run = m_new;
-        mc = m_safe * c;
-      }
-      uint32_t pf[2][2][4];
-      float sum = 0.f;
-#pragma unroll
-      for (int pi = 0; pi < 16; ++pi) {
-        const int kt = pi >> 3, e = (pi & 7) * 2;
-        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[kt][e], c, -mc)), p1 = __builtin_amdgcn_exp2f(fmaf(s[kt][e + 1], c, -mc));
-        sum += p0 + p1;
-        pf[kt][(pi & 7) >> 2][pi & 3] = M::pack2(p0, p1);
-      }
-      l_run += sum;
-      const char* vb = lds + (2 + buf) * TILEB;
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-        for (int g = 0; g < 2; ++g)
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt) {
-            const char* vp = vb + (kt * 32 + g * 16) * ROWB + (v_lane ^ ((dt * 64) % ROWB));
-            const s16x4_r lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_rp)(vp));
-            const s16x4_r hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_rp)(vp + 8 * ROWB));
-            u32x4_v pb;
-            pb.x = pf[kt][g][0]; pb.y = pf[kt][g][1]; pb.z = pf[kt][g][2]; pb.w = pf[kt][g][3];
-            o[dt] = M::run(__builtin_bit_cast(frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7)), __builtin_bit_cast(frag, pb), o[dt]);
-          }
-    }
-    __builtin_amdgcn_s_waitcnt(0);  // the next tile has landed
+    for (int ks = 0; ks < QL; ++ks) q_lds[ks * NW * 64 + tid] = __builtin_bit_cast(u32x4_v, qf[ks]);
+    __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
+    f32x16_v sa[2], sb[2];
+    {
+      const int t0 = tile_at(0) * BN;
+      seen = some_see(t0);
+      first_values(t0, sa);
+#pragma unroll
+      for (int i = 0; i < 2 * KS; ++i) sa[i & 1] = M::run(__builtin_bit_cast(frag, k_at(lds, i)), q_at(i >> 1), sa[i & 1]);
+      settle_max(finish_scores(t0, all_see(t0), sa));
+      live = seen;
+    }
+    __syncthreads();  // (the loop's first load goes where the first keys were)
+    for (int i = 0; i < n_tiles; i += 2) {
+      tile(i, 0, sa, sb);
+      if (i + 1 < n_tiles) tile(i + 1, 1, sb, sa);
+    }
   }
 
   // ---- epilogue ----
@@ -314,9 +530,9 @@ void attn_ruled_kernel(const RuledParams p) {
   while (bad != 0) {  // (wave-uniform)
     const int who = __builtin_ctzll(bad);
     bad &= bad - 1;
-    const int r = q0 + who, at = __builtin_amdgcn_readlane(pos, who);
-    const int from[2] = {__builtin_amdgcn_readlane(blo, who), __builtin_amdgcn_readlane(plo, who)};
-    const int to[2] = {__builtin_amdgcn_readlane(bhi, who), __builtin_amdgcn_readlane(phi, who)};
+    const int r = q0 + who, at = BIAS != 0 ? places[wave * 32 + who] : 0;
+    const int4 its = ranges[wave * 32 + who];
+    const int from[2] = {its.x, its.z}, to[2] = {its.y, its.w};
     const T* const qp = static_cast<const T*>(p.q) + b * p.qs_b + h * p.qs_h + r * p.qs_s;
     float m = -INFINITY, l = 0.f, acc[D / 64] = {};
     for (int range = 0; range < 2; ++range)
@@ -332,9 +548,10 @@ void attn_ruled_kernel(const RuledParams p) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) s = fmaf(Raw<T>::get(qv, e), Raw<T>::get(kv, e), s);
           }
-          x = CAP ? p.cap(s) : s * p.scale_log2;
-          if constexpr (BIAS == 1) x = fmaf(-slope, fabsf(static_cast<float>(key - at)), x);
-          if constexpr (BIAS == 2) x += table[clampi(key - at, -p.radius, p.radius) + p.radius];
+          float bias = 0.f;
+          if constexpr (BIAS == 1) bias = -slope * fabsf(static_cast<float>(key - at));
+          if constexpr (BIAS == 2) bias = table[clampi(key - at, -p.radius, p.radius) + p.radius + kPad];
+          x = CAP ? p.cap(s) + bias : (s + bias) * p.scale_log2;
         }
         float mx = x;
         for (int sft = 1; sft < 64; sft <<= 1) mx = fmaxf(mx, __shfl_xor(mx, sft, 64));
@@ -422,8 +639,8 @@ extern "C" int odit_attn_ruled(const void* q, const void* k, const void* v, void
   p.vs_b = v_strides[0]; p.vs_s = v_strides[1]; p.vs_h = v_strides[2];
   p.os_b = o_strides[0]; p.os_s = o_strides[1]; p.os_h = o_strides[2];
   p.scale_log2 = scale * kLog2e;
-  p.cap.in = r.cap > 0.f ? 2.f * kLog2e * scale / r.cap : 0.f;
-  p.cap.out = r.cap * kLog2e;
+  p.bias_scale = 1.f / scale;
+  p.cap = make_cap(r.cap, scale);
   const int bias = r.slopes != nullptr ? 1 : r.distance != nullptr ? 2 : 0;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == ODIT_BF16) return D == 128 ? launch_ruled<bf16_t, 128>(p, r.cap > 0.f, bias, st) : launch_ruled<bf16_t, 64>(p, r.cap > 0.f, bias, st);
