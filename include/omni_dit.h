@@ -97,10 +97,13 @@ typedef struct odit_attn_rules {
 
 /* o = softmax(rules(q k^T)) v over whole prompts: q [B,Sq,H,D], k, v [B,Sk,Hkv,D], o [B,Sq,H,D] with strides as in odit_attn_fwd, bf16 or
  * fp16, D 64 or 128. Documents cut every batch row alike. A query that sees nothing gets zeros; what keys and values hold that a query does
- * not see (NaN and infinities too) does not reach it. */
+ * not see (NaN and infinities too) does not reach it.
+ * `workspace`: NULL, or odit_attn_ruled_workspace_bytes for the same shape and rules (may be 0; no device memory is read for it), contents
+ * irrelevant before and after: few rows' long keys are then cut into ranges that run side by side and are joined by a second launch. */
 int odit_attn_ruled(const void* q, const void* k, const void* v, void* o, int B, int Sq, int Sk, int H, int Hkv, int D,
                     const int64_t q_strides[3], const int64_t k_strides[3], const int64_t v_strides[3], const int64_t o_strides[3],
-                    float scale, const odit_attn_rules* rules, int dtype, void* stream);
+                    float scale, const odit_attn_rules* rules, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+size_t odit_attn_ruled_workspace_bytes(int B, int Sq, int Sk, int H, int D, const odit_attn_rules* rules);
 
 /* The same for one new token per sequence, q and o [B,H,D] (strides for batch and head), over a paged cache: key and value caches
  * [pages,page_size,Hkv,D] (strides for page, row and head, multiples of 8), table int32 [B,max_pages] (row stride table_stride) of pages,

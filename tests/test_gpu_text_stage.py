@@ -160,6 +160,41 @@ def test_biases_that_forbid(gpu):
     _check_ruled(q[:, :, :1], k[:, :, :1], v[:, :, :1], o[:, :, :1], 0.1, dict(causal=True, window=2), {}, 0.0)
 
 
+@pytest.mark.parametrize("Sq,Sk,rules", [
+    (1, 4000, {}), (5, 3001, dict(causal=True)), (70, 2500, dict(causal=True, window=1900, prefix=[300])), (3, 2000, dict(window=700)),
+    (60, 2600, dict(q_starts=[0, 3, 50], k_starts=[0, 1300, 2590], causal=True)), (130, 2100, dict(causal=True, prefix=[2100]))], ids=str)
+@pytest.mark.parametrize("cap,kind,D,dtype", [(0.0, "", 128, BF16), (5.0, "", 64, F16), (0.0, "slopes", 64, BF16), (3.0, "table", 128, F16)])
+def test_few_rows_of_many_keys(gpu, Sq, Sk, rules, cap, kind, D, dtype):
+    """Calls whose keys are cut into ranges that run side by side."""
+    q, k, v = _randn(40, 1, Sq, 2, D, dtype=dtype, std=2), _randn(41, 1, Sk, 1, D, dtype=dtype), _randn(42, 1, Sk, 1, D, dtype=dtype)
+    bias = _bias(kind, 2, 43, 200)
+    _check_ruled(q, k, v, _ruled(q, k, v, 0.1, rules, bias, cap), 0.1, rules, bias, cap)
+    if "q_starts" in rules:  # what no query sees spoils no range's sum
+        k[0, 2590:], v[0, 2590:], v[0, 1299] = float("nan"), float("inf"), float("nan")
+        seen, away = seen_keys(Sq, Sk, **rules)
+        keep = [i for i in range(Sq) if i != 2]  # (the first document's last query sees key 1299)
+        zeroed = v.nan_to_num(0.0, 0.0, 0.0), k.nan_to_num(0.0)
+        want, tol = attention(q[0], zeroed[1][0], zeroed[0][0], 0.1, seen, away, cap, **bias)
+        o = _ruled(q, k, v, 0.1, rules, bias, cap)[0]
+        within(o[keep], want[keep], tol[keep])
+        assert o[2].isnan().all()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_bits_repeat(gpu, D):
+    """The same call gives the same bits, whatever is in the caches and registers before it."""
+    q, k, v = _randn(50, 1, 300, 4, D, std=2), _randn(51, 1, 300, 2, D), _randn(52, 1, 300, 2, D)
+    other = torch.empty(1 << 28, dtype=torch.int8, device="cuda:0")
+    starts = _i32([5, 60, 150]), _i32([10, 200, 250])
+    for kw in (dict(q_starts=starts[0], k_starts=starts[1]), dict(causal=True, window=40), dict(causal=True, cap=5.0), dict(causal=True, **_bias("slopes", 4, 0)),
+               dict(q_starts=starts[0], k_starts=starts[1], cap=2.0, **_bias("table", 4, 1))):
+        first = kernels.attn_ruled(q, k, v, 0.1, **kw)
+        for i in range(10):
+            other.fill_(i)
+            kernels.attn_ruled(k, q[:, :, :2], q[:, :, 2:], 3.0)  # (large scores left behind)
+            assert torch.equal(kernels.attn_ruled(q, k, v, 0.1, **kw), first), kw
+
+
 def test_prompt_empty(gpu):
     q, k = _randn(29, 2, 5, 2, 64), _randn(30, 2, 0, 2, 64)
     assert not kernels.attn_ruled(q, k, k, 0.1).any()
@@ -371,12 +406,13 @@ def test_prompt_then_tokens(gpu, cap, kind, window):
 def test_streams_graphs_and_threads_of_work(gpu):
     """Calls on a side stream, and two captured graphs of decoding replayed side by side with eager calls between, give the eager bits."""
     (q, kc, vc, table, lengths), _ = _paged_problem(9, [900, 1500], 16, 8, 2, 64, BF16)
-    p = _randn(10, 1, 500, 8, 64)
-    eager = kernels.attn_paged(q, kc, vc, table, lengths, 0.1), kernels.attn_ruled(p, p, p, 0.1, causal=True)
+    p = _randn(10, 1, 3000, 8, 64)
+    few = p[:, :9]
+    eager = kernels.attn_paged(q, kc, vc, table, lengths, 0.1), kernels.attn_ruled(few, p, p, 0.1, causal=True)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
-        other = kernels.attn_paged(q, kc, vc, table, lengths, 0.1), kernels.attn_ruled(p, p, p, 0.1, causal=True)
+        other = kernels.attn_paged(q, kc, vc, table, lengths, 0.1), kernels.attn_ruled(few, p, p, 0.1, causal=True)
     torch.cuda.current_stream().wait_stream(side)
     assert all(torch.equal(a, b) for a, b in zip(eager, other))
     q2 = q.flip(0).contiguous()
@@ -384,7 +420,7 @@ def test_streams_graphs_and_threads_of_work(gpu):
     for x in (q, q2):
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
-            outs.append((kernels.attn_paged(x, kc, vc, table, lengths, 0.1), kernels.attn_ruled(p, p, p, 0.1, causal=True)))
+            outs.append((kernels.attn_paged(x, kc, vc, table, lengths, 0.1), kernels.attn_ruled(few, p, p, 0.1, causal=True)))
         graphs.append(graph)
     want = [eager[0], kernels.attn_paged(q2, kc, vc, table, lengths, 0.1)]
     for _ in range(3):

@@ -21,9 +21,9 @@ def _error():
 
 
 def _ruled(q=P, k=P, v=P, o=P, B=1, Sq=4, Sk=4, H=2, Hkv=1, D=64, qs=(512, 128, 64), ks=(256, 64, 64), vs=(256, 64, 64), os=(512, 128, 64), scale=0.1,
-           dtype=BF16, **rules):
+           dtype=BF16, ws=None, ws_bytes=0, **rules):
     r = _lib.AttnRules(**rules)
-    return _lib.load().odit_attn_ruled(q, k, v, o, B, Sq, Sk, H, Hkv, D, _s(*qs), _s(*ks), _s(*vs), _s(*os), scale, C.byref(r), dtype, None)
+    return _lib.load().odit_attn_ruled(q, k, v, o, B, Sq, Sk, H, Hkv, D, _s(*qs), _s(*ks), _s(*vs), _s(*os), scale, C.byref(r), dtype, ws, ws_bytes, None)
 
 
 def _paged(q=P, k=P, v=P, table=P, lengths=P, o=P, B=2, H=4, Hkv=2, D=64, pages=3, page=16, most=5, qs=(256, 64), ks=(2048, 128, 64), vs=(2048, 128, 64), ts=5,
@@ -44,7 +44,7 @@ def _rope(q=P, k=P, v=None, pos=P, turns=P, qo=P, ko=P, slots=None, kc=None, vc=
     (dict(scale=float("nan")), -1, "scale"), (dict(window=-1), -1, "window"), (dict(window=(1 << 30) + 1), -1, "window"), (dict(docs=2), -1, "q_starts"),
     (dict(docs=-1), -1, "q_starts"), (dict(cap=-1.0), -1, "cap"), (dict(cap=9000.0), -1, "cap"), (dict(cap=float("nan")), -1, "cap"),
     (dict(slopes=P, distance=P), -1, "exclude"), (dict(distance=P, radius=1025), -1, "radius"), (dict(distance=P, radius=-1), -1, "radius"),
-    (dict(k=P + 8), -1, "aligned"), (dict(vs=(256, 60, 64)), -1, "multiples"), (dict(ks=(256, 1 << 23, 64)), -1, "apart"), (dict(ks=(256, -64, 64)), -1, "apart"),
+    (dict(k=P + 8), -1, "aligned"), (dict(ws=P + 8), -1, "aligned"), (dict(vs=(256, 60, 64)), -1, "multiples"), (dict(ks=(256, 1 << 23, 64)), -1, "apart"), (dict(ks=(256, -64, 64)), -1, "apart"),
     (dict(q=None), -1, "null"), (dict(v=None), -1, "null"), (dict(Sq=-1), -1, "shape"), (dict(Sk=(1 << 30) + 1), -1, "shape"), (dict(B=1 << 30, H=8), -1, "too many"),
     (dict(B=1 << 10, Sq=1 << 29, H=64), -1, "too large")])
 def test_ruled_refuses(change, status, text):
@@ -53,6 +53,21 @@ def test_ruled_refuses(change, status, text):
 
 def test_ruled_takes_empty_problems():
     assert _ruled(B=0) == 0 and _ruled(Sq=0) == 0
+
+
+def test_ruled_workspace():
+    """Few query blocks with many keys are cut, into at most 32; what fills the GPU, and what has few keys, is not."""
+    def chunks(B, Sq, Sk, H, D, **rules):
+        need = _lib.load().odit_attn_ruled_workspace_bytes(B, Sq, Sk, H, D, C.byref(_lib.AttnRules(**rules)))
+        part = (Sq + 127) // 128 * H * B * 128 * (D + 2) * 4
+        assert need % part == 0
+        return need // part or 1
+
+    assert chunks(1, 1, 8192, 8, 128) == 32 and 8 <= chunks(1, 100, 8192, 32, 64) <= 32
+    assert chunks(1, 1, 8192, 64, 128) == 8 and chunks(1, 1, 8192, 256, 128) == 2 and chunks(1, 1, 8192, 257, 128) == 1  # 512 of them run at once
+    assert chunks(1, 77, 77, 24, 128) == 1 and chunks(1, 16384, 16384, 16, 128) == 1
+    assert chunks(1, 1, 1 << 20, 8, 128, window=64, causal=1) == 1 and chunks(1, 64, 1 << 20, 8, 128, docs=1 << 16, q_starts=P, k_starts=P) == 1
+    assert _lib.load().odit_attn_ruled_workspace_bytes(0, 1, 8192, 8, 128, C.byref(_lib.AttnRules())) == 0
 
 
 @pytest.mark.parametrize("change,status,text", [

@@ -44,8 +44,9 @@ _SIGNATURES = {
     ),
     "odit_attn_ruled": (
         C.c_int,
-        [C.c_void_p] * 4 + [C.c_int] * 6 + [_i64p] * 4 + [C.c_float, C.c_void_p, C.c_int, C.c_void_p],
+        [C.c_void_p] * 4 + [C.c_int] * 6 + [_i64p] * 4 + [C.c_float, C.c_void_p, C.c_int, C.c_void_p, C.c_size_t, C.c_void_p],
     ),
+    "odit_attn_ruled_workspace_bytes": (C.c_size_t, [C.c_int] * 5 + [C.c_void_p]),
     "odit_attn_paged_workspace_bytes": (C.c_size_t, [C.c_int] * 7),
     "odit_attn_paged": (
         C.c_int,

@@ -31,6 +31,8 @@ struct RuledParams {
   float scale_log2, bias_scale;  // scale log2(e) and 1 / scale
   Cap cap;
   int n_qblocks, units;  // units: heads of all batch rows
+  int chunks;            // workgroups that share a query block's tiles; with more than one, their sums go to ws
+  float* ws;             // [units][n_qblocks][chunks][128][D] sums, then [...][128] (maximum in units of log2, sum)
 };
 
 // Among 64 documents from `base` on, whose starts the lanes hold: the last one that starts at or before the lane's row, one of the 32 from
@@ -108,14 +110,16 @@ void attn_ruled_kernel(const RuledParams p) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, hh = lane >> 5;
   // the last query blocks, which see most under a causal order, begin first; where the heads divide over the XCDs, an XCD keeps its heads
+  // (steep slopes leave a head little to add: with slopes the heads go round the XCDs, 1040 us of 16384 causal tokens, 16 heads of 128, otherwise, 929 so)
+  const int chunk = p.chunks > 1 ? blockIdx.x / (p.units * p.n_qblocks) : 0, block = blockIdx.x - chunk * (p.units * p.n_qblocks);
   int unit, qb;
   if (BIAS != 1 && p.units % kNumXcd == 0) {
-    const int per = p.units / kNumXcd, local = blockIdx.x / kNumXcd;
-    unit = blockIdx.x % kNumXcd * per + local % per;
+    const int per = p.units / kNumXcd, local = block / kNumXcd;
+    unit = block % kNumXcd * per + local % per;
     qb = p.n_qblocks - 1 - local / per;
   } else {
-    unit = blockIdx.x % p.units;
-    qb = p.n_qblocks - 1 - blockIdx.x / p.units;
+    unit = block % p.units;
+    qb = p.n_qblocks - 1 - block / p.units;
   }
   const int h = unit % p.H, b = unit / p.H, hkv = h / (p.H / p.Hkv);
   const int q0 = qb * BM + wave * 32;
@@ -145,6 +149,9 @@ void attn_ruled_kernel(const RuledParams p) {
 
   // ---- what this lane's query sees ----
   constexpr int kNone = 0x7fffffff;
+  // the band of a query at place `at` of a document of kn keys
+  const auto band_begin = [&](int at, int kn) { return p.window > 0 ? clampi(at - p.window + 1, 0, kn) : 0; };
+  const auto band_end = [&](int at, int kn) { return p.causal ? clampi(at + 1, 0, kn) : p.window > 0 ? clampi(at + p.window, 0, kn) : kn; };
   int blo, bhi, plo = 0, phi = 0, pos;  // pos: the key at the query's own place
   {
     int ks = 0, kn = p.Sk, qs = 0, qe = p.Sq, doc = 0, prefix = 0;
@@ -178,8 +185,7 @@ void attn_ruled_kernel(const RuledParams p) {
     constexpr int64_t kFar = (1 << 30) - 1;
     const int64_t place = static_cast<int64_t>(row) + kn - qe;
     const int at = static_cast<int>(place < -kFar ? -kFar : place > kFar ? kFar : place);
-    const int lo = p.window > 0 ? clampi(at - p.window + 1, 0, kn) : 0;
-    const int hi = p.causal ? clampi(at + 1, 0, kn) : p.window > 0 ? clampi(at + p.window, 0, kn) : kn;
+    const int lo = band_begin(at, kn), hi = band_end(at, kn);
     pos = ks + at;
     blo = in && hi > lo ? ks + lo : 0;  // (nothing: [0, 0))
     bhi = in && hi > lo ? ks + hi : 0;
@@ -190,35 +196,51 @@ void attn_ruled_kernel(const RuledParams p) {
   }
   int all0, all1;  // the keys that all queries of the wavefront have in their bands (none: all1 <= all0)
   {
-    const int b0 = half_min(bhi > 0 ? blo : kNone), b1 = half_max(bhi), p0 = half_min(phi > 0 ? plo : kNone), p1 = half_max(phi);
-    all0 = half_max(blo);
-    all1 = half_min(bhi);
     if (hh == 0) ranges[wave * 32 + l32] = make_int4(blo, bhi, plo, phi);
     if (BIAS != 0 && hh == 0) places[wave * 32 + l32] = pos;
-    if (lane == 0) { bounds[wave][0] = b0; bounds[wave][1] = b1; bounds[wave][2] = p0; bounds[wave][3] = p1; }
+    all0 = half_max(blo);
+    all1 = half_min(bhi);
+    if (p.docs > 0) {
+      const int b0 = half_min(bhi > 0 ? blo : kNone), b1 = half_max(bhi), p0 = half_min(phi > 0 ? plo : kNone), p1 = half_max(phi);
+      if (lane == 0) { bounds[wave][0] = b0; bounds[wave][1] = b1; bounds[wave][2] = p0; bounds[wave][3] = p1; }
+    }
   }
-  __syncthreads();
   // the workgroup's tiles: up to two runs
   int s1, n1, s2, n2;
   {
     int lo[2] = {kNone, kNone}, hi[2] = {0, 0};
+    if (p.docs > 0) {
+      __syncthreads();
 #pragma unroll
-    for (int w = 0; w < NW; ++w)
+      for (int w = 0; w < NW; ++w)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        lo[i] = min(lo[i], bounds[w][2 * i]);
-        hi[i] = max(hi[i], bounds[w][2 * i + 1]);
-      }
+        for (int i = 0; i < 2; ++i) {
+          lo[i] = min(lo[i], bounds[w][2 * i]);
+          hi[i] = max(hi[i], bounds[w][2 * i + 1]);
+        }
+    } else {  // one document: both ends of the band rise with the row
+      const int last = min(qb * BM + BM, p.Sq) - 1;
+      lo[0] = band_begin(qb * BM + p.Sk - p.Sq, p.Sk);
+      hi[0] = band_end(last + p.Sk - p.Sq, p.Sk);
+      lo[1] = 0;
+      hi[1] = p.prefix != nullptr ? clampi(p.prefix[b], 0, p.Sk) : 0;
+    }
     int a0 = lo[0] / BN, a1 = hi[0] > lo[0] ? (hi[0] + BN - 1) / BN : a0, c0 = lo[1] / BN, c1 = hi[1] > lo[1] ? (hi[1] + BN - 1) / BN : c0;
     if (a1 == a0) { a0 = c0; a1 = c1; c1 = c0; }                                                    // one run or none
     if (c1 > c0 && c0 <= a1 && a0 <= c1) { a0 = min(a0, c0); a1 = max(a1, c1); c0 = c1 = 0; }        // they touch
     s1 = __builtin_amdgcn_readfirstlane(a0); n1 = __builtin_amdgcn_readfirstlane(a1 - a0);
     s2 = __builtin_amdgcn_readfirstlane(c0); n2 = __builtin_amdgcn_readfirstlane(c1 - c0);
   }
-  const int n_tiles = n1 + n2;
+  // this workgroup's of them: tile i is number last - i of both runs together
+  int last = n1 + n2 - 1, n_tiles = n1 + n2;
+  if (p.chunks > 1) {
+    const int begin = static_cast<int>(static_cast<int64_t>(n_tiles) * chunk / p.chunks);
+    n_tiles = static_cast<int>(static_cast<int64_t>(n_tiles) * (chunk + 1) / p.chunks) - begin;
+    last -= begin;
+  }
   // From the last key back: under a causal order the nearest keys come first. Where distance takes from the scores, the running maximum is
-  // then near its end from the first tile on (slopes at 16384 tokens, 16 heads: 1203 us forwards, @@ backwards).
-  auto tile_at = [&](int i) { return n_tiles - 1 - i < n1 ? s1 + n_tiles - 1 - i : s2 + n_tiles - 1 - i - n1; };
+  // then near its end from the first tile on (slopes at 16384 tokens, 16 heads: 1203 us forwards, 1040 backwards).
+  auto tile_at = [&](int i) { return last - i < n1 ? s1 + last - i : s2 + last - i - n1; };
 
   // ---- tile loads: as in attn_fwd_dma.hip, but with a buffer descriptor for each tile, so that offsets stay small in any tensor ----
   const T* const kbase = static_cast<const T*>(p.k) + b * p.ks_b + hkv * p.ks_h;
@@ -502,85 +524,169 @@ void attn_ruled_kernel(const RuledParams p) {
 
   // ---- epilogue ----
   const float l_tot = l_run + swapped(l_run);
-  const float inv = l_tot > 0.f ? 1.f / l_tot : l_tot == 0.f ? 0.f : l_tot;  // (a NaN sum is a NaN row)
+  const bool mine = q0 + l32 < p.Sq;
+  const int64_t part = (static_cast<int64_t>(unit) * p.n_qblocks + qb) * p.chunks + chunk;
+  float* const po = p.ws + part * BM * D;
+  float* const pml = p.ws + static_cast<int64_t>(p.units) * p.n_qblocks * p.chunks * BM * D + part * BM * 2;
+  float probe = 0.f;  // NaN once anything is NaN or infinite
   T* const orow = static_cast<T*>(p.o) + b * p.os_b + h * p.os_h;
-  float probe = 0.f;
+  if (p.chunks > 1) {
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt)
+    for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-    for (int g = 0; g < 4; g += 2) {
-      float x[8];
+      for (int g = 0; g < 4; ++g) {
+        f32x4_v x;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x[e] = l_tot == 0.f ? 0.f : o[dt][g * 4 + e] * inv;
-        probe = fmaf(x[e], 0.f, probe);  // NaN once anything is NaN or infinite
+        for (int e = 0; e < 4; ++e) {
+          x[e] = l_tot == 0.f ? 0.f : o[dt][g * 4 + e];
+          probe = fmaf(x[e], 0.f, probe);
+        }
+        if (mine) *reinterpret_cast<f32x4_v*>(po + (wave * 32 + l32) * D + dt * 32 + g * 8 + hh * 4) = x;
       }
-      auto pair = [&](int e) __attribute__((always_inline)) {
-        return __builtin_amdgcn_permlane32_swap(M::pack2(x[e], x[e + 1]), M::pack2(x[e + 4], x[e + 5]), false, false);
-      };
-      const auto lo = pair(0), hi = pair(2);
-      u32x4_v w;
-      w.x = lo[0]; w.y = hi[0]; w.z = lo[1]; w.w = hi[1];
-      if (q0 + l32 < p.Sq) *reinterpret_cast<u32x4_v*>(orow + row * p.os_s + dt * 32 + g * 8 + hh * 8) = w;
-    }
+    if (mine && hh == 0) *reinterpret_cast<float2*>(pml + (wave * 32 + l32) * 2) = make_float2(m_run * c, l_tot);
+  } else {
+    const float inv = 1.f / l_tot;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int g = 0; g < 4; g += 2) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          x[e] = l_tot == 0.f ? 0.f : o[dt][g * 4 + e] * inv;
+          probe = fmaf(x[e], 0.f, probe);
+        }
+        auto pair = [&](int e) __attribute__((always_inline)) {
+          return __builtin_amdgcn_permlane32_swap(M::pack2(x[e], x[e + 1]), M::pack2(x[e + 4], x[e + 5]), false, false);
+        };
+        const auto lo = pair(0), hi = pair(2);
+        u32x4_v w;
+        w.x = lo[0]; w.y = hi[0]; w.z = lo[1]; w.w = hi[1];
+        if (mine) *reinterpret_cast<u32x4_v*>(orow + row * p.os_s + dt * 32 + g * 8 + hh * 8) = w;
+      }
+  }
   // rows to be done again: finite sums, but values that are not. (l_tot == 0: nothing was seen, zeros are right)
-  const bool again = q0 + l32 < p.Sq && l_tot > 0.f && l_tot < INFINITY && probe != 0.f;
-  uint64_t bad = __ballot(again);
+  uint64_t bad = __ballot(mine && l_tot > 0.f && l_tot < INFINITY && probe != 0.f);
   bad = (bad | (bad >> 32)) & 0xffffffffull;
   while (bad != 0) {  // (wave-uniform)
     const int who = __builtin_ctzll(bad);
     bad &= bad - 1;
     const int r = q0 + who, at = BIAS != 0 ? places[wave * 32 + who] : 0;
     const int4 its = ranges[wave * 32 + who];
-    const int from[2] = {its.x, its.z}, to[2] = {its.y, its.w};
     const T* const qp = static_cast<const T*>(p.q) + b * p.qs_b + h * p.qs_h + r * p.qs_s;
     float m = -INFINITY, l = 0.f, acc[D / 64] = {};
-    for (int range = 0; range < 2; ++range)
-      for (int j0 = from[range]; j0 < to[range]; j0 += 64) {
-        const int key = j0 + lane;
-        const bool live = key < to[range] && !(range == 1 && key >= from[0] && key < to[0]);  // (the band's keys have been)
-        float x = -INFINITY;
-        if (live) {
-          const T* const kp = kbase + key * p.ks_s;
-          float s = 0.f;
-          for (int d = 0; d < D; d += 8) {
-            const u32x4 qv = load_raw(qp + d), kv = load_raw(kp + d);
+    for (int i = 0; i < n_tiles; ++i) {
+      const int t0 = tile_at(i) * BN, key = t0 + lane;
+      const bool sees = (key >= its.x && key < its.y) || (key >= its.z && key < its.w);
+      const uint64_t some = __ballot(sees);
+      if (some == 0) continue;
+      float x = -INFINITY;
+      if (sees) {
+        const T* const kp = kbase + key * p.ks_s;
+        float s = 0.f;
+        for (int d = 0; d < D; d += 8) {
+          const u32x4 qv = load_raw(qp + d), kv = load_raw(kp + d);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) s = fmaf(Raw<T>::get(qv, e), Raw<T>::get(kv, e), s);
-          }
-          float bias = 0.f;
-          if constexpr (BIAS == 1) bias = -slope * fabsf(static_cast<float>(key - at));
-          if constexpr (BIAS == 2) bias = table[clampi(key - at, -p.radius, p.radius) + p.radius + kPad];
-          x = CAP ? p.cap(s) + bias : (s + bias) * p.scale_log2;
+          for (int e = 0; e < 8; ++e) s = fmaf(Raw<T>::get(qv, e), Raw<T>::get(kv, e), s);
         }
-        float mx = x;
-        for (int sft = 1; sft < 64; sft <<= 1) mx = fmaxf(mx, __shfl_xor(mx, sft, 64));
-        const float m_new = fmaxf(m, mx), m_safe = m_new == -INFINITY ? 0.f : m_new;
-        const float alpha = __builtin_amdgcn_exp2f(m - m_safe), w = __builtin_amdgcn_exp2f(x - m_safe);
-        m = m_new;
-        l = l * alpha + group_sum<64>(w);
-#pragma unroll
-        for (int e = 0; e < D / 64; ++e) acc[e] *= alpha;
-        const uint64_t some = __ballot(live);
-        for (int u = 0; u < 64; ++u) {
-          if (!((some >> u) & 1)) continue;
-          const float pw = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), u));
-          const T* const vp = vbase + (j0 + u) * p.vs_s + lane * (D / 64);
-#pragma unroll
-          for (int e = 0; e < D / 64; ++e) acc[e] = fmaf(pw, to_float(vp[e]), acc[e]);
-        }
+        float bias = 0.f;
+        if constexpr (BIAS == 1) bias = -slope * fabsf(static_cast<float>(key - at));
+        if constexpr (BIAS == 2) bias = table[clampi(key - at, -p.radius, p.radius) + p.radius + kPad];
+        x = CAP ? p.cap(s) + bias : (s + bias) * p.scale_log2;
       }
-    T* const op = orow + r * p.os_s + lane * (D / 64);
+      float mx = x;
+      for (int sft = 1; sft < 64; sft <<= 1) mx = fmaxf(mx, __shfl_xor(mx, sft, 64));
+      const float m_new = fmaxf(m, mx), m_safe = m_new == -INFINITY ? 0.f : m_new;
+      const float alpha = __builtin_amdgcn_exp2f(m - m_safe), w = __builtin_amdgcn_exp2f(x - m_safe);
+      m = m_new;
+      l = l * alpha + group_sum<64>(w);
 #pragma unroll
-    for (int e = 0; e < D / 64; ++e) op[e] = from_float<T>(acc[e] / l);
+      for (int e = 0; e < D / 64; ++e) acc[e] *= alpha;
+      for (int u = 0; u < 64; ++u) {
+        if (!((some >> u) & 1)) continue;
+        const float pw = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), u));
+        const T* const vp = vbase + (t0 + u) * p.vs_s + lane * (D / 64);
+#pragma unroll
+        for (int e = 0; e < D / 64; ++e) acc[e] = fmaf(pw, to_float(vp[e]), acc[e]);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < D / 64; ++e) {
+      if (p.chunks > 1) po[(wave * 32 + who) * D + lane * (D / 64) + e] = acc[e];
+      else (orow + r * p.os_s)[lane * (D / 64) + e] = from_float<T>(acc[e] / l);
+    }
+    if (p.chunks > 1 && lane == 0) *reinterpret_cast<float2*>(pml + (wave * 32 + who) * 2) = make_float2(m, l);
   }
+}
+
+// Joins the chunks' sums, a wavefront for each row: o = sum_c 2^(m_c - m) o_c / sum_c 2^(m_c - m) l_c, m = max_c m_c. Lane c has chunk c's
+// maximum and sum; the features' loads go out eight at a time.
+constexpr int kMaxChunks = 32;
+template <typename T, int D>
+__global__ __launch_bounds__(256) void attn_ruled_merge_kernel(const RuledParams p) {
+  constexpr int EPL = D / 64;
+  static_assert(kMaxChunks <= 64, "a lane for each chunk");
+  const int lane = threadIdx.x & 63;
+  const int64_t gr = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (gr >= static_cast<int64_t>(p.units) * p.Sq) return;
+  const int unit = static_cast<int>(gr / p.Sq), row = static_cast<int>(gr - static_cast<int64_t>(unit) * p.Sq);
+  const int64_t first = (static_cast<int64_t>(unit) * p.n_qblocks + row / 128) * p.chunks;
+  const float* const ml = p.ws + static_cast<int64_t>(p.units) * p.n_qblocks * p.chunks * 128 * D;
+  const float* const po = p.ws + (first * 128 + row % 128) * D + lane * EPL;
+  const int mine = lane < p.chunks ? lane : 0;
+  const float2 own = *reinterpret_cast<const float2*>(ml + ((first + mine) * 128 + row % 128) * 2);
+  const float mc = lane < p.chunks ? own.x : -INFINITY;
+  float m = mc;
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) m = fmaxf(m, __shfl_xor(m, s, 64));
+  const float w = __builtin_amdgcn_exp2f(mc - (m == -INFINITY ? 0.f : m)), l = wave_sum(lane < p.chunks ? w * own.y : 0.f);
+  float acc[EPL] = {};
+  for (int c0 = 0; c0 < p.chunks; c0 += 8) {
+    float x[8][EPL];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) x[i][e] = c0 + i < p.chunks ? po[static_cast<int64_t>(c0 + i) * 128 * D + e] : 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float wi = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), (c0 + i) & 63));
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) acc[e] = fmaf(wi, x[i][e], acc[e]);
+    }
+  }
+  T* const op = static_cast<T*>(p.o) + unit / p.H * p.os_b + unit % p.H * p.os_h + row * p.os_s + lane * EPL;
+#pragma unroll
+  for (int e = 0; e < EPL; ++e) op[e] = from_float<T>(l == 0.f ? 0.f : acc[e] / l);
+}
+
+// Into how many chunks a query block's tiles are cut: where the call has fewer workgroups than the GPU has room for, as many as cost least.
+// A tile is 1.1 us of a workgroup alone on its compute unit; the join is a launch of 3 us and its sums' way to memory and back, 8 bytes a feature.
+static int ruled_chunks(int B, int Sq, int Sk, int H, int D, int docs, int window, int causal) {
+  const int64_t blocks = static_cast<int64_t>((Sq + 127) / 128) * H * B, room = D == 128 ? 512 : 768;
+  int64_t keys = docs > 0 ? 2 * (Sk / docs) + 64 : Sk;  // that a query block may see, about
+  if (window > 0) {
+    const int64_t most = (causal ? 1ll : 2ll) * window + 128;
+    keys = most < keys ? most : keys;
+  }
+  const double tiles = static_cast<double>(keys) / 64, join = static_cast<double>(B) * H * Sq * D * 8 / 4e6;
+  int best = 1;
+  double cost = 1.1 * tiles;
+  for (int n = 2; n <= kMaxChunks && n * blocks <= room && n <= tiles; ++n) {
+    const double t = 1.1 * tiles / n + 3.0 + n * join;
+    if (t < cost) { cost = t; best = n; }
+  }
+  return best;
+}
+
+static size_t ruled_workspace_bytes(int chunks, int B, int Sq, int H, int D) {
+  return chunks > 1 ? static_cast<size_t>((Sq + 127) / 128) * H * B * chunks * 128 * (D + 2) * sizeof(float) : 0;
 }
 
 template <typename T, int D>
 static int launch_ruled(RuledParams& p, bool cap, int bias, hipStream_t stream) {
   p.n_qblocks = (p.Sq + 127) / 128;
   p.units = p.H * p.B;
-  const int64_t total = static_cast<int64_t>(p.n_qblocks) * p.H * p.B;
+  const int64_t total = static_cast<int64_t>(p.n_qblocks) * p.H * p.B * p.chunks;
   ODIT_CHECK_ARG(total <= 0x7fffffffll, "odit_attn_ruled: grid of %lld workgroups is too large", static_cast<long long>(total));
 #define ODIT_RULED_GO(C, X) hipLaunchKernelGGL((attn_ruled_kernel<T, D, C, X>), dim3(total), dim3(256), 0, stream, p)
   if (cap) {
@@ -589,14 +695,25 @@ static int launch_ruled(RuledParams& p, bool cap, int bias, hipStream_t stream) 
     if (bias == 0) ODIT_RULED_GO(false, 0); else if (bias == 1) ODIT_RULED_GO(false, 1); else ODIT_RULED_GO(false, 2);
   }
 #undef ODIT_RULED_GO
+  if (p.chunks > 1) {
+    const int64_t rows = static_cast<int64_t>(p.units) * p.Sq;
+    hipLaunchKernelGGL((attn_ruled_merge_kernel<T, D>), dim3((rows + 3) / 4), dim3(256), 0, stream, p);
+  }
   return check_launch("odit_attn_ruled");
 }
 
 }  // namespace odit
 
+extern "C" size_t odit_attn_ruled_workspace_bytes(int B, int Sq, int Sk, int H, int D, const odit_attn_rules* rules) {
+  using namespace odit;
+  if (B <= 0 || Sq <= 0 || Sk <= 0 || H <= 0 || D <= 0 || rules == nullptr) return 0;
+  return ruled_workspace_bytes(ruled_chunks(B, Sq, Sk, H, D, rules->docs, rules->window, rules->causal), B, Sq, H, D);
+}
+
 extern "C" int odit_attn_ruled(const void* q, const void* k, const void* v, void* o, int B, int Sq, int Sk, int H, int Hkv, int D,
                                const int64_t q_strides[3], const int64_t k_strides[3], const int64_t v_strides[3],
-                               const int64_t o_strides[3], float scale, const odit_attn_rules* rules, int dtype, void* stream) {
+                               const int64_t o_strides[3], float scale, const odit_attn_rules* rules, int dtype, void* workspace,
+                               size_t workspace_bytes, void* stream) {
   using namespace odit;
   ODIT_CHECK_ARG(rules != nullptr, "odit_attn_ruled: null rules");
   const odit_attn_rules& r = *rules;
@@ -621,6 +738,7 @@ extern "C" int odit_attn_ruled(const void* q, const void* k, const void* v, void
   ODIT_CHECK_ARG(r.distance == nullptr || (r.radius >= 0 && r.radius <= kMaxRadius), "odit_attn_ruled: radius=%d outside [0, %d]", r.radius,
                  kMaxRadius);
   ODIT_CHECK_ARG(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(o), "odit_attn_ruled: q/k/v/o must be 16-byte aligned");
+  ODIT_CHECK_ARG(aligned16(workspace), "odit_attn_ruled: the workspace must be 16-byte aligned");
   for (int i = 0; i < 3; ++i)
     ODIT_CHECK_ARG(q_strides[i] % 8 == 0 && k_strides[i] % 8 == 0 && v_strides[i] % 8 == 0 && o_strides[i] % 8 == 0,
                    "odit_attn_ruled: strides must be multiples of 8 elements");
@@ -640,6 +758,10 @@ extern "C" int odit_attn_ruled(const void* q, const void* k, const void* v, void
   p.os_b = o_strides[0]; p.os_s = o_strides[1]; p.os_h = o_strides[2];
   p.scale_log2 = scale * kLog2e;
   p.bias_scale = 1.f / scale;
+  // (without scratch, or with less than that takes, a query block's tiles stay in one piece)
+  p.chunks = ruled_chunks(B, Sq, Sk, H, D, r.docs, r.window, r.causal);
+  if (workspace == nullptr || workspace_bytes < ruled_workspace_bytes(p.chunks, B, Sq, H, D)) p.chunks = 1;
+  p.ws = static_cast<float*>(workspace);
   p.cap = make_cap(r.cap, scale);
   const int bias = r.slopes != nullptr ? 1 : r.distance != nullptr ? 2 : 0;
   hipStream_t st = static_cast<hipStream_t>(stream);

@@ -655,11 +655,14 @@ PyObject* py_attn_ruled(PyObject*, PyObject* const* a, Py_ssize_t n) {
   r.q_starts = static_cast<const int*>(ptr(qst));
   r.k_starts = static_cast<const int*>(ptr(kst));
   r.prefix = static_cast<const int*>(ptr(prefix));
-  Tensor o = fresh({B, Sq, H, D}, q->options());
+  // (scratch of the call's own, from the allocator: a captured graph then has its own too, and two of them can run side by side)
+  Tensor o = fresh({B, Sq, H, D}, q->options()), ws;
+  const size_t need = odit_attn_ruled_workspace_bytes(B, Sq, Sk, H, D, &r);
+  if (need > 0) ws = fresh({static_cast<int64_t>(need)}, q->options().dtype(at::kByte));
   const int64_t qs[3] = {q->stride(0), q->stride(1), q->stride(2)}, ks[3] = {k->stride(0), k->stride(1), k->stride(2)},
                 vs[3] = {v->stride(0), v->stride(1), v->stride(2)}, os[3] = {Sq * H * D, H * D, D};
   if (unlocked([&] { return odit_attn_ruled(ptr(q), ptr(k), ptr(v), o.data_ptr(), B, Sq, Sk, H, Hkv, D, qs, ks, vs, os, static_cast<float>(scale), &r, dt,
-                                            w.stream); }) != 0)
+                                            need > 0 ? ws.data_ptr() : nullptr, need, w.stream); }) != 0)
     return none();
   return wrap(std::move(o));
   NATIVE_END
@@ -692,7 +695,6 @@ PyObject* py_attn_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int ok = score_rules(nullptr, a[6], a[7], a[8], a[9], H, w, &r);
   if (ok <= 0) return ok < 0 ? nullptr : none();
   Tensor o = fresh({B, H, D}, q->options()), ws;
-  // (memory of the call's own, from the allocator: a captured graph then has its own too, and two of them can run side by side)
   const size_t need = odit_attn_paged_workspace_bytes(B, H, Hkv, D, table->size(1), page, r.window);
   if (need > 0) ws = fresh({static_cast<int64_t>(need)}, q->options().dtype(at::kByte));
   const int64_t qs[2] = {q->stride(0), q->stride(1)}, ks[3] = {k->stride(0), k->stride(1), k->stride(2)}, vs[3] = {v->stride(0), v->stride(1), v->stride(2)},

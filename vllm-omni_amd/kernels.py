@@ -407,11 +407,13 @@ def attn_ruled(
     rules.docs, rules.q_starts, rules.k_starts, rules.prefix = docs, _ptr(q_starts), _ptr(k_starts), _ptr(prefix)
     q, k, v = _strided8(q), _strided8(k), _strided8(v)
     o = torch.empty((B, Sq, H, D), dtype=q.dtype, device=q.device)
+    need = int(_lib.load().odit_attn_ruled_workspace_bytes(B, Sq, Sk, H, D, _lib.C.byref(rules)))
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
     with torch.cuda.device(q.device):
         rc = _lib.load().odit_attn_ruled(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), B, Sq, Sk, H, Hkv, D, _lib.i64_array(q.stride()[:3]),
             _lib.i64_array(k.stride()[:3]), _lib.i64_array(v.stride()[:3]), _lib.i64_array((Sq * H * D, H * D, D)), float(scale),
-            _lib.C.byref(rules), _code(q), _stream())
+            _lib.C.byref(rules), _code(q), _ptr(ws), need, _stream())
     _lib.check(rc, "odit_attn_ruled")
     return o
 
