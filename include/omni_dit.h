@@ -110,13 +110,15 @@ size_t odit_attn_ruled_workspace_bytes(int B, int Sq, int Sk, int H, int D, cons
  * lengths int32 [B]. Key j of a sequence is row j % page_size of page table[b][j / page_size]; the query is at the place of key
  * lengths[b] - 1. Lengths past max_pages * page_size count as that, below 0 as 0; a length of 0 gives zeros; keys whose page number lies
  * outside [0, pages) are not seen. Of the rules, docs and prefix do not apply (0 and NULL).
- * `workspace`: odit_attn_paged_workspace_bytes for the same shape and window (may be 0), contents irrelevant before and after. */
+ * `workspace`: odit_attn_paged_workspace_bytes for the same shape and window (may be 0), contents irrelevant before and after.
+ * `tickets`: NULL, or n_tickets words that are zero before the call and are left zero: with one for each sequence, key head and 16 query
+ * heads of its group, a call of up to 16 chunks a sequence is one launch, not two (the same bits). No two calls at a time may share them. */
 size_t odit_attn_paged_workspace_bytes(int B, int H, int Hkv, int D, int max_pages, int page_size, int window);
 int odit_attn_paged(const void* q, const void* key_cache, const void* value_cache, const int* table, const int* lengths, void* o, int B,
                     int H, int Hkv, int D, int pages, int page_size, int max_pages, const int64_t q_strides[2],
                     const int64_t key_cache_strides[3], const int64_t value_cache_strides[3], int64_t table_stride,
                     const int64_t o_strides[2], float scale, const odit_attn_rules* rules, int dtype, void* workspace,
-                    size_t workspace_bytes, void* stream);
+                    size_t workspace_bytes, unsigned* tickets, size_t n_tickets, void* stream);
 
 /* Rotary positions of T packed tokens, and their keys and values into such a cache. Pair i < rot/2 of each head of q [T,H,D] and k [T,Hkv,D]
  * (strides for token and head, multiples of 8; D a multiple of 8 up to 1024) is turned by positions[t] * turns[i] whole turns (fp64, so far

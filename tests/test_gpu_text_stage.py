@@ -266,6 +266,26 @@ def test_decode_rules(gpu, cap, kind, D, dtype, window):
             break
 
 
+@pytest.mark.parametrize("lengths", [[5000], [5000, 1, 130, 0, 2500]], ids=str)
+@pytest.mark.parametrize("D,dtype", [(128, BF16), (64, F16)])
+def test_decode_many_chunks(gpu, lengths, D, dtype):
+    """More chunks than the last workgroup joins by itself, beside sequences of a few and of one; repeated, on two streams, the same bits."""
+    (q, kc, vc, table, n), rows = _paged_problem(8, lengths, 16, 4, 1, D, dtype)
+    o = kernels.attn_paged(q, kc, vc, table, n, 0.1)
+    _check_paged(q, rows, o, 0.1, None, 0.0, {})
+    few = table[:, :100].contiguous()  # (up to 1600 keys: up to 13 chunks)
+    want = kernels.attn_paged(q, kc, vc, few, n, 0.1)
+    _check_paged(q, [(k[:1600], v[:1600]) for k, v in rows], want, 0.1, None, 0.0, {})
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(20):
+        a, b = kernels.attn_paged(q, kc, vc, few, n, 0.1), kernels.attn_paged(q, kc, vc, table, n, 0.1)
+        with torch.cuda.stream(side):
+            c = kernels.attn_paged(q, kc, vc, few, n, 0.1)
+        torch.cuda.synchronize()
+        assert torch.equal(a, want) and torch.equal(b, o) and torch.equal(c, want)
+
+
 def test_decode_strides_and_long_tables(gpu):
     """Keys and values as halves of one cache with the head ahead of the row; a table and lengths that are parts of larger ones; a table for far
     more pages than there are (many chunks, most of them empty)."""

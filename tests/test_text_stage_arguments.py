@@ -30,7 +30,7 @@ def _paged(q=P, k=P, v=P, table=P, lengths=P, o=P, B=2, H=4, Hkv=2, D=64, pages=
            os=(256, 64), scale=0.1, dtype=BF16, ws=P, ws_bytes=1 << 30, **rules):
     r = _lib.AttnRules(**rules)
     return _lib.load().odit_attn_paged(q, k, v, table, lengths, o, B, H, Hkv, D, pages, page, most, _s(*qs), _s(*ks), _s(*vs), ts, _s(*os), scale, C.byref(r),
-                                       dtype, ws, ws_bytes, None)
+                                       dtype, ws, ws_bytes, None, 0, None)
 
 
 def _rope(q=P, k=P, v=None, pos=P, turns=P, qo=P, ko=P, slots=None, kc=None, vc=None, T=4, H=2, Hkv=1, D=64, rot=64, pages=0, page=1, qs=(128, 64), ks=(64, 64),

@@ -50,7 +50,8 @@ _SIGNATURES = {
     "odit_attn_paged_workspace_bytes": (C.c_size_t, [C.c_int] * 7),
     "odit_attn_paged": (
         C.c_int,
-        [C.c_void_p] * 6 + [C.c_int] * 7 + [_i64p] * 3 + [C.c_int64, _i64p, C.c_float, C.c_void_p, C.c_int, C.c_void_p, C.c_size_t, C.c_void_p],
+        [C.c_void_p] * 6 + [C.c_int] * 7 + [_i64p] * 3 + [C.c_int64, _i64p, C.c_float, C.c_void_p, C.c_int, C.c_void_p, C.c_size_t,
+                                                                C.c_void_p, C.c_size_t, C.c_void_p],
     ),
     "odit_rope_append": (
         C.c_int,

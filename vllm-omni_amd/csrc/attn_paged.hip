@@ -44,13 +44,17 @@ struct PagedParams {
   Cap cap;
   int group, head_blocks, units, splits, chunk;
   float* ws;  // per unit and split: [heads of a block][D] sums, then [heads of a block] (maximum, sum)
+  unsigned* tickets;  // a word for each unit, zero between launches (nullptr: the join is a launch of its own)
 };
 
+// The join by the last workgroup costs it a trip to memory behind the others (1 us) where a launch of its own costs 2.6 us and 3 of the
+// host's; it holds all chunks' parts at once, so it is for up to kPagedTickets of them.
+constexpr int kPagedTickets = 16;
 constexpr int kPagedWaves = 4, kPagedTile = 32, kPagedEntries = 1024;
-// keys of a sequence that its query sees: [first, end)
-__device__ __forceinline__ void paged_range(const PagedParams& p, int b, int* first, int* end) {
+// keys of a sequence of this length that its query sees: [first, end)
+__device__ __forceinline__ void paged_range(const PagedParams& p, int length, int* first, int* end) {
   const int64_t most = static_cast<int64_t>(p.max_pages) * p.page;
-  int n = p.pages > 0 ? p.lengths[b] : 0;
+  int n = p.pages > 0 ? length : 0;
   if (n > most) n = static_cast<int>(most);
   if (n < 0) n = 0;
   *end = n;
@@ -67,6 +71,46 @@ __device__ __forceinline__ void load_lds16_at(uint32_t lds, const void* from) {
 #endif
 }
 
+// pairs of floats that workgroups of one launch hand to each other: past the caches of their XCD, both ways
+__device__ __forceinline__ void put_pair(float* at, float x0, float x1) {
+  __hip_atomic_store(reinterpret_cast<unsigned long long*>(at), static_cast<unsigned long long>(__float_as_uint(x1)) << 32 | __float_as_uint(x0),
+                     __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 get_pair(const float* at) {
+  const unsigned long long x = __hip_atomic_load(reinterpret_cast<const unsigned long long*>(at), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return make_float2(__uint_as_float(static_cast<uint32_t>(x)), __uint_as_float(static_cast<uint32_t>(x >> 32)));
+}
+
+// Up to kPagedTickets chunks' sums joined, features d and d + 1 of head hd: o = sum_c 2^(m_c - m) o_c / sum_c 2^(m_c - m) l_c, m = max_c m_c.
+// All loads are ahead of their first use.
+template <typename T, int D>
+__device__ __forceinline__ uint32_t join_few(const float* part0, int most, int hd, int d, int parts) {
+  float2 ml[kPagedTickets], x[kPagedTickets];
+#pragma unroll
+  for (int c = 0; c < kPagedTickets; ++c) {
+    if (c < parts) {
+      const float* const part = part0 + c * most * (D + 2);
+      ml[c] = get_pair(part + most * D + 2 * hd);
+      x[c] = get_pair(part + hd * D + d);
+    }
+  }
+  float m = -INFINITY, l = 0.f, x0 = 0.f, x1 = 0.f;
+#pragma unroll
+  for (int c = 0; c < kPagedTickets; ++c)
+    if (c < parts) m = fmaxf(m, ml[c].x);
+  const float m_safe = m == -INFINITY ? 0.f : m;
+#pragma unroll
+  for (int c = 0; c < kPagedTickets; ++c) {
+    if (c < parts) {
+      const float a = __builtin_amdgcn_exp2f(ml[c].x - m_safe);
+      l = fmaf(a, ml[c].y, l);
+      x0 = fmaf(a, x[c].x, x0);
+      x1 = fmaf(a, x[c].y, x1);
+    }
+  }
+  return l == 0.f ? 0u : Mma<T>::pack2(x0 / l, x1 / l);
+}
+
 template <typename T, int D, bool CAP, int BIAS>
 __global__ __launch_bounds__(256) void attn_paged_kernel(const PagedParams p) {
   using M = Mma16<T>;
@@ -76,7 +120,7 @@ __global__ __launch_bounds__(256) void attn_paged_kernel(const PagedParams p) {
   constexpr int KS = D / 32, DT = D / 16;
   __shared__ __attribute__((aligned(1024))) char lds[NW * 4 * TILEB];  // of each wavefront: K0 V0 K1 V1
   __shared__ int entries[kPagedEntries];
-  __shared__ int some_invalid;
+  __shared__ int outside[NW];  // whether a wavefront found page numbers that are none of the cache's
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l16 = lane & 15, g = lane >> 4;
@@ -84,21 +128,21 @@ __global__ __launch_bounds__(256) void attn_paged_kernel(const PagedParams p) {
   const int hb = unit % p.head_blocks, hkv = unit / p.head_blocks % p.Hkv, b = unit / p.head_blocks / p.Hkv;
   const int h0 = hkv * p.group + hb * 16, heads = min(16, p.group - hb * 16);
   const int h = h0 + min(l16, heads - 1);  // this lane's head
-
-  int first, n;
-  paged_range(p, b, &first, &n);
-  const int begin = first + split * p.chunk;
-  if (begin >= n && (split > 0 || p.splits > 1)) return;  // (the merge does not look at this one either)
-  const int end = min(n, begin + p.chunk);
   const auto page_of = [&](int key) { return static_cast<int>(static_cast<uint64_t>(static_cast<uint32_t>(key)) * p.page_mul >> p.page_shift); };
+
+  // Without a window a chunk's place does not depend on the sequence's length: its page numbers are on their way while that is (one trip to
+  // memory of four in a call of one short sequence)
+  const int length = p.lengths[b];
+  int first = 0, n = p.max_pages * p.page;  // (up to 2^30)
+  if (p.window > 0) paged_range(p, length, &first, &n);
+  const int begin = first + split * p.chunk;
   const int pg0 = page_of(begin);
-  if (tid == 0) some_invalid = 0;
-  __syncthreads();
-  if (end > begin) {
-    const int npg = page_of(end - 1) - pg0 + 1;
+  int bad = 0x7fffffff;  // the first of this thread's page numbers that is none
+  if (n > begin) {
+    const int npg = page_of(min(n, begin + p.chunk) - 1) - pg0 + 1;
     for (int i = tid; i < npg; i += NW * 64) {
       int e = p.table[b * p.ts + pg0 + i];
-      if (e < 0 || e >= p.pages) { e = -1; some_invalid = 1; }
+      if (e < 0 || e >= p.pages) { e = -1; bad = min(bad, i); }
       entries[i] = e;
     }
   }
@@ -109,8 +153,16 @@ __global__ __launch_bounds__(256) void attn_paged_kernel(const PagedParams p) {
   const float slope = BIAS == 1 ? p.slopes[h] * kLog2e : 0.f;
   const float* const dist = BIAS == 2 ? p.distance + static_cast<int64_t>(h) * (2 * p.radius + 1) + p.radius : nullptr;  // [away]
   const float far = BIAS == 2 ? dist[-p.radius] * kLog2e : 0.f;
+  if (p.window == 0) paged_range(p, length, &first, &n);
+  const int parts = max(1, (n - first + p.chunk - 1) / p.chunk);  // of this sequence; an empty one has one, too
+  if (split >= parts) return;
+  const int end = min(n, begin + p.chunk);
+  {
+    const bool any = __any(end > begin && bad <= page_of(end - 1) - pg0);  // (pages behind the sequence's last key may be anything)
+    if (lane == 0) outside[wave] = any;
+  }
   __syncthreads();
-  const bool invalid = some_invalid != 0;
+  const bool invalid = (outside[0] | outside[1] | outside[2] | outside[3]) != 0;
 
   const int tiles = (max(end - begin, 0) + BN - 1) / BN, mine = tiles > wave ? (tiles - wave + NW - 1) / NW : 0;
   const T* const kbase = static_cast<const T*>(p.k) + hkv * p.kc_h;
@@ -247,6 +299,9 @@ __global__ __launch_bounds__(256) void attn_paged_kernel(const PagedParams p) {
   for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4_v*>(jo + (wave * 16 + l16) * OP + dt * 16 + g * 4) = o[dt];
   if (g == 0) jm[wave * 16 + l16] = make_float2(m_run * c, l_tot);
   __syncthreads();
+  // what the call's chunks leave is written past the caches of this XCD, as another workgroup's may read it
+  const int most = min(16, p.group);
+  float* const part0 = p.ws + static_cast<int64_t>(unit) * p.splits * most * (D + 2);
   for (int i = tid; i < heads * (D / 2); i += NW * 64) {
     const int hd = i / (D / 2), d = i % (D / 2) * 2;
     float m = -INFINITY;
@@ -261,16 +316,29 @@ __global__ __launch_bounds__(256) void attn_paged_kernel(const PagedParams p) {
       x0 = fmaf(a, jo[(w * 16 + hd) * OP + d], x0);
       x1 = fmaf(a, jo[(w * 16 + hd) * OP + d + 1], x1);
     }
-    if (p.splits == 1) {
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      *reinterpret_cast<uint32_t*>(static_cast<T*>(p.o) + b * p.os_b + (h0 + hd) * p.os_h + d) = l == 0.f ? 0u : Mma<T>::pack2(x0 * inv, x1 * inv);
+    if (parts == 1) {
+      *reinterpret_cast<uint32_t*>(static_cast<T*>(p.o) + b * p.os_b + (h0 + hd) * p.os_h + d) = l == 0.f ? 0u : Mma<T>::pack2(x0 / l, x1 / l);
     } else {
-      const int most = min(16, p.group);
-      float* const part = p.ws + (static_cast<int64_t>(unit) * p.splits + split) * most * (D + 2);
-      part[hd * D + d] = x0;
-      part[hd * D + d + 1] = x1;
-      if (d == 0) { part[most * D + 2 * hd] = m; part[most * D + 2 * hd + 1] = l; }
+      float* const part = part0 + split * most * (D + 2);
+      put_pair(part + hd * D + d, x0, x1);
+      if (d == 0) put_pair(part + most * D + 2 * hd, m, l);
     }
+  }
+  if (parts == 1 || p.tickets == nullptr) return;
+  // The last of the sequence's workgroups to be done joins them, in their order, and puts the word back to zero.
+  __shared__ int is_last;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wavefront's part is where the others see it
+  __syncthreads();
+  if (tid == 0) {
+    const unsigned before = __hip_atomic_fetch_add(p.tickets + unit, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    is_last = before == static_cast<unsigned>(parts - 1);
+    if (is_last) __hip_atomic_store(p.tickets + unit, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  if (!is_last) return;
+  for (int i = tid; i < heads * (D / 2); i += NW * 64) {
+    const int hd = i / (D / 2), d = i % (D / 2) * 2;
+    *reinterpret_cast<uint32_t*>(static_cast<T*>(p.o) + b * p.os_b + (h0 + hd) * p.os_h + d) = join_few<T, D>(part0, most, hd, d, parts);
   }
 }
 
@@ -284,8 +352,15 @@ __global__ __launch_bounds__(256) void attn_paged_merge_kernel(const PagedParams
   const int hkv = h / p.group, hb = h % p.group / 16, hd = h % p.group % 16;
   const int64_t unit = (static_cast<int64_t>(b) * p.Hkv + hkv) * p.head_blocks + hb;
   int first, n;
-  paged_range(p, b, &first, &n);
+  paged_range(p, p.lengths[b], &first, &n);
   const int parts = (n - first + p.chunk - 1) / p.chunk, most = min(16, p.group);
+  if (parts <= 1) return;  // (written by its only workgroup)
+  if (parts <= kPagedTickets) {
+    const int d = threadIdx.x * 2;
+    if (d < D)
+      *reinterpret_cast<uint32_t*>(static_cast<T*>(p.o) + b * p.os_b + h * p.os_h + d) = join_few<T, D>(p.ws + unit * p.splits * most * (D + 2), most, hd, d, parts);
+    return;
+  }
   float m = -INFINITY, l = 0.f, x[EPL] = {};
   for (int i = wave; i < parts; i += 4) {
     const float* const part = p.ws + (unit * p.splits + i) * most * (D + 2);
@@ -347,7 +422,7 @@ static int launch_paged(const PagedParams& p, bool cap, int bias, hipStream_t st
     if (bias == 0) ODIT_PAGED_GO(false, 0); else if (bias == 1) ODIT_PAGED_GO(false, 1); else ODIT_PAGED_GO(false, 2);
   }
 #undef ODIT_PAGED_GO
-  if (p.splits > 1) hipLaunchKernelGGL((attn_paged_merge_kernel<T, D>), dim3(p.B * p.H), dim3(256), 0, stream, p);
+  if (p.splits > 1 && p.tickets == nullptr) hipLaunchKernelGGL((attn_paged_merge_kernel<T, D>), dim3(p.B * p.H), dim3(256), 0, stream, p);
   return check_launch("odit_attn_paged");
 }
 
@@ -369,7 +444,7 @@ extern "C" int odit_attn_paged(const void* q, const void* key_cache, const void*
                                int B, int H, int Hkv, int D, int pages, int page_size, int max_pages, const int64_t q_strides[2],
                                const int64_t key_cache_strides[3], const int64_t value_cache_strides[3], int64_t table_stride,
                                const int64_t o_strides[2], float scale, const odit_attn_rules* rules, int dtype, void* workspace,
-                               size_t workspace_bytes, void* stream) {
+                               size_t workspace_bytes, unsigned* tickets, size_t n_tickets, void* stream) {
   using namespace odit;
   ODIT_CHECK_ARG(rules != nullptr, "odit_attn_paged: null rules");
   const odit_attn_rules& r = *rules;
@@ -424,6 +499,7 @@ extern "C" int odit_attn_paged(const void* q, const void* key_cache, const void*
   const PagedPlan plan = paged_plan(units, paged_most_keys(max_pages, page_size, r.window), page_size);
   p.chunk = plan.chunk; p.splits = plan.splits;
   p.ws = static_cast<float*>(workspace);
+  p.tickets = p.splits <= kPagedTickets && tickets != nullptr && n_tickets >= static_cast<size_t>(units) ? tickets : nullptr;
   const int bias = r.slopes != nullptr ? 1 : r.distance != nullptr ? 2 : 0;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == ODIT_BF16) return D == 128 ? launch_paged<bf16_t, 128>(p, r.cap > 0.f, bias, st) : launch_paged<bf16_t, 64>(p, r.cap > 0.f, bias, st);

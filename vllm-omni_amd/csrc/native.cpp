@@ -131,6 +131,8 @@ Tensor fresh(at::IntArrayRef sizes, const at::TensorOptions& opts) {
 PyObject* g_linear_scratch_fn = nullptr;  // (device index, stream) -> tensor
 PyObject* g_attn_scratch_fn = nullptr;    // (device index, stream, bytes) -> tensor
 
+PyObject* g_ticket_scratch_fn = nullptr;  // (device index, stream, bytes) -> tensor
+
 struct Scratch { void* p = nullptr; size_t bytes = 0; };
 using ScratchRef = c10::weak_intrusive_ptr<c10::TensorImpl>;
 using ScratchPool = std::map<std::pair<int, void*>, ScratchRef>;
@@ -170,6 +172,15 @@ bool attn_scratch(const Where& w, size_t bytes, Scratch* s) {
   static thread_local ScratchPool pool;
   return scratch_from(pool, w, bytes, s, [](const Where& w_, size_t n) {
     return PyObject_CallFunction(g_attn_scratch_fn, "inn", w_.device, reinterpret_cast<Py_ssize_t>(w_.stream),
+                                 static_cast<Py_ssize_t>(n));
+  });
+}
+
+// (not in a graph capture)
+bool ticket_scratch(const Where& w, size_t bytes, Scratch* s) {
+  static thread_local ScratchPool pool;
+  return scratch_from(pool, w, bytes, s, [](const Where& w_, size_t n) {
+    return PyObject_CallFunction(g_ticket_scratch_fn, "inn", w_.device, reinterpret_cast<Py_ssize_t>(w_.stream),
                                  static_cast<Py_ssize_t>(n));
   });
 }
@@ -697,11 +708,16 @@ PyObject* py_attn_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Tensor o = fresh({B, H, D}, q->options()), ws;
   const size_t need = odit_attn_paged_workspace_bytes(B, H, Hkv, D, table->size(1), page, r.window);
   if (need > 0) ws = fresh({static_cast<int64_t>(need)}, q->options().dtype(at::kByte));
+  Scratch tickets;
+  if (need > 0 && c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None &&
+      !ticket_scratch(w, static_cast<size_t>(B * Hkv * ((H / Hkv + 15) / 16)) * sizeof(unsigned), &tickets))
+    return nullptr;
   const int64_t qs[2] = {q->stride(0), q->stride(1)}, ks[3] = {k->stride(0), k->stride(1), k->stride(2)}, vs[3] = {v->stride(0), v->stride(1), v->stride(2)},
                 os[2] = {H * D, D};
   if (unlocked([&] { return odit_attn_paged(ptr(q), ptr(k), ptr(v), static_cast<const int*>(ptr(table)), static_cast<const int*>(ptr(len)), o.data_ptr(), B, H, Hkv, D,
                                             pages, page, table->size(1), qs, ks, vs, table->stride(0), os, static_cast<float>(scale), &r, dt,
-                                            need > 0 ? ws.data_ptr() : nullptr, need, w.stream); }) != 0)
+                                            need > 0 ? ws.data_ptr() : nullptr, need, static_cast<unsigned*>(tickets.p), tickets.bytes / sizeof(unsigned),
+                                            w.stream); }) != 0)
     return none();
   return wrap(std::move(o));
   NATIVE_END
@@ -2409,10 +2425,11 @@ PyObject* py_wan_block(PyObject*, PyObject* const* a, Py_ssize_t n) {
 // -------------------------------------------------------------------------------------------- module
 // (linear scratch, attention scratch)
 PyObject* py_configure(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (n != 2) { PyErr_SetString(PyExc_TypeError, "configure takes two callables"); return nullptr; }
-  Py_INCREF(a[0]); Py_INCREF(a[1]);
+  if (n != 3) { PyErr_SetString(PyExc_TypeError, "configure takes three callables"); return nullptr; }
+  Py_INCREF(a[0]); Py_INCREF(a[1]); Py_INCREF(a[2]);
   Py_XSETREF(g_linear_scratch_fn, a[0]);
   Py_XSETREF(g_attn_scratch_fn, a[1]);
+  Py_XSETREF(g_ticket_scratch_fn, a[2]);
   Py_RETURN_NONE;
 }
 

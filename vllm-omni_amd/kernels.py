@@ -48,7 +48,7 @@ def _load_native():
     """The native module, told where its scratch comes from and which modules its block functions know."""
     global _nat
     nat = _lib.native()
-    nat.configure(_linear_scratch, _attn_scratch)
+    nat.configure(_linear_scratch, _attn_scratch, _paged_tickets)
     nat.classes(_NATIVE_CLASSES)
     _nat = nat
     return nat
@@ -418,6 +418,15 @@ def attn_ruled(
     return o
 
 
+_PAGED_TICKETS = _Scratch()
+
+
+def _paged_tickets(device: int, stream: int, need: int) -> torch.Tensor:
+    """Words that the workgroups of one ``attn_paged`` launch find their last with: zero between launches. (Not asked for in a graph capture: two
+    captured graphs may run side by side, and the join is a launch of its own there.)"""
+    return _PAGED_TICKETS.get(device, stream, max(need, 4096))
+
+
 def _cache(name: str, t: torch.Tensor, Hkv: int | None, D: int, like: torch.Tensor) -> None:
     """Checks of one part of a paged cache (which is never copied)."""
     if t.dim() != 4 or (Hkv is not None and t.shape[2] != Hkv) or t.shape[3] != D or t.shape[1] == 0:
@@ -472,7 +481,7 @@ def attn_paged(
         rc = lib.odit_attn_paged(
             q.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), table.data_ptr(), lengths.data_ptr(), o.data_ptr(), B, H, Hkv, D,
             pages, page, n, _lib.i64_array(q.stride()[:2]), _lib.i64_array(key_cache.stride()[:3]), _lib.i64_array(value_cache.stride()[:3]),
-            n, _lib.i64_array((H * D, D)), float(scale), _lib.C.byref(rules), _code(q), _ptr(ws), need, _stream())
+            n, _lib.i64_array((H * D, D)), float(scale), _lib.C.byref(rules), _code(q), _ptr(ws), need, None, 0, _stream())
     _lib.check(rc, "odit_attn_paged")
     return o
 
