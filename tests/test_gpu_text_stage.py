@@ -286,6 +286,15 @@ def test_decode_many_chunks(gpu, lengths, D, dtype):
         assert torch.equal(a, want) and torch.equal(b, o) and torch.equal(c, want)
 
 
+@pytest.mark.parametrize("B,most", [(63, 700), (64, 700), (65, 300), (200, 200)])
+def test_decode_many_sequences(gpu, B, most):
+    """More sequences than a wavefront has lanes, of any lengths."""
+    g = torch.Generator().manual_seed(B)
+    (q, kc, vc, table, n), rows = _paged_problem(9, torch.randint(0, most, (B,), generator=g).tolist(), 16, 2, 1, 64, BF16)
+    for window in (None, 100):
+        _check_paged(q, rows, kernels.attn_paged(q, kc, vc, table, n, 0.1, window=window), 0.1, window, 0.0, {})
+
+
 def test_decode_strides_and_long_tables(gpu):
     """Keys and values as halves of one cache with the head ahead of the row; a table and lengths that are parts of larger ones; a table for far
     more pages than there are (many chunks, most of them empty)."""

@@ -7,27 +7,36 @@
 // another workgroup) are the columns of v_mfma_f32_16x16x32 in both products, S^T = K Q^T and O^T = V^T P^T, so that the arithmetic costs the
 // same for one head as for 16 and stays far below the loads. A lane then owns one head and the same keys in both products: P stays in registers.
 //
-// A sequence's keys are cut into chunks, a workgroup each; a chunk's tiles of 32 keys go round its 4 wavefronts. A wavefront has two stages
+// The sequences' keys are cut into chunks, a workgroup each; a chunk's tiles of 16 keys go round its 4 wavefronts. A wavefront has two stages
 // of LDS of its own and fills one, 16 bytes a lane straight from global memory, while it computes the other: no barrier in the loop. The page
-// numbers of the chunk wait in LDS, so nothing else is loaded there. The wavefronts' sums are joined in LDS; the chunks' by a second launch.
+// numbers of the chunk wait in LDS, so nothing else is loaded there. (Tiles of 32 keys leave room for one workgroup of head size 128 on a compute
+// unit, and nothing runs while it begins and ends: 8 sequences of 4096 keys 37 to 51 us, so 31.) The wavefronts' sums are joined in LDS, the
+// chunks' by the last workgroup of a sequence to be done, or by a second launch.
 //
 // Rows behind a sequence's last key are never read, as a page may hold anything there: the tile's rest is the last key again, with no
 // weight and values of zero.
+#include <type_traits>
+
 #include "attn_rules.h"
 
 namespace odit {
 
+typedef short s16x4_p __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x4_p __attribute__((ext_vector_type(4)));
 template <typename T> struct Mma16;
 template <> struct Mma16<bf16_t> {
   using frag = bf16x8_v;
   static __device__ __forceinline__ f32x4_v run(frag a, frag b, f32x4_v c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+  static __device__ __forceinline__ f32x4_v half(s16x4_p a, s16x4_p b, f32x4_v c) { return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, b, c, 0, 0, 0); }
 };
 template <> struct Mma16<f16_t> {
   using frag = f16x8_v;
   static __device__ __forceinline__ f32x4_v run(frag a, frag b, f32x4_v c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+  static __device__ __forceinline__ f32x4_v half(s16x4_p a, s16x4_p b, f32x4_v c) {
+    return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4_p, a), __builtin_bit_cast(f16x4_p, b), c, 0, 0, 0);
+  }
 };
 
-typedef short s16x4_p __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4_p* lds_s16x4_pp;
 typedef __attribute__((address_space(3))) void* lds_void_pp;
 
@@ -42,15 +51,17 @@ struct PagedParams {
   int64_t qs_b, qs_h, kc_p, kc_r, kc_h, vc_p, vc_r, vc_h, ts, os_b, os_h;
   float scale_log2;
   Cap cap;
-  int group, head_blocks, units, splits, chunk;
-  float* ws;  // per unit and split: [heads of a block][D] sums, then [heads of a block] (maximum, sum)
-  unsigned* tickets;  // a word for each unit, zero between launches (nullptr: the join is a launch of its own)
+  int group, head_blocks, units;  // units: key heads' blocks of up to 16 query heads, of one sequence
+  int wanted, room;               // chunks of all sequences, about, and the most keys of one
+  float* ws;  // per chunk and unit: [heads of a block][D] sums, then [heads of a block] (maximum, sum)
+  unsigned* tickets;  // a word for each sequence and unit, zero between launches (nullptr: the join is a launch of its own)
 };
 
-// The join by the last workgroup costs it a trip to memory behind the others (1 us) where a launch of its own costs 2.6 us and 3 of the
-// host's; it holds all chunks' parts at once, so it is for up to kPagedTickets of them.
-constexpr int kPagedTickets = 16;
-constexpr int kPagedWaves = 4, kPagedTile = 32, kPagedEntries = 1024;
+constexpr int kPagedWaves = 4, kPagedTile = 16, kPagedEntries = 1024, kPagedStep = kPagedWaves * kPagedTile;
+constexpr int kPagedLeast = 2;  // steps of a chunk: with one, a sequence of 1000 keys takes 9.7 us, with two 8.4
+constexpr int kPagedWanted = 512;  // workgroups: two to a compute unit at head size 128 (us, 448 / 512 / 640 / 768: 4 sequences of 100000 to 131072 keys
+                                   // 345 / 335 / 366 / 362, 8 of 4096 33 / 31 / 35 / 36, one of 32768 37 / 36 / 41 / 41; head size 64 the same)
+constexpr int kPagedJoin = 12;  // chunks whose parts are loaded at once (at head size 64 16 wavefronts share a compute unit's registers)
 // keys of a sequence of this length that its query sees: [first, end)
 __device__ __forceinline__ void paged_range(const PagedParams& p, int length, int* first, int* end) {
   const int64_t most = static_cast<int64_t>(p.max_pages) * p.page;
@@ -59,6 +70,90 @@ __device__ __forceinline__ void paged_range(const PagedParams& p, int length, in
   if (n < 0) n = 0;
   *end = n;
   *first = p.window > 0 && n > p.window ? n - p.window : 0;
+}
+
+// the wavefront's sum in every lane, and the sum of the lanes up to this one
+__device__ __forceinline__ int wave_sum_int(int v) {
+  const auto moved = [](int x, auto ctrl) { return __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, 0xf, 0xf, false); };
+  v += moved(v, std::integral_constant<int, 0xB1>());
+  v += moved(v, std::integral_constant<int, 0x4E>());
+  v += moved(v, std::integral_constant<int, 0x141>());
+  v += moved(v, std::integral_constant<int, 0x140>());
+  return __builtin_amdgcn_readlane(v, 0) + __builtin_amdgcn_readlane(v, 16) + __builtin_amdgcn_readlane(v, 32) + __builtin_amdgcn_readlane(v, 48);
+}
+__device__ __forceinline__ int wave_scan_int(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr by 1, 2, 4, 8: within 16 lanes
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast of lane 15 to the second and fourth 16, of lane 31 to the upper half
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+  return v;
+}
+
+// How the sequences are cut, from their lengths, which the host does not know: into chunks of one size, whole steps of the workgroup, numbered
+// sequence by sequence, about `wanted` in all (what runs at once), and no more than that where the sequences are few, as one chunk more would
+// then have the others' time again. Cut by the longest that the table has room for instead, into 2048: 8 sequences of 4096 keys 38 us where
+// this takes 31, 48 of 17 to 8192 67 and 62; and what is short in a wide table would run on few compute units.
+// Every wavefront works it out by itself, for the chunk `index` (BY_CHUNK) or for the sequence `index`.
+struct PagedPlace { int b, part, parts, before, chunk, length; };  // before: chunks of the sequences ahead
+template <bool BY_CHUNK>
+__device__ __forceinline__ PagedPlace paged_place(const PagedParams& p, int index) {
+  const int lane = threadIdx.x & 63;
+  const auto keys_of = [&](int b, int* length) {
+    *length = b < p.B ? p.lengths[b] : 0;
+    int first, end;
+    paged_range(p, *length, &first, &end);
+    return b < p.B ? end - first : 0;
+  };
+  const auto parts_of = [&](int b, int keys, int chunk) {
+    return b < p.B ? max(1, static_cast<int>((static_cast<uint32_t>(keys) + chunk - 1) / static_cast<uint32_t>(chunk))) : 0;
+  };
+  int length;
+  const int mine = keys_of(lane, &length);
+  int chunk;
+  if (p.B <= 64) {
+    // (in steps, so that the sum of 64 stays in 32 bits)
+    const int steps = wave_sum_int((mine + kPagedStep - 1) / kPagedStep);
+    int each = max(kPagedLeast, (steps + p.wanted - 1) / p.wanted);
+    if (4 * p.B <= p.wanted) {
+      for (int i = 0; i < 3; ++i) {
+        const int made = wave_sum_int(parts_of(lane, mine, each * kPagedStep));
+        if (made <= p.wanted) break;
+        each = static_cast<int>(static_cast<int64_t>(each) * made / p.wanted) + 1;
+      }
+    }
+    chunk = min(each, p.room / kPagedStep) * kPagedStep;
+  } else {
+    double total = mine;  // (exact: below 2^53)
+    for (int b0 = 64; b0 < p.B; b0 += 64) {
+      int other;
+      total += keys_of(b0 + lane, &other);
+    }
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) total += __shfl_xor(total, s, 64);
+    const double each = ceil(total / (static_cast<double>(p.wanted) * kPagedStep));
+    chunk = static_cast<int>(each < kPagedLeast ? kPagedLeast : each > p.room / kPagedStep ? p.room / kPagedStep : each) * kPagedStep;
+  }
+  chunk = max(__builtin_amdgcn_readfirstlane(chunk), kPagedStep);
+  PagedPlace at{p.B, 0, 0, 0, chunk, 0};
+  int before = 0, keys = mine;
+  for (int b0 = 0; b0 < p.B; b0 += 64) {
+    if (b0 > 0) keys = keys_of(b0 + lane, &length);
+    const int parts = parts_of(b0 + lane, keys, chunk), upto = wave_scan_int(parts);  // of this sequence and those ahead of it among the 64
+    const uint64_t ahead = __ballot(BY_CHUNK ? before + upto <= index : b0 + lane < index);
+    const int l = __popcll(ahead);
+    if (l < 64) {
+      at.b = b0 + l;
+      at.parts = __builtin_amdgcn_readlane(parts, l);
+      at.before = before + __builtin_amdgcn_readlane(upto, l) - at.parts;
+      at.part = BY_CHUNK ? index - at.before : 0;
+      at.length = __builtin_amdgcn_readlane(length, l);
+      return at;
+    }
+    before += __builtin_amdgcn_readlane(upto, 63);
+  }
+  return at;  // (b == B: behind the last chunk)
 }
 
 // 16 bytes per lane from the lane's own address to LDS bytes lds + 16 * lane
@@ -81,68 +176,72 @@ __device__ __forceinline__ float2 get_pair(const float* at) {
   return make_float2(__uint_as_float(static_cast<uint32_t>(x)), __uint_as_float(static_cast<uint32_t>(x >> 32)));
 }
 
-// Up to kPagedTickets chunks' sums joined, features d and d + 1 of head hd: o = sum_c 2^(m_c - m) o_c / sum_c 2^(m_c - m) l_c, m = max_c m_c.
-// All loads are ahead of their first use.
+// A sequence's chunks joined, features d and d + 1 of head hd: o = sum_c 2^(m_c - m) o_c / sum_c 2^(m_c - m) l_c, m = max_c m_c, in the chunks'
+// order. kPagedJoin chunks' loads are on their way at once. part0: the first chunk's part, `step` floats ahead of the next one's.
 template <typename T, int D>
-__device__ __forceinline__ uint32_t join_few(const float* part0, int most, int hd, int d, int parts) {
-  float2 ml[kPagedTickets], x[kPagedTickets];
-#pragma unroll
-  for (int c = 0; c < kPagedTickets; ++c) {
-    if (c < parts) {
-      const float* const part = part0 + c * most * (D + 2);
-      ml[c] = get_pair(part + most * D + 2 * hd);
-      x[c] = get_pair(part + hd * D + d);
-    }
-  }
+__device__ __forceinline__ uint32_t join_parts(const float* part0, int64_t step, int most, int hd, int d, int parts) {
   float m = -INFINITY, l = 0.f, x0 = 0.f, x1 = 0.f;
+  const uint32_t at_ml = most * D + 2 * hd, at_x = hd * D + d;
+  for (int c0 = 0; c0 < parts; c0 += kPagedJoin) {
+    float2 ml[kPagedJoin], x[kPagedJoin];
 #pragma unroll
-  for (int c = 0; c < kPagedTickets; ++c)
-    if (c < parts) m = fmaxf(m, ml[c].x);
-  const float m_safe = m == -INFINITY ? 0.f : m;
+    for (int c = 0; c < kPagedJoin; ++c) {
+      if (c0 + c < parts) {
+        const float* const part = part0 + (c0 + c) * step;
+        ml[c] = get_pair(part + at_ml);
+        x[c] = get_pair(part + at_x);
+      }
+    }
+    float m_new = m;
 #pragma unroll
-  for (int c = 0; c < kPagedTickets; ++c) {
-    if (c < parts) {
-      const float a = __builtin_amdgcn_exp2f(ml[c].x - m_safe);
-      l = fmaf(a, ml[c].y, l);
-      x0 = fmaf(a, x[c].x, x0);
-      x1 = fmaf(a, x[c].y, x1);
+    for (int c = 0; c < kPagedJoin; ++c)
+      if (c0 + c < parts) m_new = fmaxf(m_new, ml[c].x);
+    const float m_safe = m_new == -INFINITY ? 0.f : m_new, a0 = __builtin_amdgcn_exp2f(m - m_safe);
+    m = m_new;
+    l *= a0; x0 *= a0; x1 *= a0;
+#pragma unroll
+    for (int c = 0; c < kPagedJoin; ++c) {
+      if (c0 + c < parts) {
+        const float a = __builtin_amdgcn_exp2f(ml[c].x - m_safe);
+        l = fmaf(a, ml[c].y, l);
+        x0 = fmaf(a, x[c].x, x0);
+        x1 = fmaf(a, x[c].y, x1);
+      }
     }
   }
   return l == 0.f ? 0u : Mma<T>::pack2(x0 / l, x1 / l);
 }
 
 template <typename T, int D, bool CAP, int BIAS>
-__global__ __launch_bounds__(256) void attn_paged_kernel(const PagedParams p) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 4 : 2))) void attn_paged_kernel(const PagedParams p) {
   using M = Mma16<T>;
   using frag = typename M::frag;
   constexpr int NW = kPagedWaves, BN = kPagedTile;
   constexpr int ROWB = D * 2, CPR = ROWB / 16, RPI = 64 / CPR, TILEB = BN * ROWB, IPT = BN / RPI;
-  constexpr int KS = D / 32, DT = D / 16;
+  constexpr int KS = D / 32, DT = D / 16, NK = BN / 16;
   __shared__ __attribute__((aligned(1024))) char lds[NW * 4 * TILEB];  // of each wavefront: K0 V0 K1 V1
   __shared__ int entries[kPagedEntries];
   __shared__ int outside[NW];  // whether a wavefront found page numbers that are none of the cache's
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l16 = lane & 15, g = lane >> 4;
-  const int unit = blockIdx.x % p.units, split = blockIdx.x / p.units;
-  const int hb = unit % p.head_blocks, hkv = unit / p.head_blocks % p.Hkv, b = unit / p.head_blocks / p.Hkv;
+  const int unit = blockIdx.x % p.units;
+  const PagedPlace at = paged_place<true>(p, blockIdx.x / p.units);
+  if (at.b >= p.B) return;
+  const int hb = unit % p.head_blocks, hkv = unit / p.head_blocks, b = at.b;
   const int h0 = hkv * p.group + hb * 16, heads = min(16, p.group - hb * 16);
   const int h = h0 + min(l16, heads - 1);  // this lane's head
   const auto page_of = [&](int key) { return static_cast<int>(static_cast<uint64_t>(static_cast<uint32_t>(key)) * p.page_mul >> p.page_shift); };
 
-  // Without a window a chunk's place does not depend on the sequence's length: its page numbers are on their way while that is (one trip to
-  // memory of four in a call of one short sequence)
-  const int length = p.lengths[b];
-  int first = 0, n = p.max_pages * p.page;  // (up to 2^30)
-  if (p.window > 0) paged_range(p, length, &first, &n);
-  const int begin = first + split * p.chunk;
-  const int pg0 = page_of(begin);
-  int bad = 0x7fffffff;  // the first of this thread's page numbers that is none
-  if (n > begin) {
-    const int npg = page_of(min(n, begin + p.chunk) - 1) - pg0 + 1;
+  int first, n;
+  paged_range(p, at.length, &first, &n);
+  const int parts = at.parts, begin = first + at.part * at.chunk, end = min(n, begin + at.chunk), pg0 = page_of(begin);
+  bool bad = false;
+  if (end > begin) {
+    const int npg = page_of(end - 1) - pg0 + 1;
     for (int i = tid; i < npg; i += NW * 64) {
       int e = p.table[b * p.ts + pg0 + i];
-      if (e < 0 || e >= p.pages) { e = -1; bad = min(bad, i); }
+      if (e < 0 || e >= p.pages) { e = -1; bad = true; }
       entries[i] = e;
     }
   }
@@ -153,12 +252,8 @@ __global__ __launch_bounds__(256) void attn_paged_kernel(const PagedParams p) {
   const float slope = BIAS == 1 ? p.slopes[h] * kLog2e : 0.f;
   const float* const dist = BIAS == 2 ? p.distance + static_cast<int64_t>(h) * (2 * p.radius + 1) + p.radius : nullptr;  // [away]
   const float far = BIAS == 2 ? dist[-p.radius] * kLog2e : 0.f;
-  if (p.window == 0) paged_range(p, length, &first, &n);
-  const int parts = max(1, (n - first + p.chunk - 1) / p.chunk);  // of this sequence; an empty one has one, too
-  if (split >= parts) return;
-  const int end = min(n, begin + p.chunk);
   {
-    const bool any = __any(end > begin && bad <= page_of(end - 1) - pg0);  // (pages behind the sequence's last key may be anything)
+    const bool any = __any(bad);
     if (lane == 0) outside[wave] = any;
   }
   __syncthreads();
@@ -210,8 +305,7 @@ __global__ __launch_bounds__(256) void attn_paged_kernel(const PagedParams p) {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the stage that is filled next has been read
     if (i + 1 < mine) {
       load_tile(i + 1);
-      if constexpr (IPT == 8) asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
-      else asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+      asm volatile("s_waitcnt vmcnt(%0)" : : "n"(2 * IPT) : "memory");  // all but the loads of the tile just asked for
     } else {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
@@ -219,11 +313,13 @@ __global__ __launch_bounds__(256) void attn_paged_kernel(const PagedParams p) {
     const char* const vb = kb + TILEB;
     const int k0 = begin + (wave + i * NW) * BN;
     const bool rest = k0 + BN > end || invalid;
-    f32x4_v s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    f32x4_v s[NK];
+#pragma unroll
+    for (int kt = 0; kt < NK; ++kt) s[kt] = f32x4_v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int st = 0; st < KS; ++st)
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
+      for (int kt = 0; kt < NK; ++kt)
         s[kt] = M::run(__builtin_bit_cast(frag, *reinterpret_cast<const u32x4_v*>(kb + kt * 16 * ROWB + (k_lane ^ (st * 64)))), qf[st], s[kt]);
     if (rest) {  // what stands in for keys that are none: values of zero, whatever the memory holds (0 times infinity is NaN)
 #pragma unroll
@@ -235,7 +331,7 @@ __global__ __launch_bounds__(256) void attn_paged_kernel(const PagedParams p) {
     }
     const bool near = BIAS == 2 && k0 + BN - 1 - (n - 1) > -p.radius;  // some key has a bias of its own
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
+    for (int kt = 0; kt < NK; ++kt)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int key = k0 + kt * 16 + g * 4 + e;
@@ -253,7 +349,7 @@ __global__ __launch_bounds__(256) void attn_paged_kernel(const PagedParams p) {
       }
     float mx = s[0][0];
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
+    for (int kt = 0; kt < NK; ++kt)
 #pragma unroll
       for (int e = 0; e < 4; ++e) mx = __builtin_elementwise_maximum(mx, s[kt][e]);
     if (__any((mx - m_run) * c > 8.f)) {  // (as in attn_fwd.hip: the maximum moves only where it is left behind by a factor of 2^8)
@@ -269,9 +365,9 @@ __global__ __launch_bounds__(256) void attn_paged_kernel(const PagedParams p) {
       m_run = m_new;
       mc = m_safe * c;
     }
-    u32x4_v pb;
+    uint32_t pb[2 * NK];
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
+    for (int kt = 0; kt < NK; ++kt)
 #pragma unroll
       for (int e = 0; e < 4; e += 2) {
         const float p0 = __builtin_amdgcn_exp2f(fmaf(s[kt][e], c, -mc)), p1 = __builtin_amdgcn_exp2f(fmaf(s[kt][e + 1], c, -mc));
@@ -282,8 +378,16 @@ __global__ __launch_bounds__(256) void attn_paged_kernel(const PagedParams p) {
     for (int dt = 0; dt < DT; ++dt) {
       const char* const vp = vb + (v_lane ^ (dt * 32));
       const s16x4_p lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_pp)(vp));
-      const s16x4_p hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_pp)(vp + 16 * ROWB));
-      o[dt] = M::run(__builtin_bit_cast(frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7)), __builtin_bit_cast(frag, pb), o[dt]);
+      if constexpr (NK == 2) {
+        const s16x4_p hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_pp)(vp + 16 * ROWB));
+        u32x4_v w;
+        w.x = pb[0]; w.y = pb[1]; w.z = pb[2]; w.w = pb[3];
+        o[dt] = M::run(__builtin_bit_cast(frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7)), __builtin_bit_cast(frag, w), o[dt]);
+      } else {
+        u32x2_v w;
+        w.x = pb[0]; w.y = pb[1];
+        o[dt] = M::half(lo, __builtin_bit_cast(s16x4_p, w), o[dt]);
+      }
     }
   }
 
@@ -301,7 +405,8 @@ __global__ __launch_bounds__(256) void attn_paged_kernel(const PagedParams p) {
   __syncthreads();
   // what the call's chunks leave is written past the caches of this XCD, as another workgroup's may read it
   const int most = min(16, p.group);
-  float* const part0 = p.ws + static_cast<int64_t>(unit) * p.splits * most * (D + 2);
+  const int64_t step = static_cast<int64_t>(p.units) * most * (D + 2);
+  float* const part0 = p.ws + at.before * step + static_cast<int64_t>(unit) * most * (D + 2);
   for (int i = tid; i < heads * (D / 2); i += NW * 64) {
     const int hd = i / (D / 2), d = i % (D / 2) * 2;
     float m = -INFINITY;
@@ -319,7 +424,7 @@ __global__ __launch_bounds__(256) void attn_paged_kernel(const PagedParams p) {
     if (parts == 1) {
       *reinterpret_cast<uint32_t*>(static_cast<T*>(p.o) + b * p.os_b + (h0 + hd) * p.os_h + d) = l == 0.f ? 0u : Mma<T>::pack2(x0 / l, x1 / l);
     } else {
-      float* const part = part0 + split * most * (D + 2);
+      float* const part = part0 + at.part * step;
       put_pair(part + hd * D + d, x0, x1);
       if (d == 0) put_pair(part + most * D + 2 * hd, m, l);
     }
@@ -330,80 +435,43 @@ __global__ __launch_bounds__(256) void attn_paged_kernel(const PagedParams p) {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wavefront's part is where the others see it
   __syncthreads();
   if (tid == 0) {
-    const unsigned before = __hip_atomic_fetch_add(p.tickets + unit, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const unsigned before = __hip_atomic_fetch_add(p.tickets + b * p.units + unit, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     is_last = before == static_cast<unsigned>(parts - 1);
-    if (is_last) __hip_atomic_store(p.tickets + unit, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (is_last) __hip_atomic_store(p.tickets + b * p.units + unit, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   __syncthreads();
   if (!is_last) return;
   for (int i = tid; i < heads * (D / 2); i += NW * 64) {
     const int hd = i / (D / 2), d = i % (D / 2) * 2;
-    *reinterpret_cast<uint32_t*>(static_cast<T*>(p.o) + b * p.os_b + (h0 + hd) * p.os_h + d) = join_few<T, D>(part0, most, hd, d, parts);
+    *reinterpret_cast<uint32_t*>(static_cast<T*>(p.o) + b * p.os_b + (h0 + hd) * p.os_h + d) = join_parts<T, D>(part0, step, most, hd, d, parts);
   }
 }
 
-// one workgroup a head of a sequence: its wavefronts go round the chunks' sums
+// the join as a launch of its own: a wavefront (or its first half) for each sequence and head
 template <typename T, int D>
-__global__ __launch_bounds__(256) void attn_paged_merge_kernel(const PagedParams p) {
-  constexpr int EPL = D / 64;
-  __shared__ float jo[4][D], jml[4][2];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int h = blockIdx.x % p.H, b = blockIdx.x / p.H;
-  const int hkv = h / p.group, hb = h % p.group / 16, hd = h % p.group % 16;
-  const int64_t unit = (static_cast<int64_t>(b) * p.Hkv + hkv) * p.head_blocks + hb;
-  int first, n;
-  paged_range(p, p.lengths[b], &first, &n);
-  const int parts = (n - first + p.chunk - 1) / p.chunk, most = min(16, p.group);
-  if (parts <= 1) return;  // (written by its only workgroup)
-  if (parts <= kPagedTickets) {
-    const int d = threadIdx.x * 2;
-    if (d < D)
-      *reinterpret_cast<uint32_t*>(static_cast<T*>(p.o) + b * p.os_b + h * p.os_h + d) = join_few<T, D>(p.ws + unit * p.splits * most * (D + 2), most, hd, d, parts);
-    return;
-  }
-  float m = -INFINITY, l = 0.f, x[EPL] = {};
-  for (int i = wave; i < parts; i += 4) {
-    const float* const part = p.ws + (unit * p.splits + i) * most * (D + 2);
-    const float pm = part[most * D + 2 * hd], pl = part[most * D + 2 * hd + 1];
-    const float m_new = fmaxf(m, pm), m_safe = m_new == -INFINITY ? 0.f : m_new;
-    const float a = __builtin_amdgcn_exp2f(m - m_safe), w = __builtin_amdgcn_exp2f(pm - m_safe);
-    m = m_new;
-    l = fmaf(l, a, w * pl);
-#pragma unroll
-    for (int e = 0; e < EPL; ++e) x[e] = fmaf(x[e], a, w * part[hd * D + lane * EPL + e]);
-  }
-#pragma unroll
-  for (int e = 0; e < EPL; ++e) jo[wave][lane * EPL + e] = x[e];
-  if (lane == 0) { jml[wave][0] = m; jml[wave][1] = l; }
-  __syncthreads();
-  if (threadIdx.x < D) {
-    float mm = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) mm = fmaxf(mm, jml[w][0]);
-    const float m_safe = mm == -INFINITY ? 0.f : mm;
-    float ll = 0.f, y = 0.f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float a = __builtin_amdgcn_exp2f(jml[w][0] - m_safe);
-      ll = fmaf(a, jml[w][1], ll);
-      y = fmaf(a, jo[w][threadIdx.x], y);
-    }
-    static_cast<T*>(p.o)[b * p.os_b + h * p.os_h + threadIdx.x] = from_float<T>(ll == 0.f ? 0.f : y / ll);
-  }
+__global__ __launch_bounds__(64) void attn_paged_join_kernel(const PagedParams p) {
+  const int h = blockIdx.x % p.H, b = blockIdx.x / p.H, d = threadIdx.x * 2;
+  const PagedPlace at = paged_place<false>(p, b);
+  if (at.parts <= 1 || d >= D) return;  // (one chunk's workgroup has written the result)
+  const int most = min(16, p.group), unit = h / p.group * p.head_blocks + h % p.group / 16, hd = h % p.group % 16;
+  const int64_t step = static_cast<int64_t>(p.units) * most * (D + 2);
+  *reinterpret_cast<uint32_t*>(static_cast<T*>(p.o) + b * p.os_b + h * p.os_h + d) =
+      join_parts<T, D>(p.ws + at.before * step + static_cast<int64_t>(unit) * most * (D + 2), step, most, hd, d, at.parts);
 }
 
-// How the keys of a call are cut: the host knows the longest that a sequence can be, not how long each is. Chunks are of whole tiles for
-// each wavefront, small enough that the call has some workgroups for every compute unit, and their page numbers fit kPagedEntries.
-struct PagedPlan { int chunk, splits; };
-static PagedPlan paged_plan(int64_t units, int64_t most_keys, int page) {
-  constexpr int64_t kStep = kPagedWaves * kPagedTile;
-  int64_t chunk = (most_keys * units + 2047) / 2048;
-  chunk = (chunk + kStep - 1) / kStep * kStep;
-  const int64_t room = static_cast<int64_t>(kPagedEntries - 1) * page / kStep * kStep;  // (a chunk may begin inside a page)
-  if (chunk > room) chunk = room;
-  if (chunk < kStep) chunk = kStep;
-  const int64_t splits = (most_keys + chunk - 1) / chunk;
-  return {static_cast<int>(chunk), static_cast<int>(splits < 1 ? 1 : splits)};
+// The most chunks that any lengths can make, and what the kernels work them out from. Where a chunk's page numbers have to fit kPagedEntries
+// it may have to be smaller than wanted.
+struct PagedPlan { int wanted, room; int64_t chunks; };
+static PagedPlan paged_plan(int B, int units, int64_t most_keys, int page) {
+  PagedPlan plan;
+  plan.wanted = kPagedWanted / units < 1 ? 1 : kPagedWanted / units;
+  int64_t room = static_cast<int64_t>(kPagedEntries - 1) * page / kPagedStep * kPagedStep;  // (a chunk may begin inside a page)
+  if (room > 1 << 29) room = 1 << 29;
+  plan.room = static_cast<int>(room < kPagedStep ? kPagedStep : room);
+  // (each sequence's last chunk may be a part of one)
+  const int64_t by_room = (B * most_keys + plan.room - 1) / plan.room;
+  plan.chunks = B + (most_keys <= kPagedLeast * kPagedStep ? 0 : by_room > plan.wanted ? by_room : plan.wanted);
+  return plan;
 }
 
 static int64_t paged_most_keys(int64_t max_pages, int page, int window) {
@@ -412,8 +480,8 @@ static int64_t paged_most_keys(int64_t max_pages, int page, int window) {
 }
 
 template <typename T, int D>
-static int launch_paged(const PagedParams& p, bool cap, int bias, hipStream_t stream) {
-  const int64_t grid = static_cast<int64_t>(p.units) * p.splits;
+static int launch_paged(const PagedParams& p, int64_t chunks, bool cap, int bias, hipStream_t stream) {
+  const int64_t grid = p.units * chunks;
   ODIT_CHECK_ARG(grid <= 0x7fffffffll, "odit_attn_paged: grid of %lld workgroups is too large", static_cast<long long>(grid));
 #define ODIT_PAGED_GO(C, X) hipLaunchKernelGGL((attn_paged_kernel<T, D, C, X>), dim3(grid), dim3(256), 0, stream, p)
   if (cap) {
@@ -422,7 +490,7 @@ static int launch_paged(const PagedParams& p, bool cap, int bias, hipStream_t st
     if (bias == 0) ODIT_PAGED_GO(false, 0); else if (bias == 1) ODIT_PAGED_GO(false, 1); else ODIT_PAGED_GO(false, 2);
   }
 #undef ODIT_PAGED_GO
-  if (p.splits > 1 && p.tickets == nullptr) hipLaunchKernelGGL((attn_paged_merge_kernel<T, D>), dim3(p.B * p.H), dim3(256), 0, stream, p);
+  if (chunks > p.B && p.tickets == nullptr) hipLaunchKernelGGL((attn_paged_join_kernel<T, D>), dim3(p.B * p.H), dim3(64), 0, stream, p);
   return check_launch("odit_attn_paged");
 }
 
@@ -433,11 +501,9 @@ static int paged_head_blocks(int H, int Hkv) { return (H / Hkv + 15) / 16; }
 extern "C" size_t odit_attn_paged_workspace_bytes(int B, int H, int Hkv, int D, int max_pages, int page_size, int window) {
   using namespace odit;
   if (B <= 0 || H <= 0 || Hkv <= 0 || H % Hkv != 0 || D <= 0 || max_pages <= 0 || page_size <= 0) return 0;
-  const int64_t units = static_cast<int64_t>(B) * Hkv * paged_head_blocks(H, Hkv);
-  const PagedPlan plan = paged_plan(units, paged_most_keys(max_pages, page_size, window), page_size);
-  if (plan.splits == 1) return 0;
-  const int heads = H / Hkv < 16 ? H / Hkv : 16;
-  return static_cast<size_t>(units) * plan.splits * heads * (D + 2) * sizeof(float);
+  const int units = Hkv * paged_head_blocks(H, Hkv), heads = H / Hkv < 16 ? H / Hkv : 16;
+  const PagedPlan plan = paged_plan(B, units, paged_most_keys(max_pages, page_size, window), page_size);
+  return plan.chunks > B ? static_cast<size_t>(plan.chunks) * units * heads * (D + 2) * sizeof(float) : 0;
 }
 
 extern "C" int odit_attn_paged(const void* q, const void* key_cache, const void* value_cache, const int* table, const int* lengths, void* o,
@@ -494,14 +560,13 @@ extern "C" int odit_attn_paged(const void* q, const void* key_cache, const void*
   p.scale_log2 = scale * kLog2e;
   p.cap = make_cap(r.cap, scale);
   p.group = H / Hkv; p.head_blocks = paged_head_blocks(H, Hkv);
-  const int64_t units = static_cast<int64_t>(B) * Hkv * p.head_blocks;
-  p.units = static_cast<int>(units);
-  const PagedPlan plan = paged_plan(units, paged_most_keys(max_pages, page_size, r.window), page_size);
-  p.chunk = plan.chunk; p.splits = plan.splits;
+  p.units = Hkv * p.head_blocks;
+  const PagedPlan plan = paged_plan(B, p.units, paged_most_keys(max_pages, page_size, r.window), page_size);
+  p.wanted = plan.wanted; p.room = plan.room;
   p.ws = static_cast<float*>(workspace);
-  p.tickets = p.splits <= kPagedTickets && tickets != nullptr && n_tickets >= static_cast<size_t>(units) ? tickets : nullptr;
+  p.tickets = tickets != nullptr && n_tickets >= static_cast<size_t>(B) * p.units ? tickets : nullptr;
   const int bias = r.slopes != nullptr ? 1 : r.distance != nullptr ? 2 : 0;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (dtype == ODIT_BF16) return D == 128 ? launch_paged<bf16_t, 128>(p, r.cap > 0.f, bias, st) : launch_paged<bf16_t, 64>(p, r.cap > 0.f, bias, st);
-  return D == 128 ? launch_paged<f16_t, 128>(p, r.cap > 0.f, bias, st) : launch_paged<f16_t, 64>(p, r.cap > 0.f, bias, st);
+  if (dtype == ODIT_BF16) return D == 128 ? launch_paged<bf16_t, 128>(p, plan.chunks, r.cap > 0.f, bias, st) : launch_paged<bf16_t, 64>(p, plan.chunks, r.cap > 0.f, bias, st);
+  return D == 128 ? launch_paged<f16_t, 128>(p, plan.chunks, r.cap > 0.f, bias, st) : launch_paged<f16_t, 64>(p, plan.chunks, r.cap > 0.f, bias, st);
 }
