@@ -57,16 +57,17 @@ def test_ruled_takes_empty_problems():
 
 def test_ruled_workspace():
     """Few query blocks with many keys are cut, into at most 32; what fills the GPU, and what has few keys, is not."""
-    def chunks(B, Sq, Sk, H, D, **rules):
+    def chunks(B, Sq, Sk, H, D, block, **rules):
         need = _lib.load().odit_attn_ruled_workspace_bytes(B, Sq, Sk, H, D, C.byref(_lib.AttnRules(**rules)))
-        part = (Sq + 127) // 128 * H * B * 128 * (D + 2) * 4
+        part = (Sq + block - 1) // block * H * B * block * (D + 2) * 4
         assert need % part == 0
         return need // part or 1
 
-    assert chunks(1, 1, 8192, 8, 128) == 32 and 8 <= chunks(1, 100, 8192, 32, 64) <= 32
-    assert chunks(1, 1, 8192, 64, 128) == 8 and chunks(1, 1, 8192, 256, 128) == 2 and chunks(1, 1, 8192, 257, 128) == 1  # 512 of them run at once
-    assert chunks(1, 77, 77, 24, 128) == 1 and chunks(1, 16384, 16384, 16, 128) == 1
-    assert chunks(1, 1, 1 << 20, 8, 128, window=64, causal=1) == 1 and chunks(1, 64, 1 << 20, 8, 128, docs=1 << 16, q_starts=P, k_starts=P) == 1
+    assert chunks(1, 1, 8192, 8, 128, 64) > 16 and chunks(1, 100, 8192, 32, 64, 64) > 8
+    assert chunks(1, 1, 8192, 100, 128, 64) == 5 and chunks(1, 1, 8192, 256, 128, 128) == 2  # 512 workgroups run at once
+    assert chunks(1, 1, 8192, 257, 128, 128) == 1 and chunks(1, 77, 77, 24, 128, 64) == 1 and chunks(1, 16384, 16384, 16, 128, 128) == 1
+    assert chunks(1, 1, 1 << 20, 8, 128, 64, window=64, causal=1) == 1
+    assert chunks(1, 64, 1 << 20, 8, 128, 64, docs=1 << 16, q_starts=P, k_starts=P) == 1
     assert _lib.load().odit_attn_ruled_workspace_bytes(0, 1, 8192, 8, 128, C.byref(_lib.AttnRules())) == 0
 
 

@@ -31,8 +31,9 @@ struct RuledParams {
   float scale_log2, bias_scale;  // scale log2(e) and 1 / scale
   Cap cap;
   int n_qblocks, units;  // units: heads of all batch rows
+  int bm;                // queries of a block
   int chunks;            // workgroups that share a query block's tiles; with more than one, their sums go to ws
-  float* ws;             // [units][n_qblocks][chunks][128][D] sums, then [...][128] (maximum in units of log2, sum)
+  float* ws;             // [units][n_qblocks][chunks][bm][D] sums, then [...][bm] (maximum in units of log2, sum)
 };
 
 // Among 64 documents from `base` on, whose starts the lanes hold: the last one that starts at or before the lane's row, one of the 32 from
@@ -88,21 +89,22 @@ __device__ __forceinline__ uint64_t range_bits(int lo, int hi, int t0) {
   return upto & (~0ull << a);
 }
 
-// BIAS 0: none, 1: slopes, 2: table
-template <typename T, int D, bool CAP, int BIAS>
+// BIAS 0: none, 1: slopes, 2: table. KH: the 32-key halves of a tile that a wavefront has. With both, the workgroup's 4 wavefronts have 32
+// queries each; with one, two wavefronts share 32 queries, a half of each tile each, and join at the end (ruled_plan says when).
+template <typename T, int D, bool CAP, int BIAS, int KH>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 3 : 2, D == 64 ? 3 : 2)))
 void attn_ruled_kernel(const RuledParams p) {
   using M = Mma<T>;
   using frag = typename M::frag;
-  constexpr int NW = 4, BM = NW * 32, BN = 64;
+  constexpr int NW = 4, BM = NW * 16 * KH, BN = 64, NS = 16 * KH;  // NS: scores of a lane
   constexpr int KS = D / 16, DT = D / 32;
   constexpr int ROWB = D * 2, CPR = ROWB / 16, RPI = 64 / CPR, TILEB = BN * ROWB;
   constexpr int IPW = BN / RPI / NW;  // wave instructions of a tile's load, per wavefront
 
   __shared__ __attribute__((aligned(1024))) char lds[4 * TILEB];  // K0 K1 V0 V1
   __shared__ int bounds[NW][4];
-  __shared__ int places[BIAS != 0 ? BM : 1];  // pos of each lane's query
-  __shared__ int4 ranges[BM];  // blo, bhi, plo, phi of each lane's query: read again at each tile, which has no registers to hold them
+  __shared__ int places[BIAS != 0 ? NW * 32 : 1];  // pos of each lane's query
+  __shared__ int4 ranges[NW * 32];  // blo, bhi, plo, phi of each lane's query: read again at each tile, which has no registers to hold them
   // BIAS 2: the head's biases, with the outermost ones once more for each further key of a tile that some distance inside begins or ends
   constexpr int kPad = BN - 1;
   __shared__ float table[BIAS == 2 ? 2 * kMaxRadius + 1 + 2 * kPad : 1];
@@ -122,7 +124,8 @@ void attn_ruled_kernel(const RuledParams p) {
     qb = p.n_qblocks - 1 - block / p.units;
   }
   const int h = unit % p.H, b = unit / p.H, hkv = h / (p.H / p.Hkv);
-  const int q0 = qb * BM + wave * 32;
+  const int kt0 = KH == 1 ? wave >> 1 : 0;  // the first of this wavefront's halves
+  const int q0 = qb * BM + (KH == 1 ? wave & 1 : wave) * 32;
   const int row = q0 + l32 < p.Sq ? q0 + l32 : p.Sq - 1;
 
   const T* const qrow = static_cast<const T*>(p.q) + b * p.qs_b + h * p.qs_h + row * p.qs_s;
@@ -276,9 +279,9 @@ void attn_ruled_kernel(const RuledParams p) {
   float m_run = -INFINITY, l_run = 0.f, mc = 0.f;
   const float slope = BIAS == 1 ? p.slopes[h] * bias_unit : 0.f;
 
-  const int k_lane = l32 * ROWB + (((hh ^ (l32 % 16)) % CPR) << 4);
+  const int k_lane = (32 * kt0 + l32) * ROWB + (((hh ^ (l32 % 16)) % CPR) << 4);
   const int sq = (lane & 15) >> 2, dh = (lane >> 4) & 1;
-  const int v_lane = (4 * hh + sq) * ROWB + ((((4 * sq) % CPR) ^ (2 * dh + ((lane & 3) >> 1))) << 4) + ((lane & 1) << 3);
+  const int v_lane = (32 * kt0 + 4 * hh + sq) * ROWB + ((((4 * sq) % CPR) ^ (2 * dh + ((lane & 3) >> 1))) << 4) + ((lane & 1) << 3);
   auto swapped = [&](float x) __attribute__((always_inline)) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return __uint_as_float(hh ? r[0] : r[1]);
@@ -289,73 +292,76 @@ void attn_ruled_kernel(const RuledParams p) {
   const float kOut = POLY ? -1e18f : -INFINITY;
   // whether some query of the wavefront sees a key of the tile from t0 on, and whether all of them see all
   auto own = [&]() __attribute__((always_inline)) { return ranges[wave * 32 + l32]; };
+  constexpr int WN = 32 * KH;  // the wavefront's keys of a tile, from t0 + 32 kt0 on
   auto some_see = [&](int t0) {
-    if (t0 >= all0 && t0 + BN <= all1) return true;  // (most tiles of a long prompt)
+    const int k0 = t0 + 32 * kt0;
+    if (k0 >= all0 && k0 + WN <= all1) return true;  // (most tiles of a long prompt)
     const int4 r = own();
-    return __any((t0 < r.y && t0 + BN > r.x) || (t0 < r.w && t0 + BN > r.z)) != 0;
+    return __any((k0 < r.y && k0 + WN > r.x) || (k0 < r.w && k0 + WN > r.z)) != 0;
   };
   auto all_see = [&](int t0) {
-    if (t0 >= all0 && t0 + BN <= all1) return true;
+    const int k0 = t0 + 32 * kt0;
+    if (k0 >= all0 && k0 + WN <= all1) return true;
     const int4 r = own();
-    return __all((t0 >= r.x && t0 + BN <= r.y) || (t0 >= r.z && t0 + BN <= r.w)) != 0;
+    return __all((k0 >= r.x && k0 + WN <= r.y) || (k0 >= r.z && k0 + WN <= r.w)) != 0;
   };
-  constexpr auto key_of = [](int e) { return (e >> 4) * 32 + ((e & 15) >> 2) * 8 + (e & 3); };  // of the lane's score e: t0 + key_of(e) + 4 hh
+  constexpr auto key_of = [](int e) { return (e >> 4) * 32 + ((e & 15) >> 2) * 8 + (e & 3); };  // of the lane's score e: t0 + 32 kt0 + key_of(e) + 4 hh
 
   // biases of the lane's keys of the tile from t0 on
-  auto biases = [&](int t0, f32x16_v(&s)[2]) __attribute__((always_inline)) {
-    const int pos = places[wave * 32 + l32], first = t0 + 4 * hh - pos;
+  auto biases = [&](int t0, f32x16_v(&s)[KH]) __attribute__((always_inline)) {
+    const int pos = places[wave * 32 + l32], k0 = t0 + 32 * kt0, first = k0 + 4 * hh - pos;
     if constexpr (BIAS == 1) {
       const float at = static_cast<float>(first);
-      const bool before = __all(t0 + BN - 1 <= pos), behind = __all(t0 >= pos);
+      const bool before = __all(k0 + WN - 1 <= pos), behind = __all(k0 >= pos);
       if (before || behind) {  // (linear: one instruction each)
         const float sl = before ? slope : -slope, b0 = sl * at;
 #pragma unroll
-        for (int e = 0; e < 32; ++e) s[e >> 4][e & 15] = fmaf(sl, static_cast<float>(key_of(e)), b0);
+        for (int e = 0; e < NS; ++e) s[e >> 4][e & 15] = fmaf(sl, static_cast<float>(key_of(e)), b0);
       } else {
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
+        for (int e = 0; e < NS; ++e) {
           s[e >> 4][e & 15] = -slope * fabsf(at + static_cast<float>(key_of(e)));
           if (e % 8 == 7) __builtin_amdgcn_sched_barrier(0);
         }
       }
     } else {
-      const bool before = __all(t0 + BN - 1 - pos <= -p.radius), behind = __all(t0 - pos >= p.radius);
+      const bool before = __all(k0 + WN - 1 - pos <= -p.radius), behind = __all(k0 - pos >= p.radius);
       if (before || behind) {
         const float far = table[before ? 0 : 2 * p.radius + 2 * kPad];
 #pragma unroll
-        for (int e = 0; e < 32; ++e) s[e >> 4][e & 15] = far;
+        for (int e = 0; e < NS; ++e) s[e >> 4][e & 15] = far;
       } else {
         const float* const from = table + clampi(first, -p.radius - kPad, p.radius) + p.radius + kPad;
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
+        for (int e = 0; e < NS; ++e) {
           s[e >> 4][e & 15] = from[key_of(e)];
           if (e % 8 == 7) __builtin_amdgcn_sched_barrier(0);  // (not all at once: there are no registers for it)
         }
       }
     }
   };
-  auto first_values = [&](int t0, f32x16_v(&s)[2]) __attribute__((always_inline)) {
+  auto first_values = [&](int t0, f32x16_v(&s)[KH]) __attribute__((always_inline)) {
     if constexpr (BIAS != 0 && !CAP) {
       biases(t0, s);
     } else {
 #pragma unroll
-      for (int e = 0; e < 32; ++e) s[e >> 4][e & 15] = 0.f;
+      for (int e = 0; e < NS; ++e) s[e >> 4][e & 15] = 0.f;
     }
   };
-  auto lane_max = [&](const f32x16_v(&s)[2]) __attribute__((always_inline)) {
+  auto lane_max = [&](const f32x16_v(&s)[KH]) __attribute__((always_inline)) {
     float mx = s[0][0];
 #pragma unroll
-    for (int e = 1; e < 32; ++e) mx = __builtin_elementwise_maximum(mx, s[e >> 4][e & 15]);
+    for (int e = 1; e < NS; ++e) mx = __builtin_elementwise_maximum(mx, s[e >> 4][e & 15]);
     return mx;
   };
   // Behind the products: the cap by its own formula and the biases behind it (CAP, unless the tile's scores stay as they are: see below),
   // keys that some query does not see; returns the lane's maximum
-  auto finish_scores = [&](int t0, bool all, f32x16_v(&s)[2]) {
+  auto finish_scores = [&](int t0, bool all, f32x16_v(&s)[KH]) {
     if constexpr (CAP) {
-      f32x16_v add[2];
+      f32x16_v add[KH];
       if constexpr (BIAS != 0) biases(t0, add);
 #pragma unroll
-      for (int e = 0; e < 32; ++e) {
+      for (int e = 0; e < NS; ++e) {
         s[e >> 4][e & 15] = p.cap(s[e >> 4][e & 15]) + (BIAS != 0 ? add[e >> 4][e & 15] : 0.f);
         if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
       }
@@ -363,9 +369,10 @@ void attn_ruled_kernel(const RuledParams p) {
     if (!all) {
       const int4 r = own();
       const uint64_t w = range_bits(r.x, r.y, t0) | range_bits(r.z, r.w, t0);
-      const uint32_t half[2] = {static_cast<uint32_t>(w) >> (4 * hh), static_cast<uint32_t>(w >> 32) >> (4 * hh)};
+      const uint32_t lower = static_cast<uint32_t>(w) >> (4 * hh), upper = static_cast<uint32_t>(w >> 32) >> (4 * hh);
+      const uint32_t half[2] = {KH == 1 && kt0 == 1 ? upper : lower, upper};
 #pragma unroll
-      for (int e = 0; e < 32; ++e) s[e >> 4][e & 15] = (half[e >> 4] & (1u << (key_of(e) & 31))) ? s[e >> 4][e & 15] : kOut;
+      for (int e = 0; e < NS; ++e) s[e >> 4][e & 15] = (half[e >> 4] & (1u << (key_of(e) & 31))) ? s[e >> 4][e & 15] : kOut;
     }
     const float mx = lane_max(s);
     return POLY && mx == kOut ? -INFINITY : mx;
@@ -392,8 +399,8 @@ void attn_ruled_kernel(const RuledParams p) {
   // (finish_scores), and their polynomial is the score itself.
   bool seen = false, live = false;  // tile i: seen by some query of this wavefront (s_cur holds its scores), with some weight
   float c0 = 1.f, c1 = 0.f, c2 = 0.f, c3 = 0.f;  // POLY: of s_cur
-  auto k_at = [&](const char* kb, int i) { return *reinterpret_cast<const u32x4_v*>(kb + (i & 1) * 32 * ROWB + (k_lane ^ ((i >> 1) * 32))); };
-  auto tile = [&](int i, const int buf, f32x16_v(&s_cur)[2], f32x16_v(&s_next)[2]) {
+  auto k_at = [&](const char* kb, int i) { return *reinterpret_cast<const u32x4_v*>(kb + i % KH * 32 * ROWB + (k_lane ^ (i / KH * 32))); };
+  auto tile = [&](int i, const int buf, f32x16_v(&s_cur)[KH], f32x16_v(&s_next)[KH]) {
     const bool has_next = i + 1 < n_tiles;
     if (i + 2 < n_tiles) load_k(i + 2, buf);
     if (has_next) load_v(i + 1, buf ^ 1);
@@ -404,7 +411,7 @@ void attn_ruled_kernel(const RuledParams p) {
       // Everything of a tile in one piece: branches around its parts would have the scores of both their ways brought together by copies
       // (32 at every tile, 10 % of a long prompt). So the next products are formed where nothing of them is seen, and probabilities of
       // scores that do not count (`live` says so), once each at the ends of a run of tiles.
-      uint32_t pf[2][2][4];
+      uint32_t pf[KH][2][4];
       float sum = 0.f;
       auto exponent = [&](float s) __attribute__((always_inline)) {
         if constexpr (!POLY) return fmaf(s, c, -mc);
@@ -426,11 +433,11 @@ void attn_ruled_kernel(const RuledParams p) {
       for (int n = 0; n < KPF; ++n) kfr[n] = k_at(kb, n);
       frag qn = q_at(0);
 #pragma unroll
-      for (int n = 0; n < 2 * KS; ++n) {
-        if (n + KPF < 2 * KS) kfr[(n + KPF) % (KPF + 1)] = k_at(kb, n + KPF);
-        s_next[n & 1] = M::run(__builtin_bit_cast(frag, kfr[n % (KPF + 1)]), qn, s_next[n & 1]);
-        if ((n & 1) && n + 1 < 2 * KS) qn = q_at((n + 1) >> 1);
-        constexpr int EACH = 16 / (2 * KS);
+      for (int n = 0; n < KH * KS; ++n) {
+        if (n + KPF < KH * KS) kfr[(n + KPF) % (KPF + 1)] = k_at(kb, n + KPF);
+        s_next[n % KH] = M::run(__builtin_bit_cast(frag, kfr[n % (KPF + 1)]), qn, s_next[n % KH]);
+        if (n % KH == KH - 1 && n + 1 < KH * KS) qn = q_at((n + 1) / KH);
+        constexpr int EACH = 8 / KS;
 #pragma unroll
         for (int m = 0; m < EACH; ++m) probabilities(n * EACH + m);
         __builtin_amdgcn_sched_barrier(0);
@@ -444,7 +451,7 @@ void attn_ruled_kernel(const RuledParams p) {
       if (live) {
         l_run += sum;
         const char* const vb = lds + (2 + buf) * TILEB;
-        constexpr int NSTEP = 4 * DT, VPF = CAP || D == 64 ? 2 : 3, EACH = 32 / NSTEP;
+        constexpr int NSTEP = 2 * KH * DT, VPF = CAP || D == 64 ? 2 : 3, EACH = NS / NSTEP;
         s16x4_r vlo[VPF + 1], vhi[VPF + 1];
         auto v_fetch = [&](int st) {
           const char* const vp = vb + (st / DT) * 16 * ROWB + (v_lane ^ ((st % DT * 64) % ROWB));
@@ -471,7 +478,7 @@ void attn_ruled_kernel(const RuledParams p) {
         }
       } else if constexpr (!CAP || BIAS == 0) {
 #pragma unroll
-        for (int e = 0; e < 32; e += 2) max_step(e);
+        for (int e = 0; e < NS; e += 2) max_step(e);
       }
       if (seen_next) {  // the next scores made ready, as far as they are not
         const bool all = all_see(tn);
@@ -505,13 +512,13 @@ void attn_ruled_kernel(const RuledParams p) {
     for (int ks = 0; ks < QL; ++ks) q_lds[ks * NW * 64 + tid] = __builtin_bit_cast(u32x4_v, qf[ks]);
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
-    f32x16_v sa[2], sb[2];
+    f32x16_v sa[KH], sb[KH];
     {
       const int t0 = tile_at(0) * BN;
       seen = some_see(t0);
       first_values(t0, sa);
 #pragma unroll
-      for (int i = 0; i < 2 * KS; ++i) sa[i & 1] = M::run(__builtin_bit_cast(frag, k_at(lds, i)), q_at(i >> 1), sa[i & 1]);
+      for (int i = 0; i < KH * KS; ++i) sa[i % KH] = M::run(__builtin_bit_cast(frag, k_at(lds, i)), q_at(i / KH), sa[i % KH]);
       settle_max(finish_scores(t0, all_see(t0), sa));
       live = seen;
     }
@@ -523,7 +530,35 @@ void attn_ruled_kernel(const RuledParams p) {
   }
 
   // ---- epilogue ----
-  const float l_tot = l_run + swapped(l_run);
+  float l_tot = l_run + swapped(l_run);
+  if constexpr (KH == 1) {  // the upper halves' sums join the lower ones' (behind the loop's last barrier nothing is read from the tiles)
+    f32x4_v* const jo = reinterpret_cast<f32x4_v*>(lds) + (wave & 1) * (DT * 4 * 64);
+    float2* const jm = reinterpret_cast<float2*>(lds + 2 * DT * 4 * 64 * 16) + (wave & 1) * 64;
+    static_assert(2 * (DT * 4 * 64 * 16 + 64 * 8) <= 4 * TILEB, "the join fits the tiles' memory");
+    if (wave >= 2) {
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) jo[(dt * 4 + g) * 64 + lane] = f32x4_v{o[dt][g * 4], o[dt][g * 4 + 1], o[dt][g * 4 + 2], o[dt][g * 4 + 3]};
+      jm[lane] = make_float2(m_run, l_tot);
+    }
+    __syncthreads();
+    if (wave >= 2) return;
+    const float2 other = jm[lane];
+    const float m = fmaxf(m_run, other.x), m_safe = m == -INFINITY ? 0.f : m;
+    const float a = __builtin_amdgcn_exp2f((m_run - m_safe) * c), b = __builtin_amdgcn_exp2f((other.x - m_safe) * c);
+    m_run = m;
+    // (a side that saw nothing has a sum of zero, but what it multiplied by zero may be NaN)
+    l_tot = (l_tot == 0.f ? 0.f : l_tot * a) + (other.y == 0.f ? 0.f : other.y * b);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4_v x = jo[(dt * 4 + g) * 64 + lane];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[dt][g * 4 + e] = o[dt][g * 4 + e] * a + x[e] * b;
+      }
+  }
   const bool mine = q0 + l32 < p.Sq;
   const int64_t part = (static_cast<int64_t>(unit) * p.n_qblocks + qb) * p.chunks + chunk;
   float* const po = p.ws + part * BM * D;
@@ -541,9 +576,9 @@ void attn_ruled_kernel(const RuledParams p) {
           x[e] = l_tot == 0.f ? 0.f : o[dt][g * 4 + e];
           probe = fmaf(x[e], 0.f, probe);
         }
-        if (mine) *reinterpret_cast<f32x4_v*>(po + (wave * 32 + l32) * D + dt * 32 + g * 8 + hh * 4) = x;
+        if (mine) *reinterpret_cast<f32x4_v*>(po + (q0 - qb * BM + l32) * D + dt * 32 + g * 8 + hh * 4) = x;
       }
-    if (mine && hh == 0) *reinterpret_cast<float2*>(pml + (wave * 32 + l32) * 2) = make_float2(m_run * c, l_tot);
+    if (mine && hh == 0) *reinterpret_cast<float2*>(pml + (q0 - qb * BM + l32) * 2) = make_float2(m_run * c, l_tot);
   } else {
     const float inv = 1.f / l_tot;
 #pragma unroll
@@ -612,10 +647,10 @@ void attn_ruled_kernel(const RuledParams p) {
     }
 #pragma unroll
     for (int e = 0; e < D / 64; ++e) {
-      if (p.chunks > 1) po[(wave * 32 + who) * D + lane * (D / 64) + e] = acc[e];
+      if (p.chunks > 1) po[(q0 - qb * BM + who) * D + lane * (D / 64) + e] = acc[e];
       else (orow + r * p.os_s)[lane * (D / 64) + e] = from_float<T>(acc[e] / l);
     }
-    if (p.chunks > 1 && lane == 0) *reinterpret_cast<float2*>(pml + (wave * 32 + who) * 2) = make_float2(m, l);
+    if (p.chunks > 1 && lane == 0) *reinterpret_cast<float2*>(pml + (q0 - qb * BM + who) * 2) = make_float2(m, l);
   }
 }
 
@@ -630,11 +665,11 @@ __global__ __launch_bounds__(256) void attn_ruled_merge_kernel(const RuledParams
   const int64_t gr = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
   if (gr >= static_cast<int64_t>(p.units) * p.Sq) return;
   const int unit = static_cast<int>(gr / p.Sq), row = static_cast<int>(gr - static_cast<int64_t>(unit) * p.Sq);
-  const int64_t first = (static_cast<int64_t>(unit) * p.n_qblocks + row / 128) * p.chunks;
-  const float* const ml = p.ws + static_cast<int64_t>(p.units) * p.n_qblocks * p.chunks * 128 * D;
-  const float* const po = p.ws + (first * 128 + row % 128) * D + lane * EPL;
+  const int64_t first = (static_cast<int64_t>(unit) * p.n_qblocks + row / p.bm) * p.chunks;
+  const float* const ml = p.ws + static_cast<int64_t>(p.units) * p.n_qblocks * p.chunks * p.bm * D;
+  const float* const po = p.ws + (first * p.bm + row % p.bm) * D + lane * EPL;
   const int mine = lane < p.chunks ? lane : 0;
-  const float2 own = *reinterpret_cast<const float2*>(ml + ((first + mine) * 128 + row % 128) * 2);
+  const float2 own = *reinterpret_cast<const float2*>(ml + ((first + mine) * p.bm + row % p.bm) * 2);
   const float mc = lane < p.chunks ? own.x : -INFINITY;
   float m = mc;
 #pragma unroll
@@ -646,7 +681,7 @@ __global__ __launch_bounds__(256) void attn_ruled_merge_kernel(const RuledParams
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
-      for (int e = 0; e < EPL; ++e) x[i][e] = c0 + i < p.chunks ? po[static_cast<int64_t>(c0 + i) * 128 * D + e] : 0.f;
+      for (int e = 0; e < EPL; ++e) x[i][e] = c0 + i < p.chunks ? po[static_cast<int64_t>(c0 + i) * p.bm * D + e] : 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float wi = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), (c0 + i) & 63));
@@ -659,36 +694,48 @@ __global__ __launch_bounds__(256) void attn_ruled_merge_kernel(const RuledParams
   for (int e = 0; e < EPL; ++e) op[e] = from_float<T>(l == 0.f ? 0.f : acc[e] / l);
 }
 
-// Into how many chunks a query block's tiles are cut: where the call has fewer workgroups than the GPU has room for, as many as cost least.
-// A tile is 1.1 us of a workgroup alone on its compute unit; the join is a launch of 3 us and its sums' way to memory and back, 8 bytes a feature.
-static int ruled_chunks(int B, int Sq, int Sk, int H, int D, int docs, int window, int causal) {
-  const int64_t blocks = static_cast<int64_t>((Sq + 127) / 128) * H * B, room = D == 128 ? 512 : 768;
+// How a call is cut.
+// Two wavefronts share 32 queries (KH = 1) where query blocks of 128 would leave compute units without any, or, under a causal order, are so
+// few that the longest of them decide: a tile then takes a wavefront alone on its SIMD 0.83 us, 1.1 otherwise, and there are twice as many
+// blocks, but each of them reads all its keys. us, KH = 2 / 1, blocks of 128 in brackets, of 128 features if not said otherwise:
+//   causal      S=512 H=8 [32] 14.5 / 12.3    S=512 H=32 of 64 [128] 11.8 / 9.9    S=1024 H=24 [192] 25.0 / 22.0    S=2048 H=32 of 64 [512] 37.6 / 31.3
+//               S=4096 H=16 [512] 93.5 / 85.9    S=8192 H=8 [512] 176 / 159    S=3000 H=24 [576] 75.3 / 79.0    S=4096 H=24 of 64 [768] 75.9 / 79.3
+//   all keys    S=512 H=8 [32] 14.0 / 12.1    S=512 H=32 of 64 [128] 11.6 / 9.9    S=1024 H=24 [192] 25.4 / 25.8    B=3 S=300 H=24 [216] 11.7 / 12.9
+//               S=2048 H=32 [512] 72 / 86    four documents of 1024 tokens, H=64 of 64, with a table [512] 26.6 / 31.0
+// Where a call still has fewer workgroups than the GPU has room for, its tiles are cut into chunks, as many as cost least: the join is a launch
+// of 3 us and its sums' way to memory and back, 8 bytes a feature.
+struct RuledPlan { int halves, chunks; };
+static RuledPlan ruled_plan(int B, int Sq, int Sk, int H, int D, int docs, int window, int causal) {
+  const auto blocks = [&](int bm) { return static_cast<int64_t>((Sq + bm - 1) / bm) * H * B; };
+  RuledPlan plan{blocks(128) <= 128 || (causal && docs == 0 && blocks(128) <= 512) ? 1 : 2, 1};
+  const int64_t mine = blocks(64 * plan.halves), room = D == 128 ? 512 : 768;
   int64_t keys = docs > 0 ? 2 * (Sk / docs) + 64 : Sk;  // that a query block may see, about
   if (window > 0) {
     const int64_t most = (causal ? 1ll : 2ll) * window + 128;
     keys = most < keys ? most : keys;
   }
-  const double tiles = static_cast<double>(keys) / 64, join = static_cast<double>(B) * H * Sq * D * 8 / 4e6;
-  int best = 1;
-  double cost = 1.1 * tiles;
-  for (int n = 2; n <= kMaxChunks && n * blocks <= room && n <= tiles; ++n) {
-    const double t = 1.1 * tiles / n + 3.0 + n * join;
-    if (t < cost) { cost = t; best = n; }
+  const double tiles = static_cast<double>(keys) / 64, each = plan.halves == 1 ? 0.83 : 1.1, join = static_cast<double>(B) * H * Sq * D * 8 / 4e6;
+  double cost = each * tiles;
+  for (int n = 2; n <= kMaxChunks && n * mine <= room && n <= tiles; ++n) {
+    const double t = each * tiles / n + 3.0 + n * join;
+    if (t < cost) { cost = t; plan.chunks = n; }
   }
-  return best;
+  return plan;
 }
 
-static size_t ruled_workspace_bytes(int chunks, int B, int Sq, int H, int D) {
-  return chunks > 1 ? static_cast<size_t>((Sq + 127) / 128) * H * B * chunks * 128 * (D + 2) * sizeof(float) : 0;
+static size_t ruled_workspace_bytes(const RuledPlan& plan, int B, int Sq, int H, int D) {
+  const int bm = 64 * plan.halves;
+  return plan.chunks > 1 ? static_cast<size_t>((Sq + bm - 1) / bm) * H * B * plan.chunks * bm * (D + 2) * sizeof(float) : 0;
 }
 
-template <typename T, int D>
+template <typename T, int D, int KH>
 static int launch_ruled(RuledParams& p, bool cap, int bias, hipStream_t stream) {
-  p.n_qblocks = (p.Sq + 127) / 128;
+  p.bm = 64 * KH;
+  p.n_qblocks = (p.Sq + p.bm - 1) / p.bm;
   p.units = p.H * p.B;
   const int64_t total = static_cast<int64_t>(p.n_qblocks) * p.H * p.B * p.chunks;
   ODIT_CHECK_ARG(total <= 0x7fffffffll, "odit_attn_ruled: grid of %lld workgroups is too large", static_cast<long long>(total));
-#define ODIT_RULED_GO(C, X) hipLaunchKernelGGL((attn_ruled_kernel<T, D, C, X>), dim3(total), dim3(256), 0, stream, p)
+#define ODIT_RULED_GO(C, X) hipLaunchKernelGGL((attn_ruled_kernel<T, D, C, X, KH>), dim3(total), dim3(256), 0, stream, p)
   if (cap) {
     if (bias == 0) ODIT_RULED_GO(true, 0); else if (bias == 1) ODIT_RULED_GO(true, 1); else ODIT_RULED_GO(true, 2);
   } else {
@@ -701,13 +748,17 @@ static int launch_ruled(RuledParams& p, bool cap, int bias, hipStream_t stream) 
   }
   return check_launch("odit_attn_ruled");
 }
+template <typename T, int D>
+static int launch_ruled(RuledParams& p, const RuledPlan& plan, bool cap, int bias, hipStream_t stream) {
+  return plan.halves == 1 ? launch_ruled<T, D, 1>(p, cap, bias, stream) : launch_ruled<T, D, 2>(p, cap, bias, stream);
+}
 
 }  // namespace odit
 
 extern "C" size_t odit_attn_ruled_workspace_bytes(int B, int Sq, int Sk, int H, int D, const odit_attn_rules* rules) {
   using namespace odit;
   if (B <= 0 || Sq <= 0 || Sk <= 0 || H <= 0 || D <= 0 || rules == nullptr) return 0;
-  return ruled_workspace_bytes(ruled_chunks(B, Sq, Sk, H, D, rules->docs, rules->window, rules->causal), B, Sq, H, D);
+  return ruled_workspace_bytes(ruled_plan(B, Sq, Sk, H, D, rules->docs, rules->window, rules->causal), B, Sq, H, D);
 }
 
 extern "C" int odit_attn_ruled(const void* q, const void* k, const void* v, void* o, int B, int Sq, int Sk, int H, int Hkv, int D,
@@ -759,12 +810,13 @@ extern "C" int odit_attn_ruled(const void* q, const void* k, const void* v, void
   p.scale_log2 = scale * kLog2e;
   p.bias_scale = 1.f / scale;
   // (without scratch, or with less than that takes, a query block's tiles stay in one piece)
-  p.chunks = ruled_chunks(B, Sq, Sk, H, D, r.docs, r.window, r.causal);
-  if (workspace == nullptr || workspace_bytes < ruled_workspace_bytes(p.chunks, B, Sq, H, D)) p.chunks = 1;
+  RuledPlan plan = ruled_plan(B, Sq, Sk, H, D, r.docs, r.window, r.causal);
+  if (workspace == nullptr || workspace_bytes < ruled_workspace_bytes(plan, B, Sq, H, D)) plan.chunks = 1;
+  p.chunks = plan.chunks;
   p.ws = static_cast<float*>(workspace);
   p.cap = make_cap(r.cap, scale);
   const int bias = r.slopes != nullptr ? 1 : r.distance != nullptr ? 2 : 0;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (dtype == ODIT_BF16) return D == 128 ? launch_ruled<bf16_t, 128>(p, r.cap > 0.f, bias, st) : launch_ruled<bf16_t, 64>(p, r.cap > 0.f, bias, st);
-  return D == 128 ? launch_ruled<f16_t, 128>(p, r.cap > 0.f, bias, st) : launch_ruled<f16_t, 64>(p, r.cap > 0.f, bias, st);
+  if (dtype == ODIT_BF16) return D == 128 ? launch_ruled<bf16_t, 128>(p, plan, r.cap > 0.f, bias, st) : launch_ruled<bf16_t, 64>(p, plan, r.cap > 0.f, bias, st);
+  return D == 128 ? launch_ruled<f16_t, 128>(p, plan, r.cap > 0.f, bias, st) : launch_ruled<f16_t, 64>(p, plan, r.cap > 0.f, bias, st);
 }
