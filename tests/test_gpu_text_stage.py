@@ -30,18 +30,27 @@ def _bias(kind, H, seed, radius=5):
     return {}
 
 
-def _check_ruled(q, k, v, o, scale, rules, bias, cap):
+def _check_ruled(q, k, v, os, scale, rules, bias, cap):
     seen, away = seen_keys(q.shape[1], k.shape[1], **rules)
     for b in range(q.shape[0]):
         want, tol = attention(q[b], k[b], v[b], scale, seen, away, cap, **bias)
-        within(o[b], want, tol)
+        for o in os:
+            within(o[b], want, tol)
 
 
 def _ruled(q, k, v, scale, rules, bias, cap):
+    """The results of the call as it is and of one with 300 times the batch rows, whose workgroups are cut otherwise; all copies' bits are one's."""
     r = dict(rules)
     for name in ("q_starts", "k_starts", "prefix"):
         r[name] = _i32(r.get(name))
-    return kernels.attn_ruled(q, k, v, scale, cap=cap, **r, **bias)
+    o = kernels.attn_ruled(q, k, v, scale, cap=cap, **r, **bias)
+    B, n = q.shape[0], 300
+    if r["prefix"] is not None and r["q_starts"] is None:
+        r["prefix"] = r["prefix"].repeat(n)
+    many = kernels.attn_ruled(*(t[None].expand(n, *t.shape).flatten(0, 1) if B > 1 else t.expand(n, *t.shape[1:]) for t in (q, k, v)), scale, cap=cap, **r, **bias)
+    many = many.view(n, *o.shape)
+    assert torch.equal(many[1:].nan_to_num(7.0), many[:1].nan_to_num(7.0).expand_as(many[1:]))
+    return o, many[0]
 
 
 # ------------------------------------------------------------------------------------------------ whole prompts
@@ -62,10 +71,10 @@ def test_prompt_lengths(gpu, Sq, Sk, causal, D, dtype):
 def test_prompt_rules(gpu, rules, cap, kind, D, dtype):
     q, k, v = _randn(4, 2, 150, 4, D, dtype=dtype, std=2), _randn(5, 2, 190, 2, D, dtype=dtype), _randn(6, 2, 190, 2, D, dtype=dtype)
     bias = _bias(kind, 4, 7)
-    o = _ruled(q, k, v, 0.1, rules, bias, cap)
+    os = _ruled(q, k, v, 0.1, rules, bias, cap)
     for b in range(2):  # (prefixes differ from batch row to batch row)
         own = dict(rules, prefix=[rules["prefix"][b]]) if "prefix" in rules else rules
-        _check_ruled(q[b:b + 1], k[b:b + 1], v[b:b + 1], o[b:b + 1], 0.1, own, bias, cap)
+        _check_ruled(q[b:b + 1], k[b:b + 1], v[b:b + 1], [o[b:b + 1] for o in os], 0.1, own, bias, cap)
 
 
 @pytest.mark.parametrize("cap,kind", list(itertools.product([0.0, 3.0], ["", "slopes", "table"])))
@@ -78,9 +87,9 @@ def test_documents(gpu, cap, kind, q_starts, k_starts, causal, window, prefix):
     q, k, v = _randn(8, 1, 300, 2, 64, std=2), _randn(9, 1, 300, 2, 64), _randn(10, 1, 300, 2, 64)
     rules = dict(q_starts=q_starts, k_starts=k_starts, causal=causal, window=window, prefix=[2, 70, 0, 5, 1][:len(q_starts) - 1] if prefix else None)
     bias = _bias(kind, 2, 11)
-    o = _ruled(q, k, v, 0.125, rules, bias, cap)
-    _check_ruled(q, k, v, o, 0.125, rules, bias, cap)
-    assert not o[0, q_starts[-1]:].any() and not o[0, :q_starts[0]].any()
+    os = _ruled(q, k, v, 0.125, rules, bias, cap)
+    _check_ruled(q, k, v, os, 0.125, rules, bias, cap)
+    assert not any(o[0, q_starts[-1]:].any() or o[0, :q_starts[0]].any() for o in os)
 
 
 def test_many_documents_and_a_long_gap(gpu):
@@ -103,9 +112,9 @@ def test_prompt_strides(gpu, D):
     rules = dict(causal=True)
     _check_ruled(q, k, v, _ruled(q, k, v, 0.1, rules, {}, 0.0), 0.1, rules, {}, 0.0)
     k2, v2 = k.transpose(1, 2).contiguous().transpose(1, 2), v.transpose(1, 2).contiguous().transpose(1, 2)
-    assert torch.equal(_ruled(q, k2, v2, 0.1, rules, {}, 0.0), _ruled(q, k, v, 0.1, rules, {}, 0.0))
+    assert all(map(torch.equal, _ruled(q, k2, v2, 0.1, rules, {}, 0.0), _ruled(q, k, v, 0.1, rules, {}, 0.0)))
     odd = _randn(19, 2, 100, 2, D + 1)[..., 1:]
-    assert torch.equal(_ruled(q, odd, v, 0.1, rules, {}, 0.0), _ruled(q, odd.contiguous(), v, 0.1, rules, {}, 0.0))
+    assert all(map(torch.equal, _ruled(q, odd, v, 0.1, rules, {}, 0.0), _ruled(q, odd.contiguous(), v, 0.1, rules, {}, 0.0)))
     wide = torch.cat([k, k.roll(1, 3)], dim=3)[..., 24:24 + D]  # (row stride 2 D Hkv, rows that do not start on a multiple of their length)
     _check_ruled(q, wide, v, _ruled(q, wide, v, 0.1, rules, {}, 0.0), 0.1, rules, {}, 0.0)
     one = k[:, :1].expand(2, 100, 2, D)
@@ -126,16 +135,16 @@ def test_what_is_not_seen_does_not_count(gpu, what, cap, kind, D, dtype):
         t[0, 199] = what     # the last key of the third: its last query alone sees it
     dirty = _ruled(q, k, v, 0.1, rules, bias, cap)
     keep = list(range(90)) + list(range(150, 199))
-    assert not dirty[0, keep].isnan().any()
     zero = k.clone(), v.clone()
     for t in zero:
         t[0, 90:150] = 0
         t[0, 199] = 0
     seen, away = seen_keys(200, 200, **rules)
     want, tol = attention(q[0], zero[0][0], zero[1][0], 0.1, seen, away, cap, **bias)
-    within(dirty[0][keep], want[keep], tol[keep])
-    within(clean[0][keep], want[keep], tol[keep])
-    assert not dirty[0, 90:150].isfinite().any() and not dirty[0, 199].isfinite().any()
+    for o in dirty + clean:
+        within(o[0][keep], want[keep], tol[keep])
+    for o in dirty:
+        assert not o[0, 90:150].isfinite().any() and not o[0, 199].isfinite().any()
 
 
 def test_scores_far_apart(gpu):
@@ -155,9 +164,9 @@ def test_biases_that_forbid(gpu):
     distance = torch.zeros(2, 7, device="cuda:0")
     distance[0, :2] = -float("inf")     # head 0: away <= -2 is out
     distance[1, :] = -float("inf")      # head 1: everything is
-    o = _ruled(q, k, v, 0.1, dict(causal=True), dict(distance=distance), 0.0)
-    assert not o[:, :, 1].any()
-    _check_ruled(q[:, :, :1], k[:, :, :1], v[:, :, :1], o[:, :, :1], 0.1, dict(causal=True, window=2), {}, 0.0)
+    os = _ruled(q, k, v, 0.1, dict(causal=True), dict(distance=distance), 0.0)
+    assert not any(o[:, :, 1].any() for o in os)
+    _check_ruled(q[:, :, :1], k[:, :, :1], v[:, :, :1], [o[:, :, :1] for o in os], 0.1, dict(causal=True, window=2), {}, 0.0)
 
 
 @pytest.mark.parametrize("Sq,Sk,rules", [
@@ -175,15 +184,16 @@ def test_few_rows_of_many_keys(gpu, Sq, Sk, rules, cap, kind, D, dtype):
         keep = [i for i in range(Sq) if i != 2]  # (the first document's last query sees key 1299)
         zeroed = v.nan_to_num(0.0, 0.0, 0.0), k.nan_to_num(0.0)
         want, tol = attention(q[0], zeroed[1][0], zeroed[0][0], 0.1, seen, away, cap, **bias)
-        o = _ruled(q, k, v, 0.1, rules, bias, cap)[0]
-        within(o[keep], want[keep], tol[keep])
-        assert o[2].isnan().all()
+        for o in _ruled(q, k, v, 0.1, rules, bias, cap):
+            within(o[0][keep], want[keep], tol[keep])
+            assert o[0, 2].isnan().all()
 
 
+@pytest.mark.parametrize("copies", [1, 60])
 @pytest.mark.parametrize("D", [64, 128])
-def test_bits_repeat(gpu, D):
+def test_bits_repeat(gpu, D, copies):
     """The same call gives the same bits, whatever is in the caches and registers before it."""
-    q, k, v = _randn(50, 1, 300, 4, D, std=2), _randn(51, 1, 300, 2, D), _randn(52, 1, 300, 2, D)
+    q, k, v = _randn(50, copies, 300, 4, D, std=2), _randn(51, copies, 300, 2, D), _randn(52, copies, 300, 2, D)
     other = torch.empty(1 << 28, dtype=torch.int8, device="cuda:0")
     starts = _i32([5, 60, 150]), _i32([10, 200, 250])
     for kw in (dict(q_starts=starts[0], k_starts=starts[1]), dict(causal=True, window=40), dict(causal=True, cap=5.0), dict(causal=True, **_bias("slopes", 4, 0)),
@@ -415,8 +425,8 @@ def test_prompt_then_tokens(gpu, cap, kind, window):
         k = kernels.rope_append(packed[1], packed[1], None, torch.tensor(positions, device="cuda:0"), turns)[1]
         starts = [0, lengths[0], sum(lengths)]
         rules = dict(causal=True, window=window, q_starts=starts, k_starts=starts)
-        o = _ruled(q[None], k[None], packed[2][None], 0.125, rules, bias, cap)
-        _check_ruled(q[None], k[None], packed[2][None], o, 0.125, rules, bias, cap)
+        os = _ruled(q[None], k[None], packed[2][None], 0.125, rules, bias, cap)
+        _check_ruled(q[None], k[None], packed[2][None], os, 0.125, rules, bias, cap)
         for step in range(3):
             now = [n + step for n in lengths]
             parts = [torch.stack([data[b][i][now[b]] for b in range(2)]) for i in range(3)]
@@ -425,11 +435,12 @@ def test_prompt_then_tokens(gpu, cap, kind, window):
             for b in range(2):
                 at = torch.tensor([int(table[b, p // page]) * page + p % page for p in range(now[b] + 1)], device="cuda:0")
                 kk, vv = kc.flatten(0, 1)[at], vc.flatten(0, 1)[at]
-                whole = _ruled(q[None, b:b + 1], kk[None], vv[None], 0.125, dict(causal=True, window=window), bias, cap)[0]
+                whole = _ruled(q[None, b:b + 1], kk[None], vv[None], 0.125, dict(causal=True, window=window), bias, cap)
                 seen, away = seen_keys(1, now[b] + 1, causal=True, window=window)
                 want, tol = attention(q[b:b + 1], kk, vv, 0.125, seen, away, cap, **bias)
                 within(o[b:b + 1], want, tol)
-                within(whole, want, tol)
+                for w in whole:
+                    within(w[0], want, tol)
 
 
 def test_streams_graphs_and_threads_of_work(gpu):
