@@ -20,6 +20,19 @@ typedef short s16x8_r __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) s16x4_r* lds_s16x4_rp;
 typedef __attribute__((address_space(3))) void* lds_void_rp;
 
+// n / d for n below 2^31, as n * mul >> shift (mul rounded up)
+struct Quotient {
+  uint32_t mul;
+  int shift;
+  __device__ __forceinline__ int operator()(int n) const { return static_cast<int>(static_cast<uint64_t>(static_cast<uint32_t>(n)) * mul >> shift); }
+};
+static Quotient quotient(int d) {
+  Quotient q{0, 31};
+  while ((1ll << (q.shift - 31)) < d) ++q.shift;
+  q.mul = static_cast<uint32_t>(((1ull << q.shift) + d - 1) / d);
+  return q;
+}
+
 struct RuledParams {
   const void *q, *k, *v;
   void* o;
@@ -31,6 +44,8 @@ struct RuledParams {
   float scale_log2, bias_scale;  // scale log2(e) and 1 / scale
   Cap cap;
   int n_qblocks, units;  // units: heads of all batch rows
+  int group;             // query heads of a key head
+  Quotient by_blocks, by_units, by_heads, by_group;  // by n_qblocks * units, by the units of a row of blocks (of an XCD), by H, by group
   int bm;                // queries of a block
   int chunks;            // workgroups that share a query block's tiles; with more than one, their sums go to ws
   float* ws;             // [units][n_qblocks][chunks][bm][D] sums, then [...][bm] (maximum in units of log2, sum)
@@ -113,17 +128,18 @@ void attn_ruled_kernel(const RuledParams p) {
   const int l32 = lane & 31, hh = lane >> 5;
   // the last query blocks, which see most under a causal order, begin first; where the heads divide over the XCDs, an XCD keeps its heads
   // (steep slopes leave a head little to add: with slopes the heads go round the XCDs, 1040 us of 16384 causal tokens, 16 heads of 128, otherwise, 929 so)
-  const int chunk = p.chunks > 1 ? blockIdx.x / (p.units * p.n_qblocks) : 0, block = blockIdx.x - chunk * (p.units * p.n_qblocks);
+  const int chunk = p.chunks > 1 ? p.by_blocks(blockIdx.x) : 0, block = blockIdx.x - chunk * (p.units * p.n_qblocks);
   int unit, qb;
   if (BIAS != 1 && p.units % kNumXcd == 0) {
-    const int per = p.units / kNumXcd, local = block / kNumXcd;
-    unit = block % kNumXcd * per + local % per;
-    qb = p.n_qblocks - 1 - local / per;
+    const int per = p.units / kNumXcd, local = block / kNumXcd, at = p.by_units(local);
+    unit = block % kNumXcd * per + local - at * per;
+    qb = p.n_qblocks - 1 - at;
   } else {
-    unit = block % p.units;
-    qb = p.n_qblocks - 1 - block / p.units;
+    const int at = p.by_units(block);
+    unit = block - at * p.units;
+    qb = p.n_qblocks - 1 - at;
   }
-  const int h = unit % p.H, b = unit / p.H, hkv = h / (p.H / p.Hkv);
+  const int b = p.by_heads(unit), h = unit - b * p.H, hkv = p.by_group(h);
   const int kt0 = KH == 1 ? wave >> 1 : 0;  // the first of this wavefront's halves
   const int q0 = qb * BM + (KH == 1 ? wave & 1 : wave) * 32;
   const int row = q0 + l32 < p.Sq ? q0 + l32 : p.Sq - 1;
@@ -201,9 +217,9 @@ void attn_ruled_kernel(const RuledParams p) {
   {
     if (hh == 0) ranges[wave * 32 + l32] = make_int4(blo, bhi, plo, phi);
     if (BIAS != 0 && hh == 0) places[wave * 32 + l32] = pos;
-    all0 = half_max(blo);
-    all1 = half_min(bhi);
     if (p.docs > 0) {
+      all0 = half_max(blo);
+      all1 = half_min(bhi);
       const int b0 = half_min(bhi > 0 ? blo : kNone), b1 = half_max(bhi), p0 = half_min(phi > 0 ? plo : kNone), p1 = half_max(phi);
       if (lane == 0) { bounds[wave][0] = b0; bounds[wave][1] = b1; bounds[wave][2] = p0; bounds[wave][3] = p1; }
     }
@@ -222,6 +238,9 @@ void attn_ruled_kernel(const RuledParams p) {
           hi[i] = max(hi[i], bounds[w][2 * i + 1]);
         }
     } else {  // one document: both ends of the band rise with the row
+      const int row0 = min(q0, p.Sq - 1) + p.Sk - p.Sq, row1 = min(q0 + 31, p.Sq - 1) + p.Sk - p.Sq;
+      all0 = band_begin(row1, p.Sk);
+      all1 = band_end(row0, p.Sk);
       const int last = min(qb * BM + BM, p.Sq) - 1;
       lo[0] = band_begin(qb * BM + p.Sk - p.Sq, p.Sk);
       hi[0] = band_end(last + p.Sk - p.Sq, p.Sk);
@@ -249,22 +268,27 @@ void attn_ruled_kernel(const RuledParams p) {
   const T* const kbase = static_cast<const T*>(p.k) + b * p.ks_b + hkv * p.ks_h;
   const T* const vbase = static_cast<const T*>(p.v) + b * p.vs_b + hkv * p.vs_h;
   const int r0 = wave * IPW * RPI + lane / CPR, pc0 = lane % CPR;
+  constexpr auto k_swizzle = [](int r) { return D == 128 ? r % 16 : r / 2 % 8; };
+  constexpr auto v_swizzle = [](int r) { return D == 128 ? 4 * (r % 4) : 4 * (r / 2 % 2); };
   // Byte offsets of the lane's first instruction; the others' rows lie a whole number of rows further down, which is the load's scalar
-  // offset. Their swizzle is the same, but for keys of head size 128, where it differs by a constant.
-  const uint32_t krow = static_cast<uint32_t>(r0 * p.ks_s * 2), kswz = static_cast<uint32_t>(((pc0 ^ (r0 % 16)) % CPR) * 16);
-  const uint32_t vvoff = static_cast<uint32_t>(r0 * p.vs_s * 2) + static_cast<uint32_t>(((pc0 ^ (4 * (r0 % 4))) % CPR) * 16);
+  // offset. The chunk of 16 bytes that a lane fetches is swizzled by its row, so that the reads of fragments touch all banks: keys by row, or by
+  // row / 2 at head size 64, where two rows share the banks (by row there, as in attn_fwd_dma.hip, 43 % of the reads' cycles were conflicts);
+  // values so that the 4 keys of a transposed read do. An instruction's rows are a multiple of 4 further down: another constant for keys, none for values.
+  const uint32_t krow = static_cast<uint32_t>(r0 * p.ks_s * 2), kswz = static_cast<uint32_t>((pc0 ^ k_swizzle(r0)) * 16);
+  const uint32_t vvoff = static_cast<uint32_t>(r0 * p.vs_s * 2) + static_cast<uint32_t>((pc0 ^ v_swizzle(r0)) * 16);
   const uint32_t lds_base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void_rp)lds));
+  const uint32_t k_bytes = static_cast<uint32_t>(((BN - 1) * p.ks_s + D) * 2), v_bytes = static_cast<uint32_t>(((BN - 1) * p.vs_s + D) * 2);
   auto load_tile = [&](const T* base, int64_t stride, bool keys, int t, int dst) __attribute__((always_inline)) {
-    const uint64_t a = reinterpret_cast<uint64_t>(base + static_cast<int64_t>(t) * BN * stride);
-    const int rows = min(BN, p.Sk - t * BN);  // rows behind the last key read as zeros
+    const uint64_t a = reinterpret_cast<uint64_t>(base) + static_cast<uint64_t>(static_cast<uint32_t>(t)) * static_cast<uint32_t>(BN * 2 * stride);
+    const int over = t * BN + BN - p.Sk;  // rows behind the last key read as zeros
     u32x4_v r;
     r.x = static_cast<uint32_t>(a); r.y = static_cast<uint32_t>(a >> 32) & 0xffffu;
-    r.z = static_cast<uint32_t>(((rows - 1) * stride + D) * 2); r.w = 0x00020000u;
+    r.z = (keys ? k_bytes : v_bytes) - (over > 0 ? static_cast<uint32_t>(over * 2) * static_cast<uint32_t>(stride) : 0); r.w = 0x00020000u;
     uint32_t row = keys ? krow : vvoff, swz = keys ? kswz : 0;
     asm volatile("" : "+v"(swz));  // (the sums are formed here, not held in registers across the loop)
 #pragma unroll
     for (int i = 0; i < IPW; ++i)
-      load_lds16(lds_base + dst + (wave * IPW + i) * 1024, row + (keys ? swz ^ static_cast<uint32_t>((RPI * i) % 16 % CPR * 16) : 0), r,
+      load_lds16(lds_base + dst + (wave * IPW + i) * 1024, row + (keys ? swz ^ static_cast<uint32_t>(k_swizzle(RPI * i) * 16) : 0), r,
                  static_cast<uint32_t>(RPI * i * stride * 2));
   };
   auto load_k = [&](int i, const int buf) { load_tile(kbase, p.ks_s, true, tile_at(i), buf * TILEB); };
@@ -279,9 +303,9 @@ void attn_ruled_kernel(const RuledParams p) {
   float m_run = -INFINITY, l_run = 0.f, mc = 0.f;
   const float slope = BIAS == 1 ? p.slopes[h] * bias_unit : 0.f;
 
-  const int k_lane = (32 * kt0 + l32) * ROWB + (((hh ^ (l32 % 16)) % CPR) << 4);
+  const int k_lane = (32 * kt0 + l32) * ROWB + ((hh ^ k_swizzle(l32)) << 4);
   const int sq = (lane & 15) >> 2, dh = (lane >> 4) & 1;
-  const int v_lane = (32 * kt0 + 4 * hh + sq) * ROWB + ((((4 * sq) % CPR) ^ (2 * dh + ((lane & 3) >> 1))) << 4) + ((lane & 1) << 3);
+  const int v_lane = (32 * kt0 + 4 * hh + sq) * ROWB + ((v_swizzle(sq) ^ (2 * dh + ((lane & 3) >> 1))) << 4) + ((lane & 1) << 3);
   auto swapped = [&](float x) __attribute__((always_inline)) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return __uint_as_float(hh ? r[0] : r[1]);
@@ -563,7 +587,7 @@ void attn_ruled_kernel(const RuledParams p) {
   const int64_t part = (static_cast<int64_t>(unit) * p.n_qblocks + qb) * p.chunks + chunk;
   float* const po = p.ws + part * BM * D;
   float* const pml = p.ws + static_cast<int64_t>(p.units) * p.n_qblocks * p.chunks * BM * D + part * BM * 2;
-  float probe = 0.f;  // NaN once anything is NaN or infinite
+  float probe = 0.f;  // the largest in size; NaN once anything is
   T* const orow = static_cast<T*>(p.o) + b * p.os_b + h * p.os_h;
   if (p.chunks > 1) {
 #pragma unroll
@@ -574,7 +598,7 @@ void attn_ruled_kernel(const RuledParams p) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           x[e] = l_tot == 0.f ? 0.f : o[dt][g * 4 + e];
-          probe = fmaf(x[e], 0.f, probe);
+          if (e & 1) probe = __builtin_elementwise_maximum(__builtin_elementwise_maximum(probe, fabsf(x[e - 1])), fabsf(x[e]));
         }
         if (mine) *reinterpret_cast<f32x4_v*>(po + (q0 - qb * BM + l32) * D + dt * 32 + g * 8 + hh * 4) = x;
       }
@@ -589,7 +613,7 @@ void attn_ruled_kernel(const RuledParams p) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           x[e] = l_tot == 0.f ? 0.f : o[dt][g * 4 + e] * inv;
-          probe = fmaf(x[e], 0.f, probe);
+          if (e & 1) probe = __builtin_elementwise_maximum(__builtin_elementwise_maximum(probe, fabsf(x[e - 1])), fabsf(x[e]));
         }
         auto pair = [&](int e) __attribute__((always_inline)) {
           return __builtin_amdgcn_permlane32_swap(M::pack2(x[e], x[e + 1]), M::pack2(x[e + 4], x[e + 5]), false, false);
@@ -601,7 +625,7 @@ void attn_ruled_kernel(const RuledParams p) {
       }
   }
   // rows to be done again: finite sums, but values that are not. (l_tot == 0: nothing was seen, zeros are right)
-  uint64_t bad = __ballot(mine && l_tot > 0.f && l_tot < INFINITY && probe != 0.f);
+  uint64_t bad = __ballot(mine && l_tot > 0.f && l_tot < INFINITY && !(probe < INFINITY));
   bad = (bad | (bad >> 32)) & 0xffffffffull;
   while (bad != 0) {  // (wave-uniform)
     const int who = __builtin_ctzll(bad);
@@ -733,8 +757,13 @@ static int launch_ruled(RuledParams& p, bool cap, int bias, hipStream_t stream) 
   p.bm = 64 * KH;
   p.n_qblocks = (p.Sq + p.bm - 1) / p.bm;
   p.units = p.H * p.B;
+  p.group = p.H / p.Hkv;
   const int64_t total = static_cast<int64_t>(p.n_qblocks) * p.H * p.B * p.chunks;
   ODIT_CHECK_ARG(total <= 0x7fffffffll, "odit_attn_ruled: grid of %lld workgroups is too large", static_cast<long long>(total));
+  p.by_blocks = quotient(p.n_qblocks * p.units);
+  p.by_units = quotient(bias != 1 && p.units % kNumXcd == 0 ? p.units / kNumXcd : p.units);
+  p.by_heads = quotient(p.H);
+  p.by_group = quotient(p.group);
 #define ODIT_RULED_GO(C, X) hipLaunchKernelGGL((attn_ruled_kernel<T, D, C, X, KH>), dim3(total), dim3(256), 0, stream, p)
   if (cap) {
     if (bias == 0) ODIT_RULED_GO(true, 0); else if (bias == 1) ODIT_RULED_GO(true, 1); else ODIT_RULED_GO(true, 2);
