@@ -18,6 +18,7 @@
 #include <type_traits>
 
 #include "attn_rules.h"
+#include "quotient.h"
 
 namespace odit {
 
@@ -46,8 +47,7 @@ struct PagedParams {
   const int *table, *lengths;
   const float *slopes, *distance;
   int B, H, Hkv, pages, page, max_pages, window, radius;
-  uint32_t page_mul;  // key / page = key * page_mul >> page_shift
-  int page_shift;
+  Quotient by_page;
   int64_t qs_b, qs_h, kc_p, kc_r, kc_h, vc_p, vc_r, vc_h, ts, os_b, os_h;
   float scale_log2;
   Cap cap;
@@ -231,7 +231,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 4
   const int hb = unit % p.head_blocks, hkv = unit / p.head_blocks, b = at.b;
   const int h0 = hkv * p.group + hb * 16, heads = min(16, p.group - hb * 16);
   const int h = h0 + min(l16, heads - 1);  // this lane's head
-  const auto page_of = [&](int key) { return static_cast<int>(static_cast<uint64_t>(static_cast<uint32_t>(key)) * p.page_mul >> p.page_shift); };
+  const auto page_of = [&](int key) { return p.by_page(key); };
 
   int first, n;
   paged_range(p, at.length, &first, &n);
@@ -551,9 +551,7 @@ extern "C" int odit_attn_paged(const void* q, const void* key_cache, const void*
   PagedParams p;
   p.q = q; p.k = key_cache; p.v = value_cache; p.o = o; p.table = table; p.lengths = lengths; p.slopes = r.slopes; p.distance = r.distance;
   p.B = B; p.H = H; p.Hkv = Hkv; p.pages = pages; p.page = page_size; p.max_pages = max_pages; p.window = r.window; p.radius = r.radius;
-  p.page_shift = 31;  // (rounded up: exact for keys below 2^31)
-  while ((1ll << (p.page_shift - 31)) < page_size) ++p.page_shift;
-  p.page_mul = static_cast<uint32_t>(((1ull << p.page_shift) + page_size - 1) / page_size);
+  p.by_page = quotient(page_size);
   p.qs_b = q_strides[0]; p.qs_h = q_strides[1]; p.os_b = o_strides[0]; p.os_h = o_strides[1]; p.ts = table_stride;
   p.kc_p = key_cache_strides[0]; p.kc_r = key_cache_strides[1]; p.kc_h = key_cache_strides[2];
   p.vc_p = value_cache_strides[0]; p.vc_r = value_cache_strides[1]; p.vc_h = value_cache_strides[2];

@@ -12,6 +12,7 @@
 // A value that is NaN or infinite spoils its tile's product also for queries that do not see its key (0 times it is NaN). Rows that come out
 // NaN with a finite sum are therefore done again at the end, over their own keys alone.
 #include "attn_rules.h"
+#include "quotient.h"
 
 namespace odit {
 
@@ -19,19 +20,6 @@ typedef short s16x4_r __attribute__((ext_vector_type(4)));
 typedef short s16x8_r __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) s16x4_r* lds_s16x4_rp;
 typedef __attribute__((address_space(3))) void* lds_void_rp;
-
-// n / d for n below 2^31, as n * mul >> shift (mul rounded up)
-struct Quotient {
-  uint32_t mul;
-  int shift;
-  __device__ __forceinline__ int operator()(int n) const { return static_cast<int>(static_cast<uint64_t>(static_cast<uint32_t>(n)) * mul >> shift); }
-};
-static Quotient quotient(int d) {
-  Quotient q{0, 31};
-  while ((1ll << (q.shift - 31)) < d) ++q.shift;
-  q.mul = static_cast<uint32_t>(((1ull << q.shift) + d - 1) / d);
-  return q;
-}
 
 struct RuledParams {
   const void *q, *k, *v;

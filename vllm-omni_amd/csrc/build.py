@@ -27,7 +27,7 @@ PROBE_LIB_PATH = PKG / "libomni_dit_probe.so"
 NATIVE_SRC = CSRC / "native.cpp"
 NATIVE_PATH = PKG / "_native.so"
 OBJ_DIR = CSRC / "build"
-HEADERS = [CSRC / "odit_common.h", CSRC / "attn_common.h", CSRC / "attn_tail.h", CSRC / "attn_rules.h", CSRC / "gemm_bf16.h",
+HEADERS = [CSRC / "odit_common.h", CSRC / "attn_common.h", CSRC / "attn_tail.h", CSRC / "attn_rules.h", CSRC / "quotient.h", CSRC / "gemm_bf16.h",
            CSRC / "gemm_epilogue.h", CSRC / "gemm_tile.h",
            CSRC / "gemm_heads.h", CSRC / "gemm_small.h", CSRC / "time_sinusoid.h", CSRC / "time_tokens.h", PKG.parent / "include" / "omni_dit.h"]
 

@@ -7,9 +7,13 @@
 // The angle is reduced in 64 bits because positions are whole numbers up to a million and beyond: in fp32 the product of such a
 // position and a turn has lost the fraction that is all that counts. Behind the reduction 24 bits are enough.
 //
-// Bound by memory: every element of q, k and v is read once and written once. A workgroup has a few tokens: its threads first make
-// their (cos, sin) pairs in LDS, once for all heads, then move 16 bytes each.
+// Bound by memory: every element of q, k and v is read once and written once. A workgroup has one token: its threads first make the token's
+// (cos, sin) pairs in LDS, once for all heads, then move 16 bytes each. us, one / two / four tokens of a workgroup: 65536 tokens, 32 heads on 8
+// of 128 into a cache 291 (5.5 TB/s) / 296 / 306, 8191 tokens, 24 heads on 24, a quarter of 128 rotated, 36.6 / 36.3 / 40.7, 4096 tokens as the
+// first 19.8 / 22.2 / 21.7. Several pieces of a thread in flight at a time gave nothing, loads and stores past the caches 287 of the 306 but
+// 12.0 where 2000 tokens take 9.6.
 #include "odit_common.h"
+#include "quotient.h"
 
 namespace odit {
 
@@ -23,7 +27,7 @@ struct RopeAppendParams {
   int64_t qs_t, qs_h, ks_t, ks_h, vs_t, vs_h;
   int64_t kc_p, kc_r, kc_h, vc_p, vc_r, vc_h;  // cache strides: page, row in the page, head
   float magnitude;
-  int tokens;  // of a workgroup
+  Quotient by_units, by_pieces;  // by a rotated head's pieces (or features), by D / 8
 };
 
 // features [8 c, 8 c + 8) of a head, or pairs (i, i + rot/2) for i in [8 c, 8 c + 8)
@@ -75,53 +79,46 @@ __device__ __forceinline__ void rope_feature(const T* src, T* dst, const float2*
 // FORM 0: interleaved, 1: halves in 16-byte pieces, 2: halves feature by feature
 template <typename T, int FORM>
 __global__ __launch_bounds__(256) void rope_append_kernel(const RopeAppendParams p) {
-  extern __shared__ float2 cs[];  // [tokens][rot / 2]
-  const int half = p.rot / 2;
-  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * p.tokens;
-  const int n = static_cast<int>(p.T - t0 < p.tokens ? p.T - t0 : p.tokens);
-  for (int i = threadIdx.x; i < n * half; i += 256) {
-    const int t = i / half;
-    double f = static_cast<double>(p.positions[t0 + t]) * p.turns[i - t * half];
+  extern __shared__ float2 cs[];  // [rot / 2]
+  const int64_t token = blockIdx.x;
+  for (int i = threadIdx.x; i < p.rot / 2; i += 256) {
+    double f = static_cast<double>(p.positions[token]) * p.turns[i];
     f -= rint(f);
     float s, c;
     sincospif(2.f * static_cast<float>(f), &s, &c);
     cs[i] = make_float2(c * p.magnitude, s * p.magnitude);
   }
+  int64_t page = 0, row = 0;
+  bool stored = true;
+  if (p.slots != nullptr) {
+    const int64_t slot = p.slots[token];
+    stored = slot >= 0 && slot < p.n_slots;  // (a padded token has none)
+    page = stored ? slot / p.page : 0;
+    row = stored ? slot - page * p.page : 0;
+  }
   __syncthreads();
   const int units = FORM == 0 ? p.D / 8 : FORM == 1 ? p.D / 8 - p.rot / 16 : p.D;  // of a head that is rotated
-  const int copies = p.v != nullptr ? p.Hkv * (p.D / 8) : 0;                       // 16-byte pieces of a token's values
-  const int turned = (p.H + p.Hkv) * units;
-  for (int t = 0; t < n; ++t) {
-    const int64_t token = t0 + t;
-    int64_t page = 0, row = 0;
-    bool stored = true;
-    if (p.slots != nullptr) {
-      const int64_t slot = p.slots[token];
-      stored = slot >= 0 && slot < p.n_slots;  // (a padded token has none)
-      page = stored ? slot / p.page : 0;
-      row = stored ? slot - page * p.page : 0;
-    }
-    for (int i = threadIdx.x; i < turned + copies; i += 256) {
-      if (i < turned) {
-        const int h = i / units, u = i - h * units;
-        const T* src;
-        T* dst;
-        if (h < p.H) {
-          src = static_cast<const T*>(p.q) + token * p.qs_t + h * p.qs_h;
-          dst = static_cast<T*>(p.q_out) + (token * p.H + h) * p.D;
-        } else {
-          if (!stored) continue;
-          src = static_cast<const T*>(p.k) + token * p.ks_t + (h - p.H) * p.ks_h;
-          dst = p.slots != nullptr ? static_cast<T*>(p.k_cache) + page * p.kc_p + row * p.kc_r + (h - p.H) * p.kc_h
-                                   : static_cast<T*>(p.k_out) + (token * p.Hkv + (h - p.H)) * p.D;
-        }
-        if constexpr (FORM == 2) rope_feature<T>(src, dst, cs + t * half, u, p.rot);
-        else rope_unit<T, FORM == 1>(src, dst, cs + t * half, u, p.rot);
-      } else if (stored) {
-        const int c = i - turned, h = c / (p.D / 8), u = c - h * (p.D / 8);
-        store_raw(static_cast<T*>(p.v_cache) + page * p.vc_p + row * p.vc_r + h * p.vc_h + u * 8,
-                  load_raw(static_cast<const T*>(p.v) + token * p.vs_t + h * p.vs_h + u * 8));
+  const int turned = (p.H + p.Hkv) * units, copies = p.v != nullptr ? p.Hkv * (p.D / 8) : 0;  // (16-byte pieces of the token's values)
+  for (int i = threadIdx.x; i < turned + copies; i += 256) {
+    if (i < turned) {
+      const int h = p.by_units(i), u = i - h * units;
+      const T* src;
+      T* dst;
+      if (h < p.H) {
+        src = static_cast<const T*>(p.q) + token * p.qs_t + h * p.qs_h;
+        dst = static_cast<T*>(p.q_out) + (token * p.H + h) * p.D;
+      } else {
+        if (!stored) continue;
+        src = static_cast<const T*>(p.k) + token * p.ks_t + (h - p.H) * p.ks_h;
+        dst = p.slots != nullptr ? static_cast<T*>(p.k_cache) + page * p.kc_p + row * p.kc_r + (h - p.H) * p.kc_h
+                                 : static_cast<T*>(p.k_out) + (token * p.Hkv + (h - p.H)) * p.D;
       }
+      if constexpr (FORM == 2) rope_feature<T>(src, dst, cs, u, p.rot);
+      else rope_unit<T, FORM == 1>(src, dst, cs, u, p.rot);
+    } else if (stored) {
+      const int c = i - turned, h = p.by_pieces(c), u = c - h * (p.D / 8);
+      store_raw(static_cast<T*>(p.v_cache) + page * p.vc_p + row * p.vc_r + h * p.vc_h + u * 8,
+                load_raw(static_cast<const T*>(p.v) + token * p.vs_t + h * p.vs_h + u * 8));
     }
   }
 }
@@ -170,16 +167,16 @@ extern "C" int odit_rope_append(const void* q, const void* k, const void* v, con
   p.kc_p = cached ? key_cache_strides[0] : 0; p.kc_r = cached ? key_cache_strides[1] : 0; p.kc_h = cached ? key_cache_strides[2] : 0;
   p.vc_p = cached ? value_cache_strides[0] : 0; p.vc_r = cached ? value_cache_strides[1] : 0; p.vc_h = cached ? value_cache_strides[2] : 0;
   p.magnitude = magnitude;
-  p.tokens = T >= 4096 ? 4 : 1;
-  const int64_t grid = (T + p.tokens - 1) / p.tokens;
-  ODIT_CHECK_ARG(grid <= 0x7fffffff, "odit_rope_append: %lld tokens are too many", static_cast<long long>(T));
-  const size_t lds = static_cast<size_t>(p.tokens) * (rot / 2) * sizeof(float2);
+  ODIT_CHECK_ARG(T <= 0x7fffffff, "odit_rope_append: %lld tokens are too many", static_cast<long long>(T));
+  const size_t lds = static_cast<size_t>(rot / 2) * sizeof(float2);
   const int form = !(flags & ODIT_FLAG_NEOX) ? 0 : rot % 16 == 0 ? 1 : 2;
+  p.by_units = quotient(form == 0 ? D / 8 : form == 1 ? D / 8 - rot / 16 : D);
+  p.by_pieces = quotient(D / 8);
   hipStream_t st = static_cast<hipStream_t>(stream);
 #define ODIT_ROPE_GO(E)                                                                                                  \
-  if (form == 0) hipLaunchKernelGGL((rope_append_kernel<E, 0>), dim3(grid), dim3(256), lds, st, p);                      \
-  else if (form == 1) hipLaunchKernelGGL((rope_append_kernel<E, 1>), dim3(grid), dim3(256), lds, st, p);                 \
-  else hipLaunchKernelGGL((rope_append_kernel<E, 2>), dim3(grid), dim3(256), lds, st, p);
+  if (form == 0) hipLaunchKernelGGL((rope_append_kernel<E, 0>), dim3(T), dim3(256), lds, st, p);                      \
+  else if (form == 1) hipLaunchKernelGGL((rope_append_kernel<E, 1>), dim3(T), dim3(256), lds, st, p);                 \
+  else hipLaunchKernelGGL((rope_append_kernel<E, 2>), dim3(T), dim3(256), lds, st, p);
   if (dtype == ODIT_BF16) { ODIT_ROPE_GO(bf16_t) }
   else { ODIT_ROPE_GO(f16_t) }
 #undef ODIT_ROPE_GO
