@@ -59,6 +59,7 @@ struct PagedParams {
 
 constexpr int kPagedWaves = 4, kPagedTile = 16, kPagedEntries = 1024, kPagedStep = kPagedWaves * kPagedTile;
 constexpr int kPagedLeast = 2;  // steps of a chunk: with one, a sequence of 1000 keys takes 9.7 us, with two 8.4
+constexpr int kPagedWhole = 256;  // keys up to which a sequence is one chunk: the join takes as long as twice 128 keys
 constexpr int kPagedWanted = 512;  // workgroups: two to a compute unit at head size 128 (us, 448 / 512 / 640 / 768: 4 sequences of 100000 to 131072 keys
                                    // 345 / 335 / 366 / 362, 8 of 4096 33 / 31 / 35 / 36, one of 32768 37 / 36 / 41 / 41; head size 64 the same)
 constexpr int kPagedJoin = 12;  // chunks whose parts are loaded at once (at head size 64 16 wavefronts share a compute unit's registers)
@@ -107,7 +108,8 @@ __device__ __forceinline__ PagedPlace paged_place(const PagedParams& p, int inde
     return b < p.B ? end - first : 0;
   };
   const auto parts_of = [&](int b, int keys, int chunk) {
-    return b < p.B ? max(1, static_cast<int>((static_cast<uint32_t>(keys) + chunk - 1) / static_cast<uint32_t>(chunk))) : 0;
+    const int n = keys <= kPagedWhole ? 1 : static_cast<int>((static_cast<uint32_t>(keys) + chunk - 1) / static_cast<uint32_t>(chunk));
+    return b < p.B ? max(1, n) : 0;
   };
   int length;
   const int mine = keys_of(lane, &length);
@@ -235,7 +237,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 4
 
   int first, n;
   paged_range(p, at.length, &first, &n);
-  const int parts = at.parts, begin = first + at.part * at.chunk, end = min(n, begin + at.chunk), pg0 = page_of(begin);
+  const int parts = at.parts, begin = first + at.part * at.chunk, end = parts == 1 ? n : min(n, begin + at.chunk), pg0 = page_of(begin);
   bool bad = false;
   if (end > begin) {
     const int npg = page_of(end - 1) - pg0 + 1;
