@@ -484,7 +484,7 @@ static int64_t paged_most_keys(int64_t max_pages, int page, int window) {
 template <typename T, int D>
 static int launch_paged(const PagedParams& p, int64_t chunks, bool cap, int bias, hipStream_t stream) {
   const int64_t grid = p.units * chunks;
-  ODIT_CHECK_ARG(grid <= 0x7fffffffll, "odit_attn_paged: grid of %lld workgroups is too large", static_cast<long long>(grid));
+  ODIT_CHECK_ARG(grid < (1ll << 24), "odit_attn_paged: grid of %lld workgroups is too large", static_cast<long long>(grid));
 #define ODIT_PAGED_GO(C, X) hipLaunchKernelGGL((attn_paged_kernel<T, D, C, X>), dim3(grid), dim3(256), 0, stream, p)
   if (cap) {
     if (bias == 0) ODIT_PAGED_GO(true, 0); else if (bias == 1) ODIT_PAGED_GO(true, 1); else ODIT_PAGED_GO(true, 2);
@@ -528,7 +528,7 @@ extern "C" int odit_attn_paged(const void* q, const void* key_cache, const void*
   ODIT_CHECK_ARG(q_strides && key_cache_strides && value_cache_strides && o_strides, "odit_attn_paged: null strides");
   ODIT_CHECK_ARG(B >= 0 && H > 0 && Hkv > 0 && pages >= 0 && max_pages >= 0 && page_size > 0, "odit_attn_paged: bad shape");
   ODIT_CHECK_ARG(H % Hkv == 0, "odit_attn_paged: H=%d is not a multiple of Hkv=%d", H, Hkv);
-  ODIT_CHECK_ARG(static_cast<int64_t>(B) * H <= 0x7fffffffll, "odit_attn_paged: %d sequences of %d heads are too many", B, H);
+  ODIT_CHECK_ARG(static_cast<int64_t>(B) * H < (1ll << 26), "odit_attn_paged: %d sequences of %d heads are too many", B, H);
   ODIT_CHECK_ARG(static_cast<int64_t>(max_pages) * page_size <= kMost, "odit_attn_paged: %d pages of %d keys are more than %d keys",
                  max_pages, page_size, kMost);
   ODIT_CHECK_ARG(scale > 0.f, "odit_attn_paged: softmax scale must be positive (got %g)", scale);

@@ -747,7 +747,7 @@ static int launch_ruled(RuledParams& p, bool cap, int bias, hipStream_t stream) 
   p.units = p.H * p.B;
   p.group = p.H / p.Hkv;
   const int64_t total = static_cast<int64_t>(p.n_qblocks) * p.H * p.B * p.chunks;
-  ODIT_CHECK_ARG(total <= 0x7fffffffll, "odit_attn_ruled: grid of %lld workgroups is too large", static_cast<long long>(total));
+  ODIT_CHECK_ARG(total < (1ll << 24), "odit_attn_ruled: grid of %lld workgroups is too large", static_cast<long long>(total));
   p.by_blocks = quotient(p.n_qblocks * p.units);
   p.by_units = quotient(bias != 1 && p.units % kNumXcd == 0 ? p.units / kNumXcd : p.units);
   p.by_heads = quotient(p.H);

@@ -130,7 +130,6 @@ Tensor fresh(at::IntArrayRef sizes, const at::TensorOptions& opts) {
 // graph capture, where kernels.py has to keep what the graph will use.
 PyObject* g_linear_scratch_fn = nullptr;  // (device index, stream) -> tensor
 PyObject* g_attn_scratch_fn = nullptr;    // (device index, stream, bytes) -> tensor
-
 PyObject* g_ticket_scratch_fn = nullptr;  // (device index, stream, bytes) -> tensor
 
 struct Scratch { void* p = nullptr; size_t bytes = 0; };
@@ -2425,11 +2424,18 @@ PyObject* py_wan_block(PyObject*, PyObject* const* a, Py_ssize_t n) {
 // -------------------------------------------------------------------------------------------- module
 // (linear scratch, attention scratch)
 PyObject* py_configure(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (n != 3) { PyErr_SetString(PyExc_TypeError, "configure takes three callables"); return nullptr; }
-  Py_INCREF(a[0]); Py_INCREF(a[1]); Py_INCREF(a[2]);
+  if (n != 2) { PyErr_SetString(PyExc_TypeError, "configure takes two callables"); return nullptr; }
+  Py_INCREF(a[0]); Py_INCREF(a[1]);
   Py_XSETREF(g_linear_scratch_fn, a[0]);
   Py_XSETREF(g_attn_scratch_fn, a[1]);
-  Py_XSETREF(g_ticket_scratch_fn, a[2]);
+  Py_RETURN_NONE;
+}
+
+// (where the tickets of paged attention come from)
+PyObject* py_tickets_from(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 1) { PyErr_SetString(PyExc_TypeError, "tickets_from takes one callable"); return nullptr; }
+  Py_INCREF(a[0]);
+  Py_XSETREF(g_ticket_scratch_fn, a[0]);
   Py_RETURN_NONE;
 }
 
@@ -2485,6 +2491,7 @@ bool intern_names() {
 #define NATIVE_FN(name, fn) {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(fn)), METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {
     NATIVE_FN("configure", &py_configure),
+    NATIVE_FN("tickets_from", &py_tickets_from),
     NATIVE_FN("silu", &py_unary<odit_silu>),
     NATIVE_FN("gelu_tanh", &py_unary<odit_gelu_tanh>),
     NATIVE_FN("adaln", &py_adaln),

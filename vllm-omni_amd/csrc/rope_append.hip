@@ -167,7 +167,7 @@ extern "C" int odit_rope_append(const void* q, const void* k, const void* v, con
   p.kc_p = cached ? key_cache_strides[0] : 0; p.kc_r = cached ? key_cache_strides[1] : 0; p.kc_h = cached ? key_cache_strides[2] : 0;
   p.vc_p = cached ? value_cache_strides[0] : 0; p.vc_r = cached ? value_cache_strides[1] : 0; p.vc_h = cached ? value_cache_strides[2] : 0;
   p.magnitude = magnitude;
-  ODIT_CHECK_ARG(T <= 0x7fffffff, "odit_rope_append: %lld tokens are too many", static_cast<long long>(T));
+  ODIT_CHECK_ARG(T < (1ll << 24), "odit_rope_append: %lld tokens are too many", static_cast<long long>(T));
   const size_t lds = static_cast<size_t>(rot / 2) * sizeof(float2);
   const int form = !(flags & ODIT_FLAG_NEOX) ? 0 : rot % 16 == 0 ? 1 : 2;
   p.by_units = quotient(form == 0 ? D / 8 : form == 1 ? D / 8 - rot / 16 : D);

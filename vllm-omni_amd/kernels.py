@@ -48,7 +48,8 @@ def _load_native():
     """The native module, told where its scratch comes from and which modules its block functions know."""
     global _nat
     nat = _lib.native()
-    nat.configure(_linear_scratch, _attn_scratch, _paged_tickets)
+    nat.configure(_linear_scratch, _attn_scratch)
+    nat.tickets_from(_paged_tickets)
     nat.classes(_NATIVE_CLASSES)
     _nat = nat
     return nat
