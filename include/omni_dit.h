@@ -79,7 +79,7 @@ int odit_attn_fwd(const void* q, const void* k, const void* v, void* o, const ui
 
 /* ---------------------------------------------------------------------------------------------
  * A text stage beside the transformer: what a query sees, and what its scores become.
- *   s = scale * q.k;  cap > 0: s = cap * tanh(s / cap);  then one of
+ *   s = scale * q.k (scale in [1e-9, 1e9]);  cap > 0: s = cap * tanh(s / cap);  then one of
  *   slopes [H]:                 s -= slopes[h] * |away|
  *   distance [H][2 radius + 1]: s += distance[h][clamp(away, -radius, radius) + radius]
  * with away = key's position - query's position. The last of a document's queries is at the place of its last key.
@@ -90,7 +90,7 @@ int odit_attn_fwd(const void* q, const void* k, const void* v, void* o, const ui
  */
 typedef struct odit_attn_rules {
   int causal, window, docs, radius;
-  float cap; /* 0 (none) or up to 8192 */
+  float cap; /* 0 (none) or in [1e-9, 8192] */
   const int *q_starts, *k_starts, *prefix;
   const float *slopes, *distance;
 } odit_attn_rules;
@@ -112,7 +112,7 @@ size_t odit_attn_ruled_workspace_bytes(int B, int Sq, int Sk, int H, int D, cons
  * outside [0, pages) are not seen. Of the rules, docs and prefix do not apply (0 and NULL).
  * `workspace`: odit_attn_paged_workspace_bytes for the same shape and window (may be 0), contents irrelevant before and after.
  * `tickets`: NULL, or n_tickets words that are zero before the call and are left zero: with one for each sequence, key head and 16 query
- * heads of its group, a call of up to 16 chunks a sequence is one launch, not two (the same bits). No two calls at a time may share them. */
+ * heads of its group, a call is one launch, not two (the same bits). No two calls at a time may share them. */
 size_t odit_attn_paged_workspace_bytes(int B, int H, int Hkv, int D, int max_pages, int page_size, int window);
 int odit_attn_paged(const void* q, const void* key_cache, const void* value_cache, const int* table, const int* lengths, void* o, int B,
                     int H, int Hkv, int D, int pages, int page_size, int max_pages, const int64_t q_strides[2],

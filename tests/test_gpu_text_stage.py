@@ -509,7 +509,8 @@ def test_refusals(gpu):
         (lambda: rope(t=turns[:0]), RuntimeError), (lambda: rope(q=lone[..., :60], k=k[0, ..., :60]), RuntimeError), (lambda: rope(k=k[0, :7]), ValueError),
         (lambda: rope(**dict(into, slots=pos.int())), TypeError), (lambda: rope(**dict(into, key_cache=cache[..., :32])), ValueError),
         (lambda: rope(**dict(into, value_cache=cache[:3])), ValueError), (lambda: rope(**dict(into, key_cache=cache.half())), TypeError),
-        (lambda: rope(q=lone.float(), k=k[0].float()), TypeError),
+        (lambda: rope(q=lone.float(), k=k[0].float()), TypeError), (lambda: rope(**dict(into, key_cache=cache[:, :, :1].expand(-1, -1, 2, -1))), RuntimeError),
+        (lambda: ruled(cap=1e-12), ValueError), (lambda: kernels.attn_ruled(q, k, k, 1e-12), RuntimeError), (lambda: paged(cap=1e-12), ValueError),
         (lambda: kernels.attn_ruled(q.clone().requires_grad_(), k, k, 0.1), RuntimeError), (lambda: paged(q=lone.clone().requires_grad_()), RuntimeError),
         (lambda: rope(q=lone.clone().requires_grad_()), RuntimeError),
     ]:

@@ -46,7 +46,7 @@ def _rope(q=P, k=P, v=None, pos=P, turns=P, qo=P, ko=P, slots=None, kc=None, vc=
     (dict(slopes=P, distance=P), -1, "exclude"), (dict(distance=P, radius=1025), -1, "radius"), (dict(distance=P, radius=-1), -1, "radius"),
     (dict(k=P + 8), -1, "aligned"), (dict(ws=P + 8), -1, "aligned"), (dict(vs=(256, 60, 64)), -1, "multiples"), (dict(ks=(256, 1 << 23, 64)), -1, "apart"), (dict(ks=(256, -64, 64)), -1, "apart"),
     (dict(q=None), -1, "null"), (dict(v=None), -1, "null"), (dict(Sq=-1), -1, "shape"), (dict(Sk=(1 << 30) + 1), -1, "shape"), (dict(B=1 << 30, H=8), -1, "too many"),
-    (dict(B=1 << 10, Sq=1 << 29, H=64), -1, "too large"),
+    (dict(scale=1e-10), -1, "scale"), (dict(scale=float("inf")), -1, "scale"), (dict(cap=1e-12), -1, "cap"), (dict(B=1 << 10, Sq=1 << 29, H=64), -1, "too large"),
     (dict(B=1 << 12, Sq=1 << 16, H=8), -1, "too large")])
 def test_ruled_refuses(change, status, text):
     assert _ruled(**change) == status and text in _error(), _error()
@@ -78,7 +78,7 @@ def test_ruled_workspace():
     (dict(prefix=P), -1, "prompts"), (dict(cap=1e9), -1, "cap"), (dict(slopes=P, distance=P), -1, "exclude"), (dict(distance=P, radius=2000), -1, "radius"),
     (dict(q=P + 2), -1, "aligned"), (dict(qs=(256, 60)), -1, "multiples"), (dict(vs=(2048, 128, 4)), -1, "multiples"), (dict(k=None), -1, "null"),
     (dict(lengths=None), -1, "null"), (dict(most=100, ws_bytes=16), -4, "workspace"), (dict(most=100, ws=None), -4, "workspace"), (dict(most=100, ws=P + 4), -4, "workspace"),
-    (dict(B=1 << 20, H=1 << 12, Hkv=1 << 12), -1, "too many"),
+    (dict(scale=1e-10), -1, "scale"), (dict(scale=float("inf")), -1, "scale"), (dict(cap=1e-12), -1, "cap"), (dict(B=1 << 20, H=1 << 12, Hkv=1 << 12), -1, "too many"),
     (dict(B=1 << 22, H=8, Hkv=8), -1, "too large")])
 def test_paged_refuses(change, status, text):
     assert _paged(**change) == status and text in _error(), _error()
@@ -87,11 +87,11 @@ def test_paged_refuses(change, status, text):
 def test_paged_empty_and_workspace():
     assert _paged(B=0) == 0
     need = _lib.load().odit_attn_paged_workspace_bytes
-    assert need(3, 8, 2, 128, 8, 16, 0) == 0                                # 128 keys are one chunk
+    assert need(3, 8, 2, 128, 16, 16, 0) == 0                               # 256 keys are one chunk
     assert need(3, 8, 2, 128, 1000, 16, 100) == 0                           # as is a window of 100
-    one = need(1, 8, 2, 128, 16, 16, 0)
+    one = need(1, 8, 2, 128, 17, 16, 0)
     assert one > 0 and one % (2 * 4 * 130 * 4) == 0                         # chunks of 2 kv heads, 4 heads each, 128 features and two statistics
-    assert need(1, 48, 2, 64, 16, 16, 0) % (4 * 16 * 66 * 4) == 0           # 24 heads of a group are two blocks of up to 16
+    assert need(1, 48, 2, 64, 17, 16, 0) % (4 * 16 * 66 * 4) == 0           # 24 heads of a group are two blocks of up to 16
     assert need(0, 8, 2, 128, 8, 16, 0) == 0 and need(1, 8, 2, 128, 0, 16, 0) == 0
 
 
@@ -111,7 +111,7 @@ def test_the_workspace_has_room_for_chunks_of_small_pages(page):
     (dict(slots=P, v=P, kc=P, vc=P, pages=2, page=4), -1, "slots"), (dict(slots=P, v=P, kc=P, vc=P, ko=None, page=0), -1, "slots"),
     (dict(slots=P, v=P, kc=P, ko=None, pages=2), -1, "null"), (dict(slots=P, kc=P, vc=P, ko=None, pages=2), -1, "null"),
     (dict(slots=P, v=P, kc=P, vc=P, ko=None, pages=2, kcs=(64, 60, 64)), -1, "multiples"), (dict(qs=(127, 64)), -1, "multiples"), (dict(k=P + 4), -1, "aligned"),
-    (dict(turns=None), -1, "null"), (dict(ko=None), -1, "null"), (dict(T=1 << 24), -1, "too many")])
+    (dict(slots=P, v=P, kc=P, vc=P, ko=None, pages=2, page=4, kcs=(64, 0, 64), vcs=(256, 64, 64)), -1, "share"), (dict(turns=None), -1, "null"), (dict(ko=None), -1, "null"), (dict(T=1 << 24), -1, "too many")])
 def test_rope_refuses(change, status, text):
     assert _rope(**change) == status and text in _error(), _error()
 

@@ -472,7 +472,7 @@ static PagedPlan paged_plan(int B, int units, int64_t most_keys, int page) {
   plan.room = static_cast<int>(room < kPagedStep ? kPagedStep : room);
   // (each sequence's last chunk may be a part of one)
   const int64_t by_room = (B * most_keys + plan.room - 1) / plan.room;
-  plan.chunks = B + (most_keys <= kPagedLeast * kPagedStep ? 0 : by_room > plan.wanted ? by_room : plan.wanted);
+  plan.chunks = B + (most_keys <= kPagedWhole ? 0 : by_room > plan.wanted ? by_room : plan.wanted);
   return plan;
 }
 
@@ -531,10 +531,10 @@ extern "C" int odit_attn_paged(const void* q, const void* key_cache, const void*
   ODIT_CHECK_ARG(static_cast<int64_t>(B) * H < (1ll << 26), "odit_attn_paged: %d sequences of %d heads are too many", B, H);
   ODIT_CHECK_ARG(static_cast<int64_t>(max_pages) * page_size <= kMost, "odit_attn_paged: %d pages of %d keys are more than %d keys",
                  max_pages, page_size, kMost);
-  ODIT_CHECK_ARG(scale > 0.f, "odit_attn_paged: softmax scale must be positive (got %g)", scale);
+  ODIT_CHECK_ARG(scale >= kMinScale && scale <= kMaxScale, "odit_attn_paged: softmax scale %g outside [%g, %g]", scale, kMinScale, kMaxScale);
   ODIT_CHECK_ARG(r.window >= 0 && r.window <= kMost, "odit_attn_paged: window=%d outside [0, %d]", r.window, kMost);
   ODIT_CHECK_ARG(r.docs == 0 && r.prefix == nullptr, "odit_attn_paged: documents and prefixes are for whole prompts");
-  ODIT_CHECK_ARG(r.cap >= 0.f && r.cap <= kMaxCap, "odit_attn_paged: cap=%g outside [0, %g]", r.cap, kMaxCap);
+  ODIT_CHECK_ARG(r.cap == 0.f || (r.cap >= kMinScale && r.cap <= kMaxCap), "odit_attn_paged: cap=%g is neither 0 nor in [%g, %g]", r.cap, kMinScale, kMaxCap);
   ODIT_CHECK_ARG(r.slopes == nullptr || r.distance == nullptr, "odit_attn_paged: slopes and a table exclude each other");
   ODIT_CHECK_ARG(r.distance == nullptr || (r.radius >= 0 && r.radius <= kMaxRadius), "odit_attn_paged: radius=%d outside [0, %d]", r.radius,
                  kMaxRadius);

@@ -798,10 +798,10 @@ extern "C" int odit_attn_ruled(const void* q, const void* k, const void* v, void
   ODIT_CHECK_ARG(B >= 0 && Sq >= 0 && Sk >= 0 && H > 0 && Hkv > 0 && Sq <= kMost && Sk <= kMost, "odit_attn_ruled: bad shape");
   ODIT_CHECK_ARG(static_cast<int64_t>(B) * H <= 0x7fffffffll, "odit_attn_ruled: %d batch rows of %d heads are too many", B, H);
   ODIT_CHECK_ARG(H % Hkv == 0, "odit_attn_ruled: H=%d is not a multiple of Hkv=%d", H, Hkv);
-  ODIT_CHECK_ARG(scale > 0.f, "odit_attn_ruled: softmax scale must be positive (got %g)", scale);
+  ODIT_CHECK_ARG(scale >= kMinScale && scale <= kMaxScale, "odit_attn_ruled: softmax scale %g outside [%g, %g]", scale, kMinScale, kMaxScale);
   ODIT_CHECK_ARG(r.window >= 0 && r.window <= kMost, "odit_attn_ruled: window=%d outside [0, %d]", r.window, kMost);
   ODIT_CHECK_ARG(r.docs >= 0 && (r.docs == 0 || (r.q_starts && r.k_starts)), "odit_attn_ruled: documents need q_starts and k_starts");
-  ODIT_CHECK_ARG(r.cap >= 0.f && r.cap <= kMaxCap, "odit_attn_ruled: cap=%g outside [0, %g]", r.cap, kMaxCap);
+  ODIT_CHECK_ARG(r.cap == 0.f || (r.cap >= kMinScale && r.cap <= kMaxCap), "odit_attn_ruled: cap=%g is neither 0 nor in [%g, %g]", r.cap, kMinScale, kMaxCap);
   ODIT_CHECK_ARG(r.slopes == nullptr || r.distance == nullptr, "odit_attn_ruled: slopes and a table exclude each other");
   ODIT_CHECK_ARG(r.distance == nullptr || (r.radius >= 0 && r.radius <= kMaxRadius), "odit_attn_ruled: radius=%d outside [0, %d]", r.radius,
                  kMaxRadius);

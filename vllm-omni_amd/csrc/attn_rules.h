@@ -14,6 +14,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 // For |y| <= 1/2, where a cap leaves most scores, y times a polynomial in y^2 does, the best one in the largest error (a linear
 // programme over 4000 places; 2^-22.9): four instructions at full rate where those two alone take as long as eight.
 constexpr float kMaxCap = 8192.f;
+constexpr float kMinScale = 1e-9f, kMaxScale = 1e9f;  // of scales (and the least cap): their quotients and products with log2(e) are fp32 numbers
 struct Cap {
   float in, out;     // of the exact form: 2 log2(e) scale / cap and cap log2(e)
   float few;         // products below this in size are small enough for the polynomial (0: none)

@@ -149,6 +149,10 @@ extern "C" int odit_rope_append(const void* q, const void* k, const void* v, con
   for (int i = 0; cached && i < 3; ++i)
     ODIT_CHECK_ARG(key_cache_strides[i] % 8 == 0 && value_cache_strides[i] % 8 == 0,
                    "odit_rope_append: cache strides must be multiples of 8 elements");
+  const int64_t cache_sizes[3] = {pages, page_size, Hkv};
+  for (int i = 0; cached && i < 3; ++i)
+    ODIT_CHECK_ARG(cache_sizes[i] <= 1 || (key_cache_strides[i] != 0 && value_cache_strides[i] != 0),
+                   "odit_rope_append: cache rows must not share memory (a stride of 0)");
   if (T == 0) return ODIT_OK;
   ODIT_CHECK_ARG(q && k && positions && turns && q_out && (cached ? v != nullptr : k_out != nullptr), "odit_rope_append: null tensors");
   ODIT_CHECK_ARG(!cached || pages == 0 || (key_cache && value_cache), "odit_rope_append: null caches");

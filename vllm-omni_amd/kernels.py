@@ -342,8 +342,8 @@ def _score_rules(causal, window, cap, slopes, distance, H: int):
     """The ``odit_attn_rules`` that both attentions have, and the tensors that it points into."""
     if window is not None and not 0 < int(window) <= 1 << 30:
         raise ValueError(f"window={window} must be None or in [1, {1 << 30}]")
-    if not 0.0 <= float(cap) <= 8192.0:
-        raise ValueError(f"cap={cap} must be 0 (none) or up to 8192")
+    if not (float(cap) == 0.0 or 1e-9 <= float(cap) <= 8192.0):
+        raise ValueError(f"cap={cap} must be 0 (none) or in [1e-9, 8192]")
     if slopes is not None and distance is not None:
         raise ValueError("slopes and distance exclude each other")
     slopes, distance = _vector("slopes", slopes, torch.float32, H), _vector("distance", distance, torch.float32, H, -1)
