@@ -305,6 +305,16 @@ def test_decode_many_sequences(gpu, B, most):
         _check_paged(q, rows, kernels.attn_paged(q, kc, vc, table, n, 0.1, window=window), 0.1, window, 0.0, {})
 
 
+@pytest.mark.parametrize("B,few", [(1100, {0: 900, 63: 700, 64: 300, 511: 1000, 512: 257, 1050: 600, 1099: 2000}), (600, {}), (513, {512: 5000})], ids=str)
+def test_decode_long_sequences_among_many_short(gpu, B, few):
+    g = torch.Generator().manual_seed(B)
+    lengths = [few.get(b, n) for b, n in enumerate(torch.randint(0, 40, (B,), generator=g).tolist())]
+    (q, kc, vc, table, n), rows = _paged_problem(10, lengths, 16, 2, 1, 64, BF16)
+    o = kernels.attn_paged(q, kc, vc, torch.nn.functional.pad(table, (0, 40)), n, 0.1)  # (also the short ones have a table for more keys than one chunk has)
+    _check_paged(q, rows, o, 0.1, None, 0.0, {})
+    assert torch.equal(o, kernels.attn_paged(q, kc, vc, torch.nn.functional.pad(table, (0, 40)), n, 0.1))
+
+
 def test_decode_strides_and_long_tables(gpu):
     """Keys and values as halves of one cache with the head ahead of the row; a table and lengths that are parts of larger ones; a table for far
     more pages than there are (many chunks, most of them empty)."""

@@ -53,6 +53,7 @@ struct PagedParams {
   Cap cap;
   int group, head_blocks, units;  // units: key heads' blocks of up to 16 query heads, of one sequence
   int wanted, room;               // chunks of all sequences, about, and the most keys of one
+  bool whole;                     // no sequence has more than one
   float* ws;  // per chunk and unit: [heads of a block][D] sums, then [heads of a block] (maximum, sum)
   unsigned* tickets;  // a word for each sequence and unit, zero between launches (nullptr: the join is a launch of its own)
 };
@@ -92,70 +93,100 @@ __device__ __forceinline__ int wave_scan_int(int v) {
   return v;
 }
 
-// How the sequences are cut, from their lengths, which the host does not know: into chunks of one size, whole steps of the workgroup, numbered
-// sequence by sequence, about `wanted` in all (what runs at once), and no more than that where the sequences are few, as one chunk more would
-// then have the others' time again. Cut by the longest that the table has room for instead, into 2048: 8 sequences of 4096 keys 38 us where
-// this takes 31, 48 of 17 to 8192 67 and 62; and what is short in a wide table would run on few compute units.
-// Every wavefront works it out by itself, for the chunk `index` (BY_CHUNK) or for the sequence `index`.
+// How the sequences are cut, from their lengths, which the host does not know: into chunks of one size, whole steps of the workgroup, about
+// `wanted` in all (what runs at once), and no more than that where the sequences are few, as one chunk more would then have the others' time
+// again. Cut by the longest that the table has room for instead, into 2048: 8 sequences of 4096 keys 38 us where this takes 31, 48 of 17 to
+// 8192 67 and 62; and what is short in a wide table would run on few compute units.
+// Workgroups [0, B) have the sequences' first chunks, those behind them the further ones, sequence by sequence: where many sequences are
+// short, next to nobody has to count what lies ahead (numbered sequence by sequence: 4096 sequences of 16 to 64 keys 1500 us, so 300; 1000 of
+// 16 to 300 keys 190 and 136). Every wavefront works it out by itself.
 struct PagedPlace { int b, part, parts, before, chunk, length; };  // before: chunks of the sequences ahead
-template <bool BY_CHUNK>
+// keys that sequence b's query sees
+__device__ __forceinline__ int paged_keys(const PagedParams& p, int b, int* length) {
+  *length = b < p.B ? p.lengths[b] : 0;
+  int first, end;
+  paged_range(p, *length, &first, &end);
+  return end - first;
+}
+// a sequence's chunks past the first
+__device__ __forceinline__ int paged_more(int keys, int chunk) {
+  return keys <= kPagedWhole ? 0 : static_cast<int>(static_cast<uint32_t>(keys - 1) / static_cast<uint32_t>(chunk));
+}
+// The place of chunk `index` among 64 sequences from b0 on, whose keys and lengths the lanes hold; *before: chunks past the first of the
+// sequences ahead of them. True if it is there; otherwise *before includes these 64.
+__device__ __forceinline__ bool paged_among(const PagedParams& p, int index, int b0, int keys, int length, int* before, PagedPlace* at) {
+  const int more = paged_more(keys, at->chunk), upto = wave_scan_int(more);  // of this sequence and those ahead of it among the 64
+  const int past = index - p.B;  // (below 0: a first chunk, of sequence `index`)
+  const int l = __popcll(__ballot(past < 0 ? b0 + static_cast<int>(threadIdx.x & 63) < index : *before + upto <= past));
+  if (l == 64) {
+    *before += __builtin_amdgcn_readlane(upto, 63);
+    return false;
+  }
+  const int own = __builtin_amdgcn_readlane(more, l), ahead = *before + __builtin_amdgcn_readlane(upto, l) - own;
+  at->b = b0 + l;
+  at->before = at->b + ahead;
+  at->parts = 1 + own;
+  at->part = past < 0 ? 0 : 1 + past - ahead;
+  at->length = __builtin_amdgcn_readlane(length, l);
+  return true;
+}
 __device__ __forceinline__ PagedPlace paged_place(const PagedParams& p, int index) {
   const int lane = threadIdx.x & 63;
-  const auto keys_of = [&](int b, int* length) {
-    *length = b < p.B ? p.lengths[b] : 0;
-    int first, end;
-    paged_range(p, *length, &first, &end);
-    return b < p.B ? end - first : 0;
-  };
-  const auto parts_of = [&](int b, int keys, int chunk) {
-    const int n = keys <= kPagedWhole ? 1 : static_cast<int>((static_cast<uint32_t>(keys) + chunk - 1) / static_cast<uint32_t>(chunk));
-    return b < p.B ? max(1, n) : 0;
-  };
-  int length;
-  const int mine = keys_of(lane, &length);
-  int chunk;
+  PagedPlace at{p.B, 0, 1, 0, 0, 0};  // (b == B: behind the last chunk)
+  int length, before = 0;
+  const int mine = paged_keys(p, lane, &length);
   if (p.B <= 64) {
     // (in steps, so that the sum of 64 stays in 32 bits)
     const int steps = wave_sum_int((mine + kPagedStep - 1) / kPagedStep);
     int each = max(kPagedLeast, (steps + p.wanted - 1) / p.wanted);
     if (4 * p.B <= p.wanted) {
       for (int i = 0; i < 3; ++i) {
-        const int made = wave_sum_int(parts_of(lane, mine, each * kPagedStep));
+        const int made = p.B + wave_sum_int(paged_more(mine, each * kPagedStep));
         if (made <= p.wanted) break;
         each = static_cast<int>(static_cast<int64_t>(each) * made / p.wanted) + 1;
       }
     }
-    chunk = min(each, p.room / kPagedStep) * kPagedStep;
-  } else {
-    double total = mine;  // (exact: below 2^53)
-    for (int b0 = 64; b0 < p.B; b0 += 64) {
-      int other;
-      total += keys_of(b0 + lane, &other);
-    }
+    at.chunk = min(each, p.room / kPagedStep) * kPagedStep;
+    paged_among(p, index, 0, mine, length, &before, &at);
+    return at;
+  }
+  int other;
+  if (p.whole) {
+    at.b = index;
+    at.length = p.lengths[index];
+    return at;
+  }
+  int64_t sum = mine;
+  for (int b0 = 64; b0 < p.B; b0 += 512) {
 #pragma unroll
-    for (int s = 1; s < 64; s <<= 1) total += __shfl_xor(total, s, 64);
-    const double each = ceil(total / (static_cast<double>(p.wanted) * kPagedStep));
-    chunk = static_cast<int>(each < kPagedLeast ? kPagedLeast : each > p.room / kPagedStep ? p.room / kPagedStep : each) * kPagedStep;
+    for (int i = 0; i < 8; ++i) sum += paged_keys(p, b0 + i * 64 + lane, &other);
   }
-  chunk = max(__builtin_amdgcn_readfirstlane(chunk), kPagedStep);
-  PagedPlace at{p.B, 0, 0, 0, chunk, 0};
-  int before = 0, keys = mine;
-  for (int b0 = 0; b0 < p.B; b0 += 64) {
-    if (b0 > 0) keys = keys_of(b0 + lane, &length);
-    const int parts = parts_of(b0 + lane, keys, chunk), upto = wave_scan_int(parts);  // of this sequence and those ahead of it among the 64
-    const uint64_t ahead = __ballot(BY_CHUNK ? before + upto <= index : b0 + lane < index);
-    const int l = __popcll(ahead);
-    if (l < 64) {
-      at.b = b0 + l;
-      at.parts = __builtin_amdgcn_readlane(parts, l);
-      at.before = before + __builtin_amdgcn_readlane(upto, l) - at.parts;
-      at.part = BY_CHUNK ? index - at.before : 0;
-      at.length = __builtin_amdgcn_readlane(length, l);
-      return at;
+  double total = static_cast<double>(sum);  // (exact: below 2^53)
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) total += __shfl_xor(total, s, 64);
+  const double each = ceil(total / (static_cast<double>(p.wanted) * kPagedStep));
+  at.chunk = static_cast<int>(each < kPagedLeast ? kPagedLeast : each > p.room / kPagedStep ? p.room / kPagedStep : each) * kPagedStep;
+  at.chunk = max(__builtin_amdgcn_readfirstlane(at.chunk), kPagedStep);
+  if (index < p.B && paged_more(paged_keys(p, index, &other), at.chunk) == 0) {
+    at.b = index;
+    at.length = other;
+    return at;
+  }
+  for (int b0 = 0; b0 < p.B; b0 += 512) {  // 512 sequences at once where the place is none of theirs
+    int more = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) more += paged_more(paged_keys(p, b0 + i * 64 + lane, &other), at.chunk);
+    const int all = wave_sum_int(more);
+    if (index < p.B ? b0 + 512 <= index : before + all <= index - p.B) {
+      before += all;
+      continue;
     }
-    before += __builtin_amdgcn_readlane(upto, 63);
+    for (int i = 0; i < 512; i += 64) {
+      const int keys = paged_keys(p, b0 + i + lane, &length);
+      if (paged_among(p, index, b0 + i, keys, length, &before, &at)) return at;
+    }
   }
-  return at;  // (b == B: behind the last chunk)
+  return at;
 }
 
 // 16 bytes per lane from the lane's own address to LDS bytes lds + 16 * lane
@@ -228,7 +259,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 4
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l16 = lane & 15, g = lane >> 4;
   const int unit = blockIdx.x % p.units;
-  const PagedPlace at = paged_place<true>(p, blockIdx.x / p.units);
+  const PagedPlace at = paged_place(p, blockIdx.x / p.units);
   if (at.b >= p.B) return;
   const int hb = unit % p.head_blocks, hkv = unit / p.head_blocks, b = at.b;
   const int h0 = hkv * p.group + hb * 16, heads = min(16, p.group - hb * 16);
@@ -453,7 +484,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 4
 template <typename T, int D>
 __global__ __launch_bounds__(64) void attn_paged_join_kernel(const PagedParams p) {
   const int h = blockIdx.x % p.H, b = blockIdx.x / p.H, d = threadIdx.x * 2;
-  const PagedPlace at = paged_place<false>(p, b);
+  const PagedPlace at = paged_place(p, b);
   if (at.parts <= 1 || d >= D) return;  // (one chunk's workgroup has written the result)
   const int most = min(16, p.group), unit = h / p.group * p.head_blocks + h % p.group / 16, hd = h % p.group % 16;
   const int64_t step = static_cast<int64_t>(p.units) * most * (D + 2);
@@ -563,6 +594,7 @@ extern "C" int odit_attn_paged(const void* q, const void* key_cache, const void*
   p.units = Hkv * p.head_blocks;
   const PagedPlan plan = paged_plan(B, p.units, paged_most_keys(max_pages, page_size, r.window), page_size);
   p.wanted = plan.wanted; p.room = plan.room;
+  p.whole = plan.chunks == B;
   p.ws = static_cast<float*>(workspace);
   p.tickets = tickets != nullptr && n_tickets >= static_cast<size_t>(B) * p.units ? tickets : nullptr;
   const int bias = r.slopes != nullptr ? 1 : r.distance != nullptr ? 2 : 0;
