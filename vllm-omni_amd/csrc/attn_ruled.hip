@@ -74,6 +74,8 @@ __device__ __forceinline__ int doc_of(const int* starts, int docs, int row0, int
   return doc;
 }
 
+__device__ __forceinline__ int clampi(int x, int lo, int hi) { return x < lo ? lo : x > hi ? hi : x; }
+
 // of the 32 lanes of each half of a wavefront, which hold the same
 template <int CTRL> __device__ __forceinline__ int dpp_int(int v) { return __builtin_amdgcn_update_dpp(v, v, CTRL, 0xf, 0xf, false); }
 __device__ __forceinline__ int half_min(int v) {
@@ -81,8 +83,6 @@ __device__ __forceinline__ int half_min(int v) {
   return min(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16));
 }
 __device__ __forceinline__ int half_max(int v) { return ~half_min(~v); }
-
-__device__ __forceinline__ int clampi(int x, int lo, int hi) { return x < lo ? lo : x > hi ? hi : x; }
 
 // bits of the keys of [t0, t0 + 64) in [lo, hi)
 __device__ __forceinline__ uint64_t range_bits(int lo, int hi, int t0) {
@@ -127,6 +127,14 @@ void attn_ruled_kernel(const RuledParams p) {
     unit = block - at * p.units;
     qb = p.n_qblocks - 1 - at;
   }
+  // (ahead of the queries' loads: they come back in the order of their issue)
+  int q_start = 0, k_start = 0, first_keys = 0;  // docs < 64: the lanes hold all starts, in one trip to memory
+  if (p.docs > 0 && p.docs < 64) {
+    const int at = lane <= p.docs ? lane : p.docs;
+    q_start = p.q_starts[at];
+    k_start = p.k_starts[at];
+    if (p.prefix != nullptr) first_keys = p.prefix[min(at, p.docs - 1)];
+  }
   const int b = p.by_heads(unit), h = unit - b * p.H, hkv = p.by_group(h);
   const int kt0 = KH == 1 ? wave >> 1 : 0;  // the first of this wavefront's halves
   const int q0 = qb * BM + (KH == 1 ? wave & 1 : wave) * 32;
@@ -165,15 +173,13 @@ void attn_ruled_kernel(const RuledParams p) {
     bool in = true;
     if (p.docs > 0) {
       const int row0 = q0 < p.Sq ? q0 : p.Sq - 1;
-      if (p.docs < 64) {  // the lanes hold all starts: one trip to memory
-        const int at = lane <= p.docs ? lane : p.docs;
-        const int q_start = p.q_starts[at], k_start = p.k_starts[at], seen = p.prefix != nullptr ? p.prefix[min(at, p.docs - 1)] : 0;
+      if (p.docs < 64) {
         doc = doc_among(lane < p.docs ? q_start : kNone, 0, row0, row, 0, nullptr);
         qs = __shfl(q_start, doc, 64);
         qe = __shfl(q_start, doc + 1, 64);
         ks = __shfl(k_start, doc, 64);
         kn = __shfl(k_start, doc + 1, 64);
-        prefix = __shfl(seen, doc, 64);
+        prefix = __shfl(first_keys, doc, 64);
       } else {
         doc = doc_of(p.q_starts, p.docs, row0, row);
         qs = p.q_starts[doc];
