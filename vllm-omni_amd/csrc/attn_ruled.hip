@@ -115,7 +115,9 @@ void attn_ruled_kernel(const RuledParams p) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, hh = lane >> 5;
   // the last query blocks, which see most under a causal order, begin first; where the heads divide over the XCDs, an XCD keeps its heads
-  // (steep slopes leave a head little to add: with slopes the heads go round the XCDs, 1040 us of 16384 causal tokens, 16 heads of 128, otherwise, 929 so)
+  // (steep slopes leave a head little to add: with slopes the heads go round the XCDs and back again, so that each has steep and shallow ones: us, of 16384
+  // causal tokens, 16 heads of 128, 1040 with neighbours on an XCD, 929 going round; on another day 970 going round, 950 there and back, 1115 where an XCD
+  // changes its heads with every row of blocks, 917 with every eighth, which costs 8192 tokens 3 %)
   const int chunk = p.chunks > 1 ? p.by_blocks(blockIdx.x) : 0, block = blockIdx.x - chunk * (p.units * p.n_qblocks);
   int unit, qb;
   if (BIAS != 1 && p.units % kNumXcd == 0) {
@@ -126,6 +128,7 @@ void attn_ruled_kernel(const RuledParams p) {
     const int at = p.by_units(block);
     unit = block - at * p.units;
     qb = p.n_qblocks - 1 - at;
+    if (BIAS == 1 && p.units % kNumXcd == 0 && (unit / kNumXcd & 1)) unit ^= kNumXcd - 1;
   }
   // (ahead of the queries' loads: they come back in the order of their issue)
   int q_start = 0, k_start = 0, first_keys = 0;  // docs < 64: the lanes hold all starts, in one trip to memory
