@@ -1,6 +1,7 @@
 """A text stage's operators (``rope_append``, ``attn_ruled``, ``attn_paged``) against their definitions in 64 bits."""
 
 import itertools
+import threading
 
 import pytest
 import torch
@@ -102,6 +103,21 @@ def test_many_documents_and_a_long_gap(gpu):
     for prefix in (1, 64, 130):
         rules = dict(causal=True, window=33, prefix=[prefix])
         _check_ruled(q, k, v, _ruled(q, k, v, 0.1, rules, {}, 0.0), 0.1, rules, {}, 0.0)
+
+
+@pytest.mark.parametrize("causal,window,cap,kind", [(True, None, 0.0, ""), (True, 1000, 5.0, ""), (True, None, 0.0, "slopes"), (False, 700, 0.0, "table"),
+                                                    (False, None, 5.0, "slopes")])
+@pytest.mark.parametrize("D,dtype", [(64, BF16), (128, F16)])
+def test_long_prompts_at_some_rows(gpu, causal, window, cap, kind, D, dtype):
+    S, H, Hkv = 4100, 16, 4  # 33 blocks of 128 queries, the last one of 4
+    q, k, v = _randn(90, 1, S, H, D, dtype=dtype, std=2), _randn(91, 1, S, Hkv, D, dtype=dtype), _randn(92, 1, S, Hkv, D, dtype=dtype)
+    bias = _bias(kind, H, 93, radius=100)
+    o = kernels.attn_ruled(q, k, v, 0.1, causal=causal, window=window, cap=cap, **bias)
+    rows = torch.tensor([0, 1, 127, 128, 1700, 2047, 4090, 4099])
+    away = torch.arange(S)[None] - rows[:, None]
+    seen = (away <= 0 if causal else torch.ones_like(away, dtype=torch.bool)) & (away.abs() < (window or S))
+    want, tol = attention(q[0, rows], k[0], v[0], 0.1, seen, away, cap, **bias)
+    within(o[0, rows], want, tol)
 
 
 @pytest.mark.parametrize("D", [64, 128])
@@ -485,6 +501,84 @@ def test_streams_graphs_and_threads_of_work(gpu):
         for i in range(2):
             assert torch.equal(outs[i][0], want[i]) and torch.equal(outs[i][1], eager[1])
         assert torch.equal(kernels.attn_paged(q, kc, vc, table, lengths, 0.1), eager[0])
+
+
+def test_a_replayed_graph_follows_its_lengths_and_places(gpu):
+    """One captured step of two sequences, replayed as they grow from one chunk to many: each replay gives the eager bits, caches included."""
+    H, Hkv, D, page, pages = 8, 2, 128, 16, 260
+    caches = [[_randn(60 + i, pages, page, Hkv, D) for i in range(2)] for _ in range(2)]  # the graph's and the eager calls'
+    table = torch.randperm(pages, generator=torch.Generator().manual_seed(62)).int().view(2, 130).to("cuda:0")
+    turns = torch.rand(D // 2, generator=torch.Generator().manual_seed(63), dtype=torch.float64).to("cuda:0")
+    q, k, v = (torch.empty(2, h, D, dtype=BF16, device="cuda:0") for h in (H, Hkv, Hkv))
+    lengths, slots = torch.ones(2, dtype=torch.int32, device="cuda:0"), torch.zeros(2, dtype=torch.int64, device="cuda:0")
+
+    def step(kc, vc):
+        turned = kernels.rope_append(q, k, v, lengths.long() - 1, turns, slots=slots, key_cache=kc, value_cache=vc)[0]
+        return kernels.attn_paged(turned, kc, vc, table, lengths, 0.1, window=1500)
+
+    def fill(i, n):
+        for j, t in enumerate((q, k, v)):
+            t.copy_(_randn(64 + 3 * i + j, *t.shape))
+        lengths.copy_(_i32(n))
+        slots.copy_(torch.tensor([int(table[b, (m - 1) // page]) * page + (m - 1) % page for b, m in enumerate(n)], device="cuda:0"))
+
+    fill(0, [1, 1])
+    for both in caches:
+        step(*both)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o = step(*caches[0])
+    for i, n in enumerate([[1, 30], [700, 2080], [2, 257], [2000, 2000], [1, 1]]):
+        fill(i, n)
+        o.zero_()
+        graph.replay()
+        want = step(*caches[1])
+        torch.cuda.synchronize()
+        assert torch.equal(o, want), n
+        assert all(map(torch.equal, caches[0], caches[1]))
+
+
+def test_threads_on_one_stream(gpu):
+    """Each thread's calls join their own chunks."""
+    problems = [_paged_problem(70 + i, n, 16, 8, 2, 64, BF16)[0] for i, n in enumerate([[3000, 40], [500, 4000]])]
+    wants = [kernels.attn_paged(*p, 0.1) for p in problems]
+    torch.cuda.synchronize()
+    failed = []
+
+    def run(i):
+        for _ in range(60):
+            if not torch.equal(kernels.attn_paged(*problems[i], 0.1), wants[i]):
+                failed.append(i)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+
+
+def test_places_past_32_bits(gpu):
+    """Caches and prompts of more than 2^31 elements, their last rows used."""
+    H, Hkv, D, page = 4, 2, 128, 16
+    pages = (1 << 31) // (page * Hkv * D) + 300
+    kc, vc = (torch.empty(pages, page, Hkv, D, dtype=BF16, device="cuda:0") for _ in range(2))
+    n = 70
+    q, k, v = _randn(80, n, H, D), _randn(81, n, Hkv, D), _randn(82, n, Hkv, D)
+    order = [pages - 1 - 7 * i for i in range(-(-n // page))]
+    slots = torch.tensor([order[t // page] * page + t % page for t in range(n)], device="cuda:0")
+    turns, at = torch.zeros(D // 2, dtype=torch.float64, device="cuda:0"), torch.arange(n, device="cuda:0")
+    kernels.rope_append(q, k, v, at, turns, slots=slots, key_cache=kc, value_cache=vc)
+    for t in (0, 15, 16, n - 1):
+        assert torch.equal(kc[order[t // page], t % page], k[t]) and torch.equal(vc[order[t // page], t % page], v[t])
+    o = kernels.attn_paged(q[-1:], kc, vc, _i32([order]), _i32([n]), 0.1)
+    _check_paged(q[-1:], [(k, v)], o, 0.1, None, 0.0, {})
+    far_k, far_v = (t.view(-1, 1).view(-1).as_strided((2, n, Hkv, D), ((1 << 31) + 1024, Hkv * D, D, 1)) for t in (kc, vc))
+    for t, x in ((far_k, k), (far_v, v)):
+        t[0], t[1] = x, x.flip(0)
+    rules = dict(causal=True)
+    os = (kernels.attn_ruled(q[None].expand(2, n, H, D), far_k, far_v, 0.1, **rules),)
+    _check_ruled(q[None].expand(2, n, H, D), torch.stack([k, k.flip(0)]), torch.stack([v, v.flip(0)]), os, 0.1, rules, {}, 0.0)
 
 
 # ------------------------------------------------------------------------------------------------ refusals
