@@ -4,7 +4,7 @@
 //   the query being the last of them. Key j lies in row j % page of cache page table[j / page].
 //
 // Bound by memory: the keys and values are read once, for all query heads of their group together. The group's heads (up to 16; more take
-// another workgroup) are the columns of v_mfma_f32_16x16x32 in both products, S^T = K Q^T and O^T = V^T P^T, so that the arithmetic costs the
+// another workgroup) are the columns of 16 x 16 products, S^T = K Q^T and O^T = V^T P^T, so that the arithmetic costs the
 // same for one head as for 16 and stays far below the loads. A lane then owns one head and the same keys in both products: P stays in registers.
 //
 // The sequences' keys are cut into chunks, a workgroup each; a chunk's tiles of 16 keys go round its 4 wavefronts. A wavefront has two stages
@@ -251,7 +251,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 4
   using frag = typename M::frag;
   constexpr int NW = kPagedWaves, BN = kPagedTile;
   constexpr int ROWB = D * 2, CPR = ROWB / 16, RPI = 64 / CPR, TILEB = BN * ROWB, IPT = BN / RPI;
-  constexpr int KS = D / 32, DT = D / 16, NK = BN / 16;
+  constexpr int KS = D / 32, DT = D / 16;
+  static_assert(BN == 16, "a tile is one product's rows");
   __shared__ __attribute__((aligned(1024))) char lds[NW * 4 * TILEB];  // of each wavefront: K0 V0 K1 V1
   __shared__ int entries[kPagedEntries];
   __shared__ int outside[NW];  // whether a wavefront found page numbers that are none of the cache's
@@ -346,14 +347,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 4
     const char* const vb = kb + TILEB;
     const int k0 = begin + (wave + i * NW) * BN;
     const bool rest = k0 + BN > end || invalid;
-    f32x4_v s[NK];
+    f32x4_v s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int kt = 0; kt < NK; ++kt) s[kt] = f32x4_v{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int st = 0; st < KS; ++st)
-#pragma unroll
-      for (int kt = 0; kt < NK; ++kt)
-        s[kt] = M::run(__builtin_bit_cast(frag, *reinterpret_cast<const u32x4_v*>(kb + kt * 16 * ROWB + (k_lane ^ (st * 64)))), qf[st], s[kt]);
+    for (int st = 0; st < KS; ++st) s = M::run(__builtin_bit_cast(frag, *reinterpret_cast<const u32x4_v*>(kb + (k_lane ^ (st * 64)))), qf[st], s);
     if (rest) {  // what stands in for keys that are none: values of zero, whatever the memory holds (0 times infinity is NaN)
 #pragma unroll
       for (int j = 0; j < IPT; ++j) {
@@ -364,27 +360,21 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 4
     }
     const bool near = BIAS == 2 && k0 + BN - 1 - (n - 1) > -p.radius;  // some key has a bias of its own
 #pragma unroll
-    for (int kt = 0; kt < NK; ++kt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int key = k0 + kt * 16 + g * 4 + e;
-        float x = s[kt][e];
-        if constexpr (MADE) x = CAP ? p.cap(x) : x * p.scale_log2;
-        if constexpr (BIAS == 1) x = fmaf(-slope, static_cast<float>(n - 1 - key), x);
-        if constexpr (BIAS == 2) {
-          if (near) x = fmaf(dist[max(min(key, n - 1) - (n - 1), -p.radius)], kLog2e, x);
-          else x += far;
-        }
-        if (rest) {
-          x = counts(key) ? x : -INFINITY;
-        }
-        s[kt][e] = x;
+    for (int e = 0; e < 4; ++e) {
+      const int key = k0 + g * 4 + e;
+      float x = s[e];
+      if constexpr (MADE) x = CAP ? p.cap(x) : x * p.scale_log2;
+      if constexpr (BIAS == 1) x = fmaf(-slope, static_cast<float>(n - 1 - key), x);
+      if constexpr (BIAS == 2) {
+        if (near) x = fmaf(dist[max(min(key, n - 1) - (n - 1), -p.radius)], kLog2e, x);
+        else x += far;
       }
-    float mx = s[0][0];
+      if (rest) x = counts(key) ? x : -INFINITY;
+      s[e] = x;
+    }
+    float mx = s[0];
 #pragma unroll
-    for (int kt = 0; kt < NK; ++kt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) mx = __builtin_elementwise_maximum(mx, s[kt][e]);
+    for (int e = 1; e < 4; ++e) mx = __builtin_elementwise_maximum(mx, s[e]);
     if (__any((mx - m_run) * c > 8.f)) {  // (as in attn_fwd.hip: the maximum moves only where it is left behind by a factor of 2^8)
       mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
       mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
@@ -398,29 +388,17 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 4
       m_run = m_new;
       mc = m_safe * c;
     }
-    uint32_t pb[2 * NK];
+    u32x2_v pb;
 #pragma unroll
-    for (int kt = 0; kt < NK; ++kt)
-#pragma unroll
-      for (int e = 0; e < 4; e += 2) {
-        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[kt][e], c, -mc)), p1 = __builtin_amdgcn_exp2f(fmaf(s[kt][e + 1], c, -mc));
-        l_run += p0 + p1;
-        pb[kt * 2 + e / 2] = Mma<T>::pack2(p0, p1);
-      }
+    for (int e = 0; e < 4; e += 2) {
+      const float p0 = __builtin_amdgcn_exp2f(fmaf(s[e], c, -mc)), p1 = __builtin_amdgcn_exp2f(fmaf(s[e + 1], c, -mc));
+      l_run += p0 + p1;
+      pb[e / 2] = Mma<T>::pack2(p0, p1);
+    }
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
-      const char* const vp = vb + (v_lane ^ (dt * 32));
-      const s16x4_p lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_pp)(vp));
-      if constexpr (NK == 2) {
-        const s16x4_p hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_pp)(vp + 16 * ROWB));
-        u32x4_v w;
-        w.x = pb[0]; w.y = pb[1]; w.z = pb[2]; w.w = pb[3];
-        o[dt] = M::run(__builtin_bit_cast(frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7)), __builtin_bit_cast(frag, w), o[dt]);
-      } else {
-        u32x2_v w;
-        w.x = pb[0]; w.y = pb[1];
-        o[dt] = M::half(lo, __builtin_bit_cast(s16x4_p, w), o[dt]);
-      }
+      const s16x4_p v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_pp)(vb + (v_lane ^ (dt * 32))));
+      o[dt] = M::half(v, __builtin_bit_cast(s16x4_p, pb), o[dt]);
     }
   }
 

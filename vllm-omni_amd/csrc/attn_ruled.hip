@@ -17,7 +17,6 @@
 namespace odit {
 
 typedef short s16x4_r __attribute__((ext_vector_type(4)));
-typedef short s16x8_r __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) s16x4_r* lds_s16x4_rp;
 typedef __attribute__((address_space(3))) void* lds_void_rp;
 
