@@ -91,10 +91,12 @@ __device__ __forceinline__ uint64_t range_bits(int lo, int hi, int t0) {
   return upto & (~0ull << a);
 }
 
+constexpr int kTablePad = 63;  // a tile's keys but one
 // BIAS 0: none, 1: slopes, 2: table. KH: the 32-key halves of a tile that a wavefront has. With both, the workgroup's 4 wavefronts have 32
 // queries each; with one, two wavefronts share 32 queries, a half of each tile each, and join at the end (ruled_plan says when).
+constexpr int ruled_waves(int D, int KH) { return D == 128 ? 2 : KH == 1 ? 4 : 3; }  // wavefronts of a SIMD, workgroups of a compute unit
 template <typename T, int D, bool CAP, int BIAS, int KH>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 3 : 2, D == 64 ? 3 : 2)))
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ruled_waves(D, KH), ruled_waves(D, KH))))
 void attn_ruled_kernel(const RuledParams p) {
   using M = Mma<T>;
   using frag = typename M::frag;
@@ -108,8 +110,8 @@ void attn_ruled_kernel(const RuledParams p) {
   __shared__ int places[BIAS != 0 ? NW * 32 : 1];  // pos of each lane's query
   __shared__ int4 ranges[NW * 32];  // blo, bhi, plo, phi of each lane's query: read again at each tile, which has no registers to hold them
   // BIAS 2: the head's biases, with the outermost ones once more for each further key of a tile that some distance inside begins or ends
-  constexpr int kPad = BN - 1;
-  __shared__ float table[BIAS == 2 ? 2 * kMaxRadius + 1 + 2 * kPad : 1];
+  constexpr int kPad = kTablePad;
+  extern __shared__ float table[];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, hh = lane >> 5;
@@ -146,8 +148,8 @@ void attn_ruled_kernel(const RuledParams p) {
   frag qf[KS];
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) qf[ks] = __builtin_bit_cast(frag, *reinterpret_cast<const u32x4_v*>(qrow + hh * 8 + ks * 16));
-  // (three workgroups to a compute unit: some fragments are read again at each tile, for want of a few registers)
-  constexpr int QL = D != 64 ? 0 : CAP && BIAS != 2 ? 4 : 2;
+  // (three or four workgroups to a compute unit: some fragments are read again at each tile, for want of a few registers)
+  constexpr int QL = D != 64 ? 0 : KH == 1 ? (BIAS == 2 ? 0 : 1) : CAP && BIAS != 2 ? 4 : 2;
   __shared__ u32x4_v q_lds[QL > 0 ? QL * NW * 64 : 1];
   auto q_at = [&](int ks) __attribute__((always_inline)) {
     if (ks >= QL) return qf[ks];
@@ -721,14 +723,18 @@ __global__ __launch_bounds__(256) void attn_ruled_merge_kernel(const RuledParams
 //   causal      S=512 H=8 [32] 14.5 / 12.3    S=512 H=32 of 64 [128] 11.8 / 9.9    S=1024 H=24 [192] 25.0 / 22.0    S=2048 H=32 of 64 [512] 37.6 / 31.3
 //               S=4096 H=16 [512] 93.5 / 85.9    S=8192 H=8 [512] 176 / 159    S=3000 H=24 [576] 75.3 / 79.0    S=4096 H=24 of 64 [768] 75.9 / 79.3
 //   all keys    S=512 H=8 [32] 14.0 / 12.1    S=512 H=32 of 64 [128] 11.6 / 9.9    S=1024 H=24 [192] 25.4 / 25.8    B=3 S=300 H=24 [216] 11.7 / 12.9
-//               S=2048 H=32 [512] 72 / 86    four documents of 1024 tokens, H=64 of 64, with a table [512] 26.6 / 31.0
+//               S=2048 H=32 [512] 72 / 86    S=1024 H=64 of 64 [512] 27.5 / 29.6
+//   documents   (ragged, whose workgroups end at different times) S=1024 H=24 [192] 25.1 / 22.9, causal 23.0 / 20.0    S=1024 H=64 [512] 32.7 / 43.5
+//               of 64 features: S=1024 H=64 [512] with a table 28.1 / 27.3, causal 20.7 / 18.8    8 in S=2048 H=32 causal [512] 25.0 / 20.4
+//               S=1500 H=64 causal [768] 29.5 / 26.6    10 in S=4000 H=48 causal [1536] 46.0 / 47.6    23 in S=12007 H=32 causal [3008] 100 / 107
 // Where a call still has fewer workgroups than the GPU has room for, its tiles are cut into chunks, as many as cost least: the join is a launch
 // of 3 us and its sums' way to memory and back, 8 bytes a feature.
 struct RuledPlan { int halves, chunks; };
 static RuledPlan ruled_plan(int B, int Sq, int Sk, int H, int D, int docs, int window, int causal) {
   const auto blocks = [&](int bm) { return static_cast<int64_t>((Sq + bm - 1) / bm) * H * B; };
-  RuledPlan plan{blocks(128) <= 128 || (causal && docs == 0 && blocks(128) <= 512) ? 1 : 2, 1};
-  const int64_t mine = blocks(64 * plan.halves), room = D == 128 ? 512 : 768;
+  const int64_t few = docs > 0 ? (D == 128 ? 256 : 768) : causal ? 512 : 128;
+  RuledPlan plan{blocks(128) <= few ? 1 : 2, 1};
+  const int64_t mine = blocks(64 * plan.halves), room = D == 128 ? 512 : 768;  // (1024 at halves of 64 features: 500 rows of 3000 keys 31.1 us, so 29.7)
   int64_t keys = docs > 0 ? 2 * (Sk / docs) + 64 : Sk;  // that a query block may see, about
   if (window > 0) {
     const int64_t most = (causal ? 1ll : 2ll) * window + 128;
@@ -760,7 +766,8 @@ static int launch_ruled(RuledParams& p, bool cap, int bias, hipStream_t stream) 
   p.by_units = quotient(bias != 1 && p.units % kNumXcd == 0 ? p.units / kNumXcd : p.units);
   p.by_heads = quotient(p.H);
   p.by_group = quotient(p.group);
-#define ODIT_RULED_GO(C, X) hipLaunchKernelGGL((attn_ruled_kernel<T, D, C, X, KH>), dim3(total), dim3(256), 0, stream, p)
+  const size_t lds = bias == 2 ? (2 * p.radius + 1 + 2 * kTablePad) * sizeof(float) : 0;
+#define ODIT_RULED_GO(C, X) hipLaunchKernelGGL((attn_ruled_kernel<T, D, C, X, KH>), dim3(total), dim3(256), lds, stream, p)
   if (cap) {
     if (bias == 0) ODIT_RULED_GO(true, 0); else if (bias == 1) ODIT_RULED_GO(true, 1); else ODIT_RULED_GO(true, 2);
   } else {
