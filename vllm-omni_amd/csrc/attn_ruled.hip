@@ -310,6 +310,10 @@ void attn_ruled_kernel(const RuledParams p) {
   };
 
   constexpr bool POLY = CAP && BIAS == 0;
+  // Where a tile's probabilities are made: between the matrix instructions of the next one's scores, or where the compiler would have them, in the branch
+  // that takes them, beside the second product. us, there / pinned: 4096 tokens, 24 heads of 64, all keys 125 / 117, causal 82.8 / 85.7; capped window of
+  // 4096 in 8192 tokens, 32 heads of 128, 533 / 526; a table in 12 documents, 24 heads of 128, 109 / 106. With slopes many tiles have none: 940 / 974.
+  constexpr bool PINNED = BIAS == 0 || (BIAS == 2 && D == 128);
   // the score of a key that is not seen (POLY: finite, as are all capped ones, for the polynomial 1 + 0 s^2 + ..; its exp2 is zero all the same)
   const float kOut = POLY ? -1e18f : -INFINITY;
   // whether some query of the wavefront sees a key of the tile from t0 on, and whether all of them see all
@@ -444,7 +448,9 @@ void attn_ruled_kernel(const RuledParams p) {
         const int kt = pi >> 3, e = (pi & 7) * 2;
         const float p0 = __builtin_amdgcn_exp2f(exponent(s_cur[kt][e])), p1 = __builtin_amdgcn_exp2f(exponent(s_cur[kt][e + 1]));
         sum += p0 + p1;
-        pf[kt][(pi & 7) >> 2][pi & 3] = M::pack2(p0, p1);
+        uint32_t both = M::pack2(p0, p1);
+        if constexpr (PINNED) asm volatile("" : "+v"(both), "+v"(sum));
+        pf[kt][(pi & 7) >> 2][pi & 3] = both;
       };
       __builtin_amdgcn_s_setprio(2);
       const char* const kb = lds + (buf ^ 1) * TILEB;
