@@ -99,7 +99,8 @@ typedef struct odit_attn_rules {
  * fp16, D 64 or 128. Documents cut every batch row alike. A query that sees nothing gets zeros; what keys and values hold that a query does
  * not see (NaN and infinities too) does not reach it.
  * `workspace`: NULL, or odit_attn_ruled_workspace_bytes for the same shape and rules (may be 0; no device memory is read for it), contents
- * irrelevant before and after: few rows' long keys are then cut into ranges that run side by side and are joined by a second launch. */
+ * irrelevant before and after: few rows' long keys are then cut into ranges that run side by side and are joined by a second launch, and
+ * with slopes far keys whose probabilities are zero in 32 bits are left out, by a bound that a first launch takes from all keys. */
 int odit_attn_ruled(const void* q, const void* k, const void* v, void* o, int B, int Sq, int Sk, int H, int Hkv, int D,
                     const int64_t q_strides[3], const int64_t k_strides[3], const int64_t v_strides[3], const int64_t o_strides[3],
                     float scale, const odit_attn_rules* rules, int dtype, void* workspace, size_t workspace_bytes, void* stream);

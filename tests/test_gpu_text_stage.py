@@ -1,5 +1,6 @@
 """A text stage's operators (``rope_append``, ``attn_ruled``, ``attn_paged``) against their definitions in 64 bits."""
 
+import ctypes
 import itertools
 import threading
 
@@ -7,7 +8,7 @@ import pytest
 import torch
 
 from text_stage import attention, rotated, seen_keys, within
-from vllm_omni_amd import kernels
+from vllm_omni_amd import _lib, kernels
 
 pytestmark = pytest.mark.gpu
 
@@ -117,6 +118,50 @@ def test_long_prompts_at_some_rows(gpu, causal, window, cap, kind, D, dtype):
     away = torch.arange(S)[None] - rows[:, None]
     seen = (away <= 0 if causal else torch.ones_like(away, dtype=torch.bool)) & (away.abs() < (window or S))
     want, tol = attention(q[0, rows], k[0], v[0], 0.1, seen, away, cap, **bias)
+    within(o[0, rows], want, tol)
+
+
+def _all_tiles(q, k, v, scale, causal, window, cap, slopes, prefix=None):
+    """The call without scratch, which visits all tiles that are seen."""
+    lib = _lib.load()
+    rules = _lib.AttnRules(causal=int(causal), window=window or 0, cap=cap, slopes=slopes.data_ptr(), prefix=None if prefix is None else prefix.data_ptr())
+    o = torch.empty_like(q)
+    (B, Sq, H, D), (_, Sk, Hkv, _) = q.shape, k.shape
+    _lib.check(lib.odit_attn_ruled(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), B, Sq, Sk, H, Hkv, D, *(_lib.i64_array(t.stride()[:3]) for t in (q, k, v, o)), scale,
+        ctypes.byref(rules), 0 if q.dtype == BF16 else 1, None, 0, torch.cuda.current_stream().cuda_stream), "odit_attn_ruled")
+    return o
+
+
+@pytest.mark.parametrize("Sq,Sk,causal,window", [(6200, 6200, True, None), (1030, 6145, True, None), (6144, 6144, False, None), (6300, 6300, True, 700)])
+@pytest.mark.parametrize("D,dtype,H,Hkv", [(128, BF16, 24, 8), (64, F16, 40, 40)])
+def test_slopes_leave_far_tiles_out(gpu, Sq, Sk, causal, window, D, dtype, H, Hkv):
+    """What is left out has no weight in 32 bits: the bits of the call that visits all tiles, under a causal order, where both begin at a query's own
+    key. (Otherwise the far keys come first, and the running maximum, which may lag by a factor of 2^8, goes another way: other roundings of the
+    probabilities, so some rows against the definition.) Also with one long key far away, one that holds NaN, one that holds infinities, slopes of
+    zero and below, and a prefix that all see."""
+    q, k, v = _randn(100, 1, Sq, H, D, dtype=dtype), _randn(101, 1, Sk, Hkv, D, dtype=dtype), _randn(102, 1, Sk, Hkv, D, dtype=dtype)
+    slopes = torch.tensor([4.0 * 2.0 ** (-12.0 * h / H) for h in range(H)], device="cuda:0")
+    slopes[5], slopes[7] = 0.0, -0.01
+    rows = torch.tensor([0, 600, Sq - 1])
+    away = torch.arange(Sk)[None] - (rows[:, None] + Sk - Sq)
+    seen = (away <= 0 if causal else torch.ones_like(away, dtype=torch.bool)) & (away.abs() < (window or Sk))
+    for what in (None, 30.0, float("nan"), float("inf")):
+        if what is not None:
+            k[0, 3, 0] = k[0, 3, 0] * what
+        for prefix in (None, _i32([70])):
+            o = kernels.attn_ruled(q, k, v, D ** -0.5, causal=causal, window=window, slopes=slopes, prefix=prefix)
+            full = _all_tiles(q, k, v, D ** -0.5, causal, window, 0.0, slopes, prefix)
+            assert torch.equal(o.isnan(), full.isnan())
+            if causal:
+                assert torch.equal(o.nan_to_num(77.0), full.nan_to_num(77.0)), (what, prefix)
+            if what in (None, 30.0) and prefix is None:
+                want, tol = attention(q[0, rows], k[0], v[0], D ** -0.5, seen, away, 0.0, slopes=slopes)
+                within(o[0, rows], want, tol)
+                within(full[0, rows], want, tol)
+    k = _randn(101, 1, Sk, Hkv, D, dtype=dtype)
+    o = kernels.attn_ruled(q, k, v, D ** -0.5, causal=causal, window=window, slopes=slopes, cap=5.0)  # (a cap is a bound by itself)
+    want, tol = attention(q[0, rows], k[0], v[0], D ** -0.5, seen, away, 5.0, slopes=slopes)
     within(o[0, rows], want, tol)
 
 

@@ -35,6 +35,8 @@ struct RuledParams {
   Quotient by_blocks, by_units, by_heads, by_group;  // by n_qblocks * units, by the units of a row of blocks (of an XCD), by H, by group
   int bm;                // queries of a block
   int chunks;            // workgroups that share a query block's tiles; with more than one, their sums go to ws
+  bool cut;              // slopes: far tiles are left out whose probabilities are zero
+  const float* norms;    // [B][Hkv][kNormParts]: the largest squared length of a part's keys (with a cap: nullptr, not needed)
   float* ws;             // [units][n_qblocks][chunks][bm][D] sums, then [...][bm] (maximum in units of log2, sum)
 };
 
@@ -92,6 +94,40 @@ __device__ __forceinline__ uint64_t range_bits(int lo, int hi, int t0) {
 }
 
 constexpr int kTablePad = 63;  // a tile's keys but one
+// The keys' largest squared lengths, in kNormParts parts of each head's: a lane of the kernel below reads each. A workgroup has a part; D / 8 lanes a key.
+constexpr int kNormParts = 64;
+template <typename T, int D>
+__global__ __launch_bounds__(256) void attn_ruled_norms_kernel(const RuledParams p, float* norms) {
+  constexpr int LPK = D / 8, KPI = 256 / LPK;
+  __shared__ float waves[4];
+  const int part = blockIdx.x % kNormParts, head = blockIdx.x / kNormParts, b = head / p.Hkv, hkv = head % p.Hkv;
+  const int each = (p.Sk + kNormParts - 1) / kNormParts, begin = min(part * each, p.Sk), end = min(begin + each, p.Sk);
+  const T* const base = static_cast<const T*>(p.k) + b * p.ks_b + hkv * p.ks_h + threadIdx.x % LPK * 8;
+  float most = 0.f;
+  for (int first = begin; first < end; first += 4 * KPI) {  // (for all lanes alike: they exchange sums)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int key = min(first + i * KPI + static_cast<int>(threadIdx.x) / LPK, end - 1);
+      const u32x4 x = load_raw(base + key * p.ks_s);
+      float sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum = fmaf(Raw<T>::get(x, e), Raw<T>::get(x, e), sum);
+#pragma unroll
+      for (int s = 1; s < LPK; s <<= 1) sum += __shfl_xor(sum, s, 64);
+      most = __builtin_elementwise_maximum(most, sum);
+    }
+  }
+#pragma unroll
+  for (int s = LPK; s < 64; s <<= 1) most = __builtin_elementwise_maximum(most, __shfl_xor(most, s, 64));
+  if (threadIdx.x % 64 == 0) waves[threadIdx.x / 64] = most;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int w = 1; w < 4; ++w) most = __builtin_elementwise_maximum(most, waves[w]);
+    norms[blockIdx.x] = most;
+  }
+}
+
 // BIAS 0: none, 1: slopes, 2: table. KH: the 32-key halves of a tile that a wavefront has. With both, the workgroup's 4 wavefronts have 32
 // queries each; with one, two wavefronts share 32 queries, a half of each tile each, and join at the end (ruled_plan says when).
 constexpr int ruled_waves(int D, int KH) { return D == 128 ? 2 : KH == 1 ? 4 : 3; }  // wavefronts of a SIMD, workgroups of a compute unit
@@ -116,9 +152,10 @@ void attn_ruled_kernel(const RuledParams p) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, hh = lane >> 5;
   // the last query blocks, which see most under a causal order, begin first; where the heads divide over the XCDs, an XCD keeps its heads
-  // (steep slopes leave a head little to add: with slopes the heads go round the XCDs and back again, so that each has steep and shallow ones: us, of 16384
-  // causal tokens, 16 heads of 128, 1040 with neighbours on an XCD, 929 going round; on another day 970 going round, 950 there and back, 1115 where an XCD
-  // changes its heads with every row of blocks, 917 with every eighth, which costs 8192 tokens 3 %)
+  // (steep slopes leave a head little to do: with slopes the heads go round the XCDs and back again, so that each has steep and shallow ones, and an XCD
+  // begins its rows of blocks with each of its heads in turn: it hands workgroups to its shader engines in a fixed order, so that those which
+  // would get steep heads alone stood empty while the others were full. us of 16384 causal tokens, 16 heads of 128: 1040 with neighbours on an XCD, 929 going
+  // round, 910 there and back; with far tiles left out 860, and 645 with the heads in turn)
   const int chunk = p.chunks > 1 ? p.by_blocks(blockIdx.x) : 0, block = blockIdx.x - chunk * (p.units * p.n_qblocks);
   int unit, qb;
   if (BIAS != 1 && p.units % kNumXcd == 0) {
@@ -129,7 +166,10 @@ void attn_ruled_kernel(const RuledParams p) {
     const int at = p.by_units(block);
     unit = block - at * p.units;
     qb = p.n_qblocks - 1 - at;
-    if (BIAS == 1 && p.units % kNumXcd == 0 && (unit / kNumXcd & 1)) unit ^= kNumXcd - 1;
+    if (BIAS == 1 && p.units % kNumXcd == 0) {
+      const int per = p.units / kNumXcd, j = (unit / kNumXcd + at / 2) % per, xcd = unit % kNumXcd;
+      unit = j * kNumXcd + (j & 1 ? kNumXcd - 1 - xcd : xcd);
+    }
   }
   // (ahead of the queries' loads: they come back in the order of their issue)
   int q_start = 0, k_start = 0, first_keys = 0;  // docs < 64: the lanes hold all starts, in one trip to memory
@@ -250,6 +290,50 @@ void attn_ruled_kernel(const RuledParams p) {
     if (c1 > c0 && c0 <= a1 && a0 <= c1) { a0 = min(a0, c0); a1 = max(a1, c1); c0 = c1 = 0; }        // they touch
     s1 = __builtin_amdgcn_readfirstlane(a0); n1 = __builtin_amdgcn_readfirstlane(a1 - a0);
     s2 = __builtin_amdgcn_readfirstlane(c0); n2 = __builtin_amdgcn_readfirstlane(c1 - c0);
+  }
+  if constexpr (BIAS == 1) {
+    // Slopes: no product exceeds |q| |k| in size (or the cap), a query's own key has no bias, so its maximum is at least -|q| |k|, and a key
+    // `reach` away has a probability of 2^-160 at most beside it, which is zero in 32 bits (2^-8 of that is what the running maximum may lag). Tiles
+    // farther off than that from all queries are left out: of 16384 causal tokens, 16 heads with slopes of 2^-1/2 to 2^-8, more than half.
+    const float steep = p.slopes[h] * kLog2e;
+    if (p.cut && steep > 0.f) {
+      float most = p.cap.out;
+      if constexpr (!CAP) {
+        float q2 = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          const u32x4 x = __builtin_bit_cast(u32x4, qf[ks]);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) q2 = fmaf(Raw<T>::get(x, e), Raw<T>::get(x, e), q2);
+        }
+        q2 += __shfl_xor(q2, 32, 64);
+        float k2 = p.norms[(static_cast<int64_t>(b) * p.Hkv + hkv) * kNormParts + lane];
+#pragma unroll
+        for (int sft = 1; sft < 64; sft <<= 1) {  // (NaN stays NaN)
+          q2 = __builtin_elementwise_maximum(q2, __shfl_xor(q2, sft, 64));
+          k2 = __builtin_elementwise_maximum(k2, __shfl_xor(k2, sft, 64));
+        }
+        __shared__ float lengths[NW];
+        if (lane == 0) lengths[wave] = q2;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < NW; ++w) q2 = __builtin_elementwise_maximum(q2, lengths[w]);
+        most = p.scale_log2 * sqrtf(q2) * sqrtf(k2) * 1.001f;
+      }
+      const float reach = (2.f * most + 160.f) / steep * 1.001f + 1.f;
+      const int far = __builtin_amdgcn_readfirstlane(reach < 1e9f ? static_cast<int>(reach) + 1 : -1);  // (-1 for NaN and infinities too)
+      if (far >= 0) {
+        const int row0 = qb * BM + p.Sk - p.Sq, row1 = min(qb * BM + BM, p.Sq) - 1 + p.Sk - p.Sq;
+        const int from = max(row0 - far, 0) / BN, to = (row1 + far) / BN + 1;
+        const auto trim = [&](int& first, int& n) {
+          const int end = min(first + n, to);
+          first = max(first, from);
+          n = max(end - first, 0);
+        };
+        trim(s1, n1);
+        trim(s2, n2);
+      }
+    }
   }
   // this workgroup's of them: tile i is number last - i of both runs together
   int last = n1 + n2 - 1, n_tiles = n1 + n2;
@@ -735,11 +819,17 @@ __global__ __launch_bounds__(256) void attn_ruled_merge_kernel(const RuledParams
 //               S=1500 H=64 causal [768] 29.5 / 26.6    10 in S=4000 H=48 causal [1536] 46.0 / 47.6    23 in S=12007 H=32 causal [3008] 100 / 107
 // Where a call still has fewer workgroups than the GPU has room for, its tiles are cut into chunks, as many as cost least: the join is a launch
 // of 3 us and its sums' way to memory and back, 8 bytes a feature.
-struct RuledPlan { int halves, chunks; };
-static RuledPlan ruled_plan(int B, int Sq, int Sk, int H, int D, int docs, int window, int causal) {
+// With slopes and no cap, a launch that reads all keys once gives the bound that far tiles are left out by. us, without / with it, causal, slopes from
+// 2^(-8/H) to 2^-8: 4 prompts of 2048, 16 heads of 128, 84 / 93; 4096, 24 of 64, 87 / 88; 6144, 32 of 128, 271 / 232; 8192, 32 on 8, 437 / 352; 16384, 16,
+// 860 / 645. A cap is a bound by itself: 16384, 16 heads, a cap of 30, 1255 / 775.
+struct RuledPlan { int halves, chunks; bool cut, norms; };
+static RuledPlan ruled_plan(int B, int Sq, int Sk, int H, int D, const odit_attn_rules& r) {
+  const int docs = r.docs, window = r.window, causal = r.causal;
   const auto blocks = [&](int bm) { return static_cast<int64_t>((Sq + bm - 1) / bm) * H * B; };
   const int64_t few = docs > 0 ? (D == 128 ? 256 : 768) : causal ? 512 : 128;
-  RuledPlan plan{blocks(128) <= few ? 1 : 2, 1};
+  RuledPlan plan{blocks(128) <= few ? 1 : 2, 1, r.slopes != nullptr && docs == 0 && Sk >= Sq, false};  // (cut: every query has a key at its own place)
+  plan.norms = plan.cut && r.cap == 0.f && Sq >= 1024 && Sk >= 6144;
+  plan.cut = plan.norms || (plan.cut && r.cap > 0.f);
   const int64_t mine = blocks(64 * plan.halves), room = D == 128 ? 512 : 768;  // (1024 at halves of 64 features: 500 rows of 3000 keys 31.1 us, so 29.7)
   int64_t keys = docs > 0 ? 2 * (Sk / docs) + 64 : Sk;  // that a query block may see, about
   if (window > 0) {
@@ -755,9 +845,12 @@ static RuledPlan ruled_plan(int B, int Sq, int Sk, int H, int D, int docs, int w
   return plan;
 }
 
+static size_t ruled_norms_bytes(const RuledPlan& plan, int B, int H) {  // (as if each head had keys of its own)
+  return plan.norms ? static_cast<size_t>(B) * H * kNormParts * sizeof(float) : 0;
+}
 static size_t ruled_workspace_bytes(const RuledPlan& plan, int B, int Sq, int H, int D) {
   const int bm = 64 * plan.halves;
-  return plan.chunks > 1 ? static_cast<size_t>((Sq + bm - 1) / bm) * H * B * plan.chunks * bm * (D + 2) * sizeof(float) : 0;
+  return ruled_norms_bytes(plan, B, H) + (plan.chunks > 1 ? static_cast<size_t>((Sq + bm - 1) / bm) * H * B * plan.chunks * bm * (D + 2) * sizeof(float) : 0);
 }
 
 template <typename T, int D, int KH>
@@ -773,6 +866,11 @@ static int launch_ruled(RuledParams& p, bool cap, int bias, hipStream_t stream) 
   p.by_heads = quotient(p.H);
   p.by_group = quotient(p.group);
   const size_t lds = bias == 2 ? (2 * p.radius + 1 + 2 * kTablePad) * sizeof(float) : 0;
+  if (p.norms != nullptr) {
+    const int64_t heads = static_cast<int64_t>(p.B) * p.Hkv * kNormParts;
+    ODIT_CHECK_ARG(heads < (1ll << 24), "odit_attn_ruled: grid of %lld workgroups is too large", static_cast<long long>(heads));
+    hipLaunchKernelGGL((attn_ruled_norms_kernel<T, D>), dim3(heads), dim3(256), 0, stream, p, const_cast<float*>(p.norms));
+  }
 #define ODIT_RULED_GO(C, X) hipLaunchKernelGGL((attn_ruled_kernel<T, D, C, X, KH>), dim3(total), dim3(256), lds, stream, p)
   if (cap) {
     if (bias == 0) ODIT_RULED_GO(true, 0); else if (bias == 1) ODIT_RULED_GO(true, 1); else ODIT_RULED_GO(true, 2);
@@ -796,7 +894,7 @@ static int launch_ruled(RuledParams& p, const RuledPlan& plan, bool cap, int bia
 extern "C" size_t odit_attn_ruled_workspace_bytes(int B, int Sq, int Sk, int H, int D, const odit_attn_rules* rules) {
   using namespace odit;
   if (B <= 0 || Sq <= 0 || Sk <= 0 || H <= 0 || D <= 0 || rules == nullptr) return 0;
-  return ruled_workspace_bytes(ruled_plan(B, Sq, Sk, H, D, rules->docs, rules->window, rules->causal), B, Sq, H, D);
+  return ruled_workspace_bytes(ruled_plan(B, Sq, Sk, H, D, *rules), B, Sq, H, D);
 }
 
 extern "C" int odit_attn_ruled(const void* q, const void* k, const void* v, void* o, int B, int Sq, int Sk, int H, int Hkv, int D,
@@ -847,11 +945,17 @@ extern "C" int odit_attn_ruled(const void* q, const void* k, const void* v, void
   p.os_b = o_strides[0]; p.os_s = o_strides[1]; p.os_h = o_strides[2];
   p.scale_log2 = scale * kLog2e;
   p.bias_scale = 1.f / scale;
-  // (without scratch, or with less than that takes, a query block's tiles stay in one piece)
-  RuledPlan plan = ruled_plan(B, Sq, Sk, H, D, r.docs, r.window, r.causal);
-  if (workspace == nullptr || workspace_bytes < ruled_workspace_bytes(plan, B, Sq, H, D)) plan.chunks = 1;
+  // (without scratch, or with less than that takes, a query block's tiles stay in one piece and all are visited)
+  RuledPlan plan = ruled_plan(B, Sq, Sk, H, D, r);
+  if (workspace == nullptr || workspace_bytes < ruled_workspace_bytes(plan, B, Sq, H, D)) {
+    plan.chunks = 1;
+    plan.cut = plan.cut && !plan.norms;
+    plan.norms = false;
+  }
   p.chunks = plan.chunks;
-  p.ws = static_cast<float*>(workspace);
+  p.cut = plan.cut;
+  p.norms = plan.norms ? static_cast<float*>(workspace) : nullptr;
+  p.ws = static_cast<float*>(workspace) + ruled_norms_bytes(plan, B, H) / sizeof(float);
   p.cap = make_cap(r.cap, scale);
   const int bias = r.slopes != nullptr ? 1 : r.distance != nullptr ? 2 : 0;
   hipStream_t st = static_cast<hipStream_t>(stream);
