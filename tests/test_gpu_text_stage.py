@@ -165,6 +165,21 @@ def test_slopes_leave_far_tiles_out(gpu, Sq, Sk, causal, window, D, dtype, H, Hk
     within(o[0, rows], want, tol)
 
 
+@pytest.mark.parametrize("causal", [True, False])
+def test_slopes_over_cut_keys(gpu, causal):
+    """Few heads, whose keys are cut into ranges of the tiles that are left; the scratch is for both."""
+    Sq, Sk, H, D = 1030, 9000, 2, 64
+    need = lambda **rules: _lib.load().odit_attn_ruled_workspace_bytes(1, Sq, Sk, H, D, ctypes.byref(_lib.AttnRules(causal=int(causal), **rules)))  # noqa: E731
+    q, k, v = _randn(110, 1, Sq, H, D), _randn(111, 1, Sk, 1, D), _randn(112, 1, Sk, 1, D)
+    slopes = torch.tensor([0.5, 0.02], device="cuda:0")
+    assert need() > 0 and need(slopes=slopes.data_ptr()) - need() == H * 64 * 4
+    o = kernels.attn_ruled(q, k, v, 0.125, causal=causal, slopes=slopes)
+    rows = torch.tensor([0, 63, 64, 500, Sq - 1])
+    away = torch.arange(Sk)[None] - (rows[:, None] + Sk - Sq)
+    want, tol = attention(q[0, rows], k[0], v[0], 0.125, away <= 0 if causal else torch.ones_like(away, dtype=torch.bool), away, 0.0, slopes=slopes)
+    within(o[0, rows], want, tol)
+
+
 @pytest.mark.parametrize("D", [64, 128])
 def test_prompt_strides(gpu, D):
     """q, k and v as parts of one projection; keys and values with the head ahead of the row; odd strides, which are copied."""
