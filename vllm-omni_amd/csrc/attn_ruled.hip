@@ -29,6 +29,7 @@ struct RuledParams {
   int B, Sq, Sk, H, Hkv;
   int64_t qs_b, qs_s, qs_h, ks_b, ks_s, ks_h, vs_b, vs_s, vs_h, os_b, os_s, os_h;
   float scale_log2, bias_scale;  // scale log2(e) and 1 / scale
+  float unit;                    // from what scores are kept in to units of log2: scale log2(e), or 1 behind a cap
   Cap cap;
   int n_qblocks, units;  // units: heads of all batch rows
   int group;             // query heads of a key head
@@ -37,7 +38,7 @@ struct RuledParams {
   int chunks;            // workgroups that share a query block's tiles; with more than one, their sums go to ws
   bool cut;              // slopes: far tiles are left out whose probabilities are zero
   const float* norms;    // [B][Hkv][kNormParts]: the largest squared length of a part's keys (with a cap: nullptr, not needed)
-  float* ws;             // [units][n_qblocks][chunks][bm][D] sums, then [...][bm] (maximum in units of log2, sum)
+  float* ws;             // [units][n_qblocks][chunks][bm][D] sums, then [...][bm] (maximum in units of scores, sum)
 };
 
 // Among 64 documents from `base` on, whose starts the lanes hold: the last one that starts at or before the lane's row, one of the 32 from
@@ -203,7 +204,7 @@ void attn_ruled_kernel(const RuledParams p) {
   const float bias_unit = CAP ? kLog2e : p.bias_scale;
   if constexpr (BIAS == 2) {
     const float* from = p.distance + static_cast<int64_t>(h) * (2 * p.radius + 1);
-    for (int i = tid; i <= 2 * p.radius + 2 * kPad; i += 256) table[i] = from[clampi(i - kPad, 0, 2 * p.radius)] * bias_unit;
+    for (int i = tid; i <= 2 * p.radius + 2 * kPad; i += 256) table[i] = in_units(from[clampi(i - kPad, 0, 2 * p.radius)], bias_unit);
   }
 
   // ---- what this lane's query sees ----
@@ -383,7 +384,14 @@ void attn_ruled_kernel(const RuledParams p) {
     for (int e = 0; e < 16; ++e) o[dt][e] = 0.f;
   const float c = CAP ? 1.f : p.scale_log2;  // from what m_run is in to units of log2
   float m_run = -INFINITY, l_run = 0.f, mc = 0.f;
-  const float slope = BIAS == 1 ? p.slopes[h] * bias_unit : 0.f;
+  // An exponent is s c - mc in one instruction, mc being m c rounded. What that rounding loses is the same for all of a row's keys, but it grows with
+  // the maximum (past 2^31 an exponent of zero comes out above 128). So where m c is past kFar, scores are made differences from the maximum ahead of
+  // the exponent, and mc is zero. Scores of that size are rare (biases that forbid are: -1e10 at every key that a query sees so far), so it is
+  // a branch by a scalar.
+  constexpr float kFar = 1024.f;
+  bool far_max = false;  // some query of the wavefront is there
+  const auto is_far = [&]() __attribute__((always_inline)) { return fabsf(m_run * c) > kFar && fabsf(m_run) < INFINITY; };
+  const float slope = BIAS == 1 ? in_units(p.slopes[h], bias_unit) : 0.f;
 
   const int k_lane = (32 * kt0 + l32) * ROWB + ((hh ^ k_swizzle(l32)) << 4);
   const int sq = (lane & 15) >> 2, dh = (lane >> 4) & 1;
@@ -499,7 +507,18 @@ void attn_ruled_kernel(const RuledParams p) {
         for (int e = 0; e < 16; ++e) o[dt][e] *= alpha;
       m_run = m_new;
       mc = m_safe * c;
+      if constexpr (!CAP) {
+        const bool here = is_far();
+        if (here) mc = 0.f;
+        far_max = __any(here) != 0;
+      }
     }
+  };
+  auto less_far_max = [&](f32x16_v(&s)[KH]) __attribute__((always_inline)) {
+    if (CAP || !far_max) return;
+    const float m = is_far() ? m_run : 0.f;
+#pragma unroll
+    for (int e = 0; e < NS; ++e) s[e >> 4][e & 15] -= m;
   };
 
   // Tile i of the workgroup: its probabilities from s_cur while the next tile's products are formed (stage A), then its part of the output
@@ -611,6 +630,7 @@ void attn_ruled_kernel(const RuledParams p) {
     __builtin_amdgcn_s_waitcnt(0);  // this wavefront's tile loads have landed
     __syncthreads();
     settle_max(mx);
+    less_far_max(s_next);
     seen = seen_next;
     // (with biases, scores may lie so far below that all of a tile's probabilities are zero in 32 bits: nothing to add)
     live = seen_next && (BIAS == 0 || __any(!((mx - m_run) * c < -150.f)));
@@ -632,6 +652,7 @@ void attn_ruled_kernel(const RuledParams p) {
 #pragma unroll
       for (int i = 0; i < KH * KS; ++i) sa[i % KH] = M::run(__builtin_bit_cast(frag, k_at(lds, i)), q_at(i / KH), sa[i % KH]);
       settle_max(finish_scores(t0, all_see(t0), sa));
+      less_far_max(sa);
       live = seen;
     }
     __syncthreads();  // (the loop's first load goes where the first keys were)
@@ -690,7 +711,7 @@ void attn_ruled_kernel(const RuledParams p) {
         }
         if (mine) *reinterpret_cast<f32x4_v*>(po + (q0 - qb * BM + l32) * D + dt * 32 + g * 8 + hh * 4) = x;
       }
-    if (mine && hh == 0) *reinterpret_cast<float2*>(pml + (q0 - qb * BM + l32) * 2) = make_float2(m_run * c, l_tot);
+    if (mine && hh == 0) *reinterpret_cast<float2*>(pml + (q0 - qb * BM + l32) * 2) = make_float2(m_run, l_tot);
   } else {
     const float inv = 1.f / l_tot;
 #pragma unroll
@@ -739,12 +760,12 @@ void attn_ruled_kernel(const RuledParams p) {
         float bias = 0.f;
         if constexpr (BIAS == 1) bias = -slope * fabsf(static_cast<float>(key - at));
         if constexpr (BIAS == 2) bias = table[clampi(key - at, -p.radius, p.radius) + p.radius + kPad];
-        x = CAP ? p.cap(s) + bias : (s + bias) * p.scale_log2;
+        x = CAP ? p.cap(s) + bias : s + bias;
       }
       float mx = x;
       for (int sft = 1; sft < 64; sft <<= 1) mx = fmaxf(mx, __shfl_xor(mx, sft, 64));
       const float m_new = fmaxf(m, mx), m_safe = m_new == -INFINITY ? 0.f : m_new;
-      const float alpha = __builtin_amdgcn_exp2f(m - m_safe), w = __builtin_amdgcn_exp2f(x - m_safe);
+      const float alpha = __builtin_amdgcn_exp2f((m - m_safe) * c), w = __builtin_amdgcn_exp2f((x - m_safe) * c);
       m = m_new;
       l = l * alpha + group_sum<64>(w);
 #pragma unroll
@@ -786,7 +807,7 @@ __global__ __launch_bounds__(256) void attn_ruled_merge_kernel(const RuledParams
   float m = mc;
 #pragma unroll
   for (int s = 1; s < 64; s <<= 1) m = fmaxf(m, __shfl_xor(m, s, 64));
-  const float w = __builtin_amdgcn_exp2f(mc - (m == -INFINITY ? 0.f : m)), l = wave_sum(lane < p.chunks ? w * own.y : 0.f);
+  const float w = __builtin_amdgcn_exp2f((mc - (m == -INFINITY ? 0.f : m)) * p.unit), l = wave_sum(lane < p.chunks ? w * own.y : 0.f);
   float acc[EPL] = {};
   for (int c0 = 0; c0 < p.chunks; c0 += 8) {
     float x[8][EPL];
@@ -945,6 +966,7 @@ extern "C" int odit_attn_ruled(const void* q, const void* k, const void* v, void
   p.os_b = o_strides[0]; p.os_s = o_strides[1]; p.os_h = o_strides[2];
   p.scale_log2 = scale * kLog2e;
   p.bias_scale = 1.f / scale;
+  p.unit = r.cap > 0.f ? 1.f : p.scale_log2;
   // (without scratch, or with less than that takes, a query block's tiles stay in one piece and all are visited)
   RuledPlan plan = ruled_plan(B, Sq, Sk, H, D, r);
   if (workspace == nullptr || workspace_bytes < ruled_workspace_bytes(plan, B, Sq, H, D)) {

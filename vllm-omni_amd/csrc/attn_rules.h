@@ -39,6 +39,12 @@ inline Cap make_cap(float cap, float scale) {
   return c;
 }
 
+// A bias (or a slope) in the units that it is added in: a finite one stays finite, as the least float32 forbids a key beside others and no more
+__device__ __forceinline__ float in_units(float x, float unit) {
+  const float y = x * unit;
+  return fabsf(y) == INFINITY && fabsf(x) < INFINITY ? copysignf(3.402823466e38f, y) : y;
+}
+
 constexpr int kMaxRadius = 1024;  // distances with a bias of their own, either way
 
 }  // namespace odit
