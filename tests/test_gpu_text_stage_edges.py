@@ -3,8 +3,9 @@
 import pytest
 import torch
 
-from test_gpu_text_stage import BF16, F16, _randn, _ruled
+from test_gpu_text_stage import BF16, F16, _paged_problem, _randn, _ruled
 from text_stage import attention, seen_keys, within
+from vllm_omni_amd import kernels
 
 pytestmark = pytest.mark.gpu
 
@@ -77,3 +78,47 @@ def test_scores_of_any_size(gpu, size, D, rows, n, rules):
     tol = 2.0 ** -8 * 2.04 * (p @ v[:, 0].double().cpu().abs()) + 1e-30  # (a probability's rounding and the result's; scores are exact)
     for o in _ruled(q[None], k[None], v[None], 0.25, rules, {}, 0.0):
         within(o[0, :, 0], want, tol)
+
+
+def _single_and_joined(*args, **kw):
+    """The result of a call, and of one in a captured graph, whose chunks a second launch joins: the same bits."""
+    o = kernels.attn_paged(*args, **kw)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        other = kernels.attn_paged(*args, **kw)
+    graph.replay()
+    assert torch.equal(o.nan_to_num(7.0), other.nan_to_num(7.0))
+    return o
+
+
+@pytest.mark.parametrize("kind", ["least", "steep"])
+@pytest.mark.parametrize("cap", [0.0, 5.0])
+@pytest.mark.parametrize("D,dtype", [(64, F16), (128, BF16)])
+def test_decode_biases_of_any_size(gpu, kind, cap, D, dtype):
+    """The least float32 at all keys leaves their average, the steepest slopes the last key; also where the keys are cut into chunks."""
+    lengths = [1, 40, 300, 3000]
+    (q, kc, vc, table, n), rows = _paged_problem(20, lengths, 16, 4, 2, D, dtype)
+    for size in (-LEAST, 1e30, 1e10) if kind == "steep" else (LEAST, -1e30):
+        bias = dict(slopes=torch.full((4,), size, device="cuda:0")) if kind == "steep" else dict(distance=torch.full((4, 7), size, device="cuda:0"))
+        o = _single_and_joined(q, kc, vc, table, n, 0.125, cap=cap, **bias)
+        for b, (k, v) in enumerate(rows):
+            if kind == "steep":
+                assert torch.equal(o[b].cpu(), v[-1].repeat_interleave(2, dim=0))
+            else:
+                seen, away = seen_keys(1, len(k), causal=True)
+                want, tol = attention(torch.zeros_like(q[b:b + 1]), k, v, 0.125, seen, away)
+                within(o[b:b + 1], want, tol)
+
+
+@pytest.mark.parametrize("size", [1.0, 2.0 ** 20, 2.0 ** 40, 2.0 ** 60, 2.0 ** 100])
+@pytest.mark.parametrize("n", [100, 3000])
+@pytest.mark.parametrize("D", [64, 128])
+def test_decode_scores_of_any_size(gpu, size, n, D):
+    q, k = _large_scores(12, 1, n, D, size)
+    v, page = _randn(13, n, 1, D), 16
+    pages = -(-n // page)
+    kc, vc = (torch.cat([t, torch.zeros(pages * page - n, 1, D, dtype=BF16, device="cuda:0")]).view(pages, page, 1, D) for t in (k, v))
+    table = torch.arange(pages, dtype=torch.int32, device="cuda:0")[None]
+    o = _single_and_joined(q, kc, vc, table, torch.tensor([n], dtype=torch.int32, device="cuda:0"), 0.25)
+    p = torch.softmax((k[:, 0].double().cpu() @ q[0, 0].double().cpu()) * 0.25, dim=0)
+    within(o[0], (p @ v[:, 0].double().cpu())[None], 2.0 ** -8 * 2.04 * (p @ v[:, 0].double().cpu().abs())[None] + 1e-30)

@@ -50,11 +50,12 @@ struct PagedParams {
   Quotient by_page;
   int64_t qs_b, qs_h, kc_p, kc_r, kc_h, vc_p, vc_r, vc_h, ts, os_b, os_h;
   float scale_log2;
+  float unit;  // from what scores are kept in to units of log2: scale log2(e), or 1 where a cap or a bias has made them that
   Cap cap;
   int group, head_blocks, units;  // units: key heads' blocks of up to 16 query heads, of one sequence
   int wanted, room;               // chunks of all sequences, about, and the most keys of one
   bool whole;                     // no sequence has more than one
-  float* ws;  // per chunk and unit: [heads of a block][D] sums, then [heads of a block] (maximum, sum)
+  float* ws;  // per chunk and unit: [heads of a block][D] sums, then [heads of a block] (maximum in units of scores, sum)
   unsigned* tickets;  // a word for each sequence and unit, zero between launches (nullptr: the join is a launch of its own)
 };
 
@@ -209,10 +210,10 @@ __device__ __forceinline__ float2 get_pair(const float* at) {
   return make_float2(__uint_as_float(static_cast<uint32_t>(x)), __uint_as_float(static_cast<uint32_t>(x >> 32)));
 }
 
-// A sequence's chunks joined, features d and d + 1 of head hd: o = sum_c 2^(m_c - m) o_c / sum_c 2^(m_c - m) l_c, m = max_c m_c, in the chunks'
+// A sequence's chunks joined, features d and d + 1 of head hd: o = sum_c a_c o_c / sum_c a_c l_c with a_c = 2^((m_c - m) unit), m = max_c m_c, in the chunks'
 // order. kPagedJoin chunks' loads are on their way at once. part0: the first chunk's part, `step` floats ahead of the next one's.
 template <typename T, int D>
-__device__ __forceinline__ uint32_t join_parts(const float* part0, int64_t step, int most, int hd, int d, int parts) {
+__device__ __forceinline__ uint32_t join_parts(const float* part0, int64_t step, int most, int hd, int d, int parts, float unit) {
   float m = -INFINITY, l = 0.f, x0 = 0.f, x1 = 0.f;
   const uint32_t at_ml = most * D + 2 * hd, at_x = hd * D + d;
   for (int c0 = 0; c0 < parts; c0 += kPagedJoin) {
@@ -229,13 +230,13 @@ __device__ __forceinline__ uint32_t join_parts(const float* part0, int64_t step,
 #pragma unroll
     for (int c = 0; c < kPagedJoin; ++c)
       if (c0 + c < parts) m_new = fmaxf(m_new, ml[c].x);
-    const float m_safe = m_new == -INFINITY ? 0.f : m_new, a0 = __builtin_amdgcn_exp2f(m - m_safe);
+    const float m_safe = m_new == -INFINITY ? 0.f : m_new, a0 = __builtin_amdgcn_exp2f((m - m_safe) * unit);
     m = m_new;
     l *= a0; x0 *= a0; x1 *= a0;
 #pragma unroll
     for (int c = 0; c < kPagedJoin; ++c) {
       if (c0 + c < parts) {
-        const float a = __builtin_amdgcn_exp2f(ml[c].x - m_safe);
+        const float a = __builtin_amdgcn_exp2f((ml[c].x - m_safe) * unit);
         l = fmaf(a, ml[c].y, l);
         x0 = fmaf(a, x[c].x, x0);
         x1 = fmaf(a, x[c].y, x1);
@@ -283,9 +284,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 4
   frag qf[KS];
 #pragma unroll
   for (int st = 0; st < KS; ++st) qf[st] = __builtin_bit_cast(frag, *reinterpret_cast<const u32x4_v*>(qrow + g * 8 + st * 32));
-  const float slope = BIAS == 1 ? p.slopes[h] * kLog2e : 0.f;
+  const float slope = BIAS == 1 ? in_units(p.slopes[h], kLog2e) : 0.f;
   const float* const dist = BIAS == 2 ? p.distance + static_cast<int64_t>(h) * (2 * p.radius + 1) + p.radius : nullptr;  // [away]
-  const float far = BIAS == 2 ? dist[-p.radius] * kLog2e : 0.f;
+  const float far = BIAS == 2 ? in_units(dist[-p.radius], kLog2e) : 0.f;
   {
     const bool any = __any(bad);
     if (lane == 0) outside[wave] = any;
@@ -323,7 +324,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 4
   for (int dt = 0; dt < DT; ++dt) o[dt] = f32x4_v{0.f, 0.f, 0.f, 0.f};
   constexpr bool MADE = CAP || BIAS != 0;
   const float c = MADE ? 1.f : p.scale_log2;
-  float m_run = -INFINITY, l_run = 0.f, mc = 0.f;
+  float m_run = -INFINITY, l_run = 0.f, m_off = 0.f;  // m_off: m_run, or 0 while there is none
   const int k_lane = l16 * ROWB + (((g ^ (D == 128 ? l16 : l16 / 2)) % CPR) << 4);
   const int vkey = 4 * g + (l16 >> 2), vf = D == 128 ? 2 * (vkey % 8) : 2 * (vkey / 2 % 4);
   const int v_lane = vkey * ROWB + ((((l16 & 3) >> 1) ^ vf) << 4) + ((l16 & 1) << 3);
@@ -366,7 +367,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 4
       if constexpr (MADE) x = CAP ? p.cap(x) : x * p.scale_log2;
       if constexpr (BIAS == 1) x = fmaf(-slope, static_cast<float>(n - 1 - key), x);
       if constexpr (BIAS == 2) {
-        if (near) x = fmaf(dist[max(min(key, n - 1) - (n - 1), -p.radius)], kLog2e, x);
+        if (near) x += in_units(dist[max(min(key, n - 1) - (n - 1), -p.radius)], kLog2e);
         else x += far;
       }
       if (rest) x = counts(key) ? x : -INFINITY;
@@ -386,12 +387,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 4
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[dt][e] *= alpha;
       m_run = m_new;
-      mc = m_safe * c;
+      m_off = m_safe;
     }
-    u32x2_v pb;
+    u32x2_v pb;  // (differences first: with the maximum times c, rounded, in one fma, an exponent of zero comes out above 128 for scores past 2^31)
 #pragma unroll
     for (int e = 0; e < 4; e += 2) {
-      const float p0 = __builtin_amdgcn_exp2f(fmaf(s[e], c, -mc)), p1 = __builtin_amdgcn_exp2f(fmaf(s[e + 1], c, -mc));
+      const float p0 = __builtin_amdgcn_exp2f((s[e] - m_off) * c), p1 = __builtin_amdgcn_exp2f((s[e + 1] - m_off) * c);
       l_run += p0 + p1;
       pb[e / 2] = Mma<T>::pack2(p0, p1);
     }
@@ -402,7 +403,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 4
     }
   }
 
-  // ---- the wavefronts' sums joined: [wave][head][D + 4] sums and [wave][head] (maximum in units of log2, sum) ----
+  // ---- the wavefronts' sums joined: [wave][head][D + 4] sums and [wave][head] (maximum in units of scores, sum) ----
   constexpr int OP = D + 4;
   float* const jo = reinterpret_cast<float*>(lds);
   float2* const jm = reinterpret_cast<float2*>(lds + NW * 16 * OP * 4);
@@ -412,7 +413,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 4
   __syncthreads();
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4_v*>(jo + (wave * 16 + l16) * OP + dt * 16 + g * 4) = o[dt];
-  if (g == 0) jm[wave * 16 + l16] = make_float2(m_run * c, l_tot);
+  if (g == 0) jm[wave * 16 + l16] = make_float2(m_run, l_tot);
   __syncthreads();
   // what the call's chunks leave is written past the caches of this XCD, as another workgroup's may read it
   const int most = min(16, p.group);
@@ -427,7 +428,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 4
     float l = 0.f, x0 = 0.f, x1 = 0.f;
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
-      const float a = __builtin_amdgcn_exp2f(jm[w * 16 + hd].x - m_safe);
+      const float a = __builtin_amdgcn_exp2f((jm[w * 16 + hd].x - m_safe) * c);
       l = fmaf(a, jm[w * 16 + hd].y, l);
       x0 = fmaf(a, jo[(w * 16 + hd) * OP + d], x0);
       x1 = fmaf(a, jo[(w * 16 + hd) * OP + d + 1], x1);
@@ -454,7 +455,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 4
   if (!is_last) return;
   for (int i = tid; i < heads * (D / 2); i += NW * 64) {
     const int hd = i / (D / 2), d = i % (D / 2) * 2;
-    *reinterpret_cast<uint32_t*>(static_cast<T*>(p.o) + b * p.os_b + (h0 + hd) * p.os_h + d) = join_parts<T, D>(part0, step, most, hd, d, parts);
+    *reinterpret_cast<uint32_t*>(static_cast<T*>(p.o) + b * p.os_b + (h0 + hd) * p.os_h + d) = join_parts<T, D>(part0, step, most, hd, d, parts, p.unit);
   }
 }
 
@@ -467,7 +468,7 @@ __global__ __launch_bounds__(64) void attn_paged_join_kernel(const PagedParams p
   const int most = min(16, p.group), unit = h / p.group * p.head_blocks + h % p.group / 16, hd = h % p.group % 16;
   const int64_t step = static_cast<int64_t>(p.units) * most * (D + 2);
   *reinterpret_cast<uint32_t*>(static_cast<T*>(p.o) + b * p.os_b + h * p.os_h + d) =
-      join_parts<T, D>(p.ws + at.before * step + static_cast<int64_t>(unit) * most * (D + 2), step, most, hd, d, at.parts);
+      join_parts<T, D>(p.ws + at.before * step + static_cast<int64_t>(unit) * most * (D + 2), step, most, hd, d, at.parts, p.unit);
 }
 
 // The most chunks that any lengths can make, and what the kernels work them out from. Where a chunk's page numbers have to fit kPagedEntries
@@ -567,6 +568,7 @@ extern "C" int odit_attn_paged(const void* q, const void* key_cache, const void*
   p.kc_p = key_cache_strides[0]; p.kc_r = key_cache_strides[1]; p.kc_h = key_cache_strides[2];
   p.vc_p = value_cache_strides[0]; p.vc_r = value_cache_strides[1]; p.vc_h = value_cache_strides[2];
   p.scale_log2 = scale * kLog2e;
+  p.unit = r.cap > 0.f || r.slopes != nullptr || r.distance != nullptr ? 1.f : p.scale_log2;
   p.cap = make_cap(r.cap, scale);
   p.group = H / Hkv; p.head_blocks = paged_head_blocks(H, Hkv);
   p.units = Hkv * p.head_blocks;
