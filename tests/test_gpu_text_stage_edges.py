@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from test_gpu_text_stage import BF16, F16, _paged_problem, _randn, _ruled
+from test_gpu_text_stage import BF16, F16, _bias, _paged_problem, _randn, _ruled
 from text_stage import attention, seen_keys, within
 from vllm_omni_amd import kernels
 
@@ -122,3 +122,102 @@ def test_decode_scores_of_any_size(gpu, size, n, D):
     o = _single_and_joined(q, kc, vc, table, torch.tensor([n], dtype=torch.int32, device="cuda:0"), 0.25)
     p = torch.softmax((k[:, 0].double().cpu() @ q[0, 0].double().cpu()) * 0.25, dim=0)
     within(o[0], (p @ v[:, 0].double().cpu())[None], 2.0 ** -8 * 2.04 * (p @ v[:, 0].double().cpu().abs())[None] + 1e-30)
+
+
+# ------------------------------------------------------------------------------------------------ values that are not finite
+def _class_of(want, v, seen):
+    """The definition's result where some values are not finite: the kinds that a row sees decide. want [Sq,H,D] is of the others."""
+    Hkv, H = v.shape[1], want.shape[1]
+    v = v.double().cpu().repeat_interleave(H // Hkv, dim=1)
+    count = lambda what: torch.einsum("ij,jhd->ihd", seen.double(), what.double()) > 0  # noqa: E731
+    plus, minus, none = count(v == float("inf")), count(v == -float("inf")), count(v.isnan())
+    want = want.clone()
+    want[plus] = float("inf")
+    want[minus] = -float("inf")
+    want[none | (plus & minus)] = float("nan")
+    return want
+
+
+def _same(o, want, tol):
+    o = o.double().cpu()
+    for kind in (float("inf"), -float("inf")):
+        assert torch.equal(o == kind, want == kind)
+    assert torch.equal(o.isnan(), want.isnan())
+    finite = want.isfinite()
+    within(o[finite], want[finite], tol[finite])
+
+
+@pytest.mark.parametrize("rules", [
+    dict(causal=True), dict(window=40), dict(causal=True, window=70, prefix=[9]), dict(causal=True, q_starts=[0, 31, 32, 150, 200], k_starts=[0, 31, 32, 150, 200]),
+    dict(q_starts=[3, 60, 190], k_starts=[0, 57, 260], prefix=[2, 100], window=20)], ids=str)
+@pytest.mark.parametrize("cap,kind", [(0.0, ""), (3.0, ""), (0.0, "slopes"), (2.0, "table"), (0.0, "table")])
+@pytest.mark.parametrize("D,dtype", [(64, F16), (128, BF16)])
+def test_values_that_are_not_finite(gpu, rules, cap, kind, D, dtype):
+    """Each row and feature gets what the values it sees make of it: infinities of one sign, NaN of both, and nothing of those that it does not see."""
+    Sq, Sk = 200, 260 if "q_starts" in rules and rules["k_starts"][-1] == 260 else 200
+    q, k, v = _randn(30, 1, Sq, 2, D, dtype=dtype, std=0.5), _randn(31, 1, Sk, 1, D, dtype=dtype, std=0.5), _randn(32, 1, Sk, 1, D, dtype=dtype)
+    seen, away = seen_keys(Sq, Sk, **rules)
+    bias = dict(slopes=torch.tensor([0.01, 0.001], device="cuda:0")) if kind == "slopes" else _bias(kind, 2, 33)
+    want, tol = attention(q[0], k[0], v[0], 0.1, seen, away, cap, **bias)
+    for j, d, what in ((0, 0, "inf"), (5, 1, "nan"), (33, 1, "-inf"), (40, 2, "inf"), (90, 2, "-inf"), (64, D - 1, "nan"), (127, 3, "inf"), (128, 3, "inf"),
+                       (Sk - 1, 4, "-inf"), (150, slice(None), "nan"), (170, slice(8, 40), "inf")):
+        v[0, j, 0, d] = float(what)
+    clean = v.masked_fill(~v.isfinite(), 0.0)
+    want, tol = attention(q[0], k[0], clean[0], 0.1, seen, away, cap, **bias)
+    want = _class_of(want, v[0], seen)
+    for o in _ruled(q, k, v, 0.1, rules, bias, cap):
+        _same(o[0], want, tol)
+
+
+@pytest.mark.parametrize("Sq,Sk", [(3, 3000), (130, 2100)])
+@pytest.mark.parametrize("D,dtype", [(64, F16), (128, BF16)])
+def test_values_that_are_not_finite_in_cut_keys(gpu, Sq, Sk, D, dtype):
+    q, k, v = _randn(34, 1, Sq, 2, D, dtype=dtype, std=0.5), _randn(35, 1, Sk, 1, D, dtype=dtype, std=0.5), _randn(36, 1, Sk, 1, D, dtype=dtype)
+    for j, d, what in ((0, 0, "inf"), (700, 1, "nan"), (Sk - 1, 2, "inf"), (Sk - 2, 3, "nan"), (Sk - 3, 0, "-inf"), (1000, 4, "-inf")):
+        v[0, j, 0, d] = float(what)
+    seen, away = seen_keys(Sq, Sk, causal=True)
+    want, tol = attention(q[0], k[0], v[0].masked_fill(~v[0].isfinite(), 0.0), 0.1, seen, away)
+    want = _class_of(want, v[0], seen)
+    for o in _ruled(q, k, v, 0.1, dict(causal=True), {}, 0.0):
+        _same(o[0], want, tol)
+
+
+def _us(call):
+    call()
+    torch.cuda.synchronize()
+    a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    a.record()
+    call()
+    b.record()
+    torch.cuda.synchronize()
+    return a.elapsed_time(b) * 1e3
+
+
+@pytest.mark.parametrize("S,H,Hkv,D,dtype", [(2048, 4, 2, 128, BF16), (4096, 16, 4, 128, BF16), (4096, 16, 4, 64, F16)])
+def test_an_overflow_that_all_rows_see(gpu, S, H, Hkv, D, dtype):
+    """One infinite value at the head of a long prompt, and a feature that has overflowed at every key: right, and not far more work than a call is
+    anyhow (rows that see them are done again by wavefronts, if at all; the allowance is 20 times and a millisecond)."""
+    q, k, v = _randn(37, 1, S, H, D, dtype=dtype), _randn(38, 1, S, Hkv, D, dtype=dtype), _randn(39, 1, S, Hkv, D, dtype=dtype)
+    call = lambda: kernels.attn_ruled(q, k, v, 0.1, causal=True)  # noqa: E731
+    plain, time = call(), _us(call)
+    one, v = v, v.clone()
+    v[0, 3, 0, 5] = float("inf")
+    o = call()
+    group = H // Hkv
+    assert (o[0, 3:, :group, 5] == float("inf")).all()
+    o[0, 3:, :group, 5] = plain[0, 3:, :group, 5]
+    assert torch.equal(o[:, 64:], plain[:, 64:]) and torch.equal(o[:, :, group:], plain[:, :, group:])
+    seen, away = seen_keys(64, 64, causal=True)
+    want, tol = attention(q[0, :64], k[0, :64], one[0, :64], 0.1, seen, away)
+    within(o[0, :64], want, tol)
+    assert _us(call) < 20 * time + 1000
+    v = one.clone()
+    v[..., 5] = float("inf")
+    o = call()
+    assert (o[..., 5] == float("inf")).all()
+    rows = torch.tensor([0, 1, 31, 32, 63, 64, 1000, S - 1])
+    away = torch.arange(S)[None] - rows[:, None]
+    want, tol = attention(q[0, rows], k[0], one[0], 0.1, away <= 0, away)
+    keep = torch.arange(D) != 5
+    within(o[0, rows][..., keep.to("cuda:0")], want[..., keep], tol[..., keep])
+    assert _us(call) < 20 * time + 1000

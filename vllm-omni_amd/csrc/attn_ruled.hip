@@ -9,8 +9,11 @@
 // once, per lane; a tile's mask is then the two ranges' bits, formed only for tiles that some query sees in part. The tiles that a workgroup
 // visits are the union of its queries' ranges (two runs where a gap lies between).
 //
-// A value that is NaN or infinite spoils its tile's product also for queries that do not see its key (0 times it is NaN). Rows that come out
-// NaN with a finite sum are therefore done again at the end, over their own keys alone.
+// A value that is NaN or infinite spoils its tile's product also for queries that do not see its key (0 times it is NaN). Where a wavefront's rows come
+// out so with a finite sum, and there are such values in tiles that its queries see in part, its rows are therefore done again at the end, with
+// values and what is not finite among them apart.
+#include <type_traits>
+
 #include "attn_rules.h"
 #include "quotient.h"
 
@@ -93,6 +96,12 @@ __device__ __forceinline__ uint64_t range_bits(int lo, int hi, int t0) {
   const uint64_t upto = b == 64 ? ~0ull : (1ull << b) - 1;
   return upto & (~0ull << a);
 }
+
+// a value's bits: not finite (all of the exponent's bits are set)
+template <typename T> __device__ __forceinline__ bool not_finite(uint32_t v);
+template <> __device__ __forceinline__ bool not_finite<bf16_t>(uint32_t v) { return (v & 0x7f80u) == 0x7f80u; }
+template <> __device__ __forceinline__ bool not_finite<f16_t>(uint32_t v) { return (v & 0x7c00u) == 0x7c00u; }
+template <typename T> __device__ __forceinline__ bool is_nan(uint32_t v) { return not_finite<T>(v) && (v & (std::is_same<T, bf16_t>::value ? 0x7fu : 0x3ffu)) != 0; }
 
 constexpr int kTablePad = 63;  // a tile's keys but one
 // The keys' largest squared lengths, in kNormParts parts of each head's: a lane of the kernel below reads each. A workgroup has a part; D / 8 lanes a key.
@@ -696,95 +705,159 @@ void attn_ruled_kernel(const RuledParams p) {
   const int64_t part = (static_cast<int64_t>(unit) * p.n_qblocks + qb) * p.chunks + chunk;
   float* const po = p.ws + part * BM * D;
   float* const pml = p.ws + static_cast<int64_t>(p.units) * p.n_qblocks * p.chunks * BM * D + part * BM * 2;
-  float probe = 0.f;  // the largest in size; NaN once anything is
   T* const orow = static_cast<T*>(p.o) + b * p.os_b + h * p.os_h;
-  if (p.chunks > 1) {
+  // stores the rows of the lanes that have one; returns the largest value in size, NaN once anything is
+  auto store = [&](bool mine) __attribute__((always_inline)) {
+    float probe = 0.f;
+    if (p.chunks > 1) {
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
+      for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        f32x4_v x;
+        for (int g = 0; g < 4; ++g) {
+          f32x4_v x;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x[e] = l_tot == 0.f ? 0.f : o[dt][g * 4 + e];
-          if (e & 1) probe = __builtin_elementwise_maximum(__builtin_elementwise_maximum(probe, fabsf(x[e - 1])), fabsf(x[e]));
+          for (int e = 0; e < 4; ++e) {
+            x[e] = l_tot == 0.f ? 0.f : o[dt][g * 4 + e];
+            if (e & 1) probe = __builtin_elementwise_maximum(__builtin_elementwise_maximum(probe, fabsf(x[e - 1])), fabsf(x[e]));
+          }
+          if (mine) *reinterpret_cast<f32x4_v*>(po + (q0 - qb * BM + l32) * D + dt * 32 + g * 8 + hh * 4) = x;
         }
-        if (mine) *reinterpret_cast<f32x4_v*>(po + (q0 - qb * BM + l32) * D + dt * 32 + g * 8 + hh * 4) = x;
-      }
-    if (mine && hh == 0) *reinterpret_cast<float2*>(pml + (q0 - qb * BM + l32) * 2) = make_float2(m_run, l_tot);
-  } else {
-    const float inv = 1.f / l_tot;
+      if (mine && hh == 0) *reinterpret_cast<float2*>(pml + (q0 - qb * BM + l32) * 2) = make_float2(m_run, l_tot);
+    } else {
+      const float inv = 1.f / l_tot;
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
+      for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-      for (int g = 0; g < 4; g += 2) {
-        float x[8];
+        for (int g = 0; g < 4; g += 2) {
+          float x[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          x[e] = l_tot == 0.f ? 0.f : o[dt][g * 4 + e] * inv;
-          if (e & 1) probe = __builtin_elementwise_maximum(__builtin_elementwise_maximum(probe, fabsf(x[e - 1])), fabsf(x[e]));
+          for (int e = 0; e < 8; ++e) {
+            x[e] = l_tot == 0.f ? 0.f : o[dt][g * 4 + e] * inv;
+            if (e & 1) probe = __builtin_elementwise_maximum(__builtin_elementwise_maximum(probe, fabsf(x[e - 1])), fabsf(x[e]));
+          }
+          auto pair = [&](int e) __attribute__((always_inline)) {
+            return __builtin_amdgcn_permlane32_swap(M::pack2(x[e], x[e + 1]), M::pack2(x[e + 4], x[e + 5]), false, false);
+          };
+          const auto lo = pair(0), hi = pair(2);
+          u32x4_v w;
+          w.x = lo[0]; w.y = hi[0]; w.z = lo[1]; w.w = hi[1];
+          if (mine) *reinterpret_cast<u32x4_v*>(orow + row * p.os_s + dt * 32 + g * 8 + hh * 8) = w;
         }
-        auto pair = [&](int e) __attribute__((always_inline)) {
-          return __builtin_amdgcn_permlane32_swap(M::pack2(x[e], x[e + 1]), M::pack2(x[e + 4], x[e + 5]), false, false);
-        };
-        const auto lo = pair(0), hi = pair(2);
-        u32x4_v w;
-        w.x = lo[0]; w.y = hi[0]; w.z = lo[1]; w.w = hi[1];
-        if (mine) *reinterpret_cast<u32x4_v*>(orow + row * p.os_s + dt * 32 + g * 8 + hh * 8) = w;
-      }
-  }
-  // rows to be done again: finite sums, but values that are not. (l_tot == 0: nothing was seen, zeros are right)
+    }
+    return probe;
+  };
+  const float probe = store(mine);
+  // rows with finite sums, but values that are not. (l_tot == 0: nothing was seen, zeros are right)
   uint64_t bad = __ballot(mine && l_tot > 0.f && l_tot < INFINITY && !(probe < INFINITY));
   bad = (bad | (bad >> 32)) & 0xffffffffull;
-  while (bad != 0) {  // (wave-uniform)
-    const int who = __builtin_ctzll(bad);
-    bad &= bad - 1;
-    const int r = q0 + who, at = BIAS != 0 ? places[wave * 32 + who] : 0;
-    const int4 its = ranges[wave * 32 + who];
-    const T* const qp = static_cast<const T*>(p.q) + b * p.qs_b + h * p.qs_h + r * p.qs_s;
-    float m = -INFINITY, l = 0.f, acc[D / 64] = {};
-    for (int i = 0; i < n_tiles; ++i) {
-      const int t0 = tile_at(i) * BN, key = t0 + lane;
-      const bool sees = (key >= its.x && key < its.y) || (key >= its.z && key < its.w);
-      const uint64_t some = __ballot(sees);
-      if (some == 0) continue;
-      float x = -INFINITY;
-      if (sees) {
-        const T* const kp = kbase + key * p.ks_s;
-        float s = 0.f;
-        for (int d = 0; d < D; d += 8) {
-          const u32x4 qv = load_raw(qp + d), kv = load_raw(kp + d);
+  if (__builtin_expect(bad == 0, 1)) return;
+  int again = lane;
+  asm volatile("" : "+v"(again));  // (what follows from the lane is formed here, not held across the loop)
+  const int r32 = again & 31, rh = again >> 5;
+  const int4 its = ranges[wave * 32 + r32];
+  const auto see_some = [&](int k0, int n) { return __any((k0 < its.y && k0 + n > its.x) || (k0 < its.w && k0 + n > its.z)) != 0; };
+  const auto see_all = [&](int k0, int n) { return __all((k0 >= its.x && k0 + n <= its.y) || (k0 >= its.z && k0 + n <= its.w)) != 0; };
+  // Whether a value that is not finite lies in what was multiplied by a zero for some row: in keys of one product that not all rows see. Elsewhere
+  // such values are seen, and the rows are right as they are.
+  bool spoiled = false;
+  for (int i = 0; i < n_tiles && !spoiled; ++i)
+    for (int k0 = tile_at(i) * BN, n = 0; n < BN && !spoiled; n += WN, k0 += WN) {
+      if (!see_some(k0, WN) || see_all(k0, WN)) continue;
+      bool found = false;
+      for (int r = again / CPR; r < WN; r += RPI) {
+        const u32x4 x = load_raw(vbase + min(k0 + r, p.Sk - 1) * p.vs_s + again % CPR * 8);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) s = fmaf(Raw<T>::get(qv, e), Raw<T>::get(kv, e), s);
+        for (int e = 0; e < 4; ++e) found |= not_finite<T>(x[e]) || not_finite<T>(x[e] >> 16);
+      }
+      spoiled = __any(found) != 0;
+    }
+  if (!spoiled) return;
+  // The rows of the wavefront again, 32 keys at a time, straight from memory. A product takes the values that are finite, zeros for the others; where there
+  // are others, a second product counts for each feature and row those that the row sees, by kind (1, 64 and 4096 each, of 16 keys: its sum
+  // says how many of which), and they are added as what they are. us, 4096 causal tokens, 16 heads of 128 on 4: all finite 91, one infinite value at the
+  // head, which all rows see, 115, one NaN in the middle 250, a feature that is infinite at every key 846 (row by row, any of them took 20000).
+  l_run = 0.f;
+  m_run = -INFINITY;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[dt][e] = 0.f;
+  const int at = BIAS != 0 ? places[wave * 32 + r32] : 0;
+  const T* const qp = static_cast<const T*>(p.q) + b * p.qs_b + h * p.qs_h + min(q0 + r32, p.Sq - 1) * p.qs_s + rh * 8;
+  for (int i = 0; i < 2 * n_tiles; ++i) {
+    const int t0 = tile_at(i >> 1) * BN, k0 = t0 + (i & 1) * 32;
+    if (!see_some(k0, 32)) continue;
+    f32x16_v x;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) x[e] = 0.f;
+    const T* const kp = kbase + min(k0 + r32, p.Sk - 1) * p.ks_s + rh * 8;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {  // (the queries from memory too: their registers are needed here)
+      x = M::run(__builtin_bit_cast(frag, *reinterpret_cast<const u32x4_v*>(kp + ks * 16)), __builtin_bit_cast(frag, *reinterpret_cast<const u32x4_v*>(qp + ks * 16)), x);
+    }
+    const uint32_t sees = static_cast<uint32_t>((range_bits(its.x, its.y, t0) | range_bits(its.z, its.w, t0)) >> (32 * (i & 1))) >> (4 * rh);
+    float mx = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int away = k0 + key_of(e) + 4 * rh - at;
+      float bias = 0.f;
+      if constexpr (BIAS == 1) bias = -slope * fabsf(static_cast<float>(away));
+      if constexpr (BIAS == 2) bias = table[clampi(away, -p.radius, p.radius) + p.radius + kPad];
+      x[e] = (sees >> key_of(e)) & 1 ? (CAP ? p.cap(x[e]) : x[e]) + bias : -INFINITY;
+      mx = fmaxf(mx, x[e]);
+    }
+    const float m_new = fmaxf(m_run, fmaxf(mx, swapped(mx))), m_safe = m_new == -INFINITY ? 0.f : m_new;
+    const float alpha = __builtin_amdgcn_exp2f((m_run - m_safe) * c);
+    m_run = m_new;
+    l_run *= alpha;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[dt][e] = fabsf(o[dt][e]) < INFINITY ? o[dt][e] * alpha : o[dt][e];
+    u32x4_v weights[2], ones[2];
+#pragma unroll
+    for (int e = 0; e < 16; e += 2) {
+      const float p0 = __builtin_amdgcn_exp2f((x[e] - m_safe) * c), p1 = __builtin_amdgcn_exp2f((x[e + 1] - m_safe) * c);
+      l_run += p0 + p1;
+      weights[e >> 3][(e & 7) >> 1] = M::pack2(p0, p1);
+      ones[e >> 3][(e & 7) >> 1] = M::pack2((sees >> key_of(e)) & 1 ? 1.f : 0.f, (sees >> key_of(e + 1)) & 1 ? 1.f : 0.f);
+    }
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        uint32_t v[8];
+        bool others = false;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int key = min(k0 + g * 16 + (j >> 2) * 8 + 4 * rh + (j & 3), p.Sk - 1);
+          v[j] = *reinterpret_cast<const uint16_t*>(vbase + key * p.vs_s + dt * 32 + r32);
+          others |= not_finite<T>(v[j]);
         }
-        float bias = 0.f;
-        if constexpr (BIAS == 1) bias = -slope * fabsf(static_cast<float>(key - at));
-        if constexpr (BIAS == 2) bias = table[clampi(key - at, -p.radius, p.radius) + p.radius + kPad];
-        x = CAP ? p.cap(s) + bias : s + bias;
+        u32x4_v clean;
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) clean[j >> 1] = (not_finite<T>(v[j]) ? 0u : v[j]) | (not_finite<T>(v[j + 1]) ? 0u : v[j + 1] << 16);
+        o[dt] = M::run(__builtin_bit_cast(frag, clean), __builtin_bit_cast(frag, weights[g]), o[dt]);
+        if (!__any(others)) continue;
+        const auto kind = [](uint32_t u) { return !not_finite<T>(u) ? 0.f : is_nan<T>(u) ? 4096.f : (u & 0x8000u) ? 64.f : 1.f; };
+        u32x4_v kinds;
+        f32x16_v found;
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) kinds[j >> 1] = M::pack2(kind(v[j]), kind(v[j + 1]));
+#pragma unroll
+        for (int e = 0; e < 16; ++e) found[e] = 0.f;
+        found = M::run(__builtin_bit_cast(frag, kinds), __builtin_bit_cast(frag, ones[g]), found);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int n = static_cast<int>(found[e]);
+          if (n >= 4096) o[dt][e] = NAN;
+          if (n & 63) o[dt][e] += INFINITY;
+          if (n & 4032) o[dt][e] -= INFINITY;
+        }
       }
-      float mx = x;
-      for (int sft = 1; sft < 64; sft <<= 1) mx = fmaxf(mx, __shfl_xor(mx, sft, 64));
-      const float m_new = fmaxf(m, mx), m_safe = m_new == -INFINITY ? 0.f : m_new;
-      const float alpha = __builtin_amdgcn_exp2f((m - m_safe) * c), w = __builtin_amdgcn_exp2f((x - m_safe) * c);
-      m = m_new;
-      l = l * alpha + group_sum<64>(w);
-#pragma unroll
-      for (int e = 0; e < D / 64; ++e) acc[e] *= alpha;
-      for (int u = 0; u < 64; ++u) {
-        if (!((some >> u) & 1)) continue;
-        const float pw = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), u));
-        const T* const vp = vbase + (t0 + u) * p.vs_s + lane * (D / 64);
-#pragma unroll
-        for (int e = 0; e < D / 64; ++e) acc[e] = fmaf(pw, to_float(vp[e]), acc[e]);
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < D / 64; ++e) {
-      if (p.chunks > 1) po[(q0 - qb * BM + who) * D + lane * (D / 64) + e] = acc[e];
-      else (orow + r * p.os_s)[lane * (D / 64) + e] = from_float<T>(acc[e] / l);
-    }
-    if (p.chunks > 1 && lane == 0) *reinterpret_cast<float2*>(pml + (q0 - qb * BM + who) * 2) = make_float2(m, l);
   }
+  l_tot = l_run + swapped(l_run);
+  store(mine && ((bad >> l32) & 1) != 0);
 }
 
 // Joins the chunks' sums, a wavefront for each row: o = sum_c 2^(m_c - m) o_c / sum_c 2^(m_c - m) l_c, m = max_c m_c. Lane c has chunk c's
