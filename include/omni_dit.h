@@ -100,7 +100,9 @@ typedef struct odit_attn_rules {
  * not see (NaN and infinities too) does not reach it.
  * `workspace`: NULL, or odit_attn_ruled_workspace_bytes for the same shape and rules (may be 0; no device memory is read for it), contents
  * irrelevant before and after: few rows' long keys are then cut into ranges that run side by side and are joined by a second launch, and
- * with slopes far keys whose probabilities are zero in 32 bits are left out, by a bound that a first launch takes from all keys. */
+ * with slopes far keys whose probabilities are zero in 32 bits are left out, by a bound that a first launch takes from all keys. With slopes or
+ * a table, the value of a key whose probability is zero in 32 bits may be left out whatever it holds (a product with zero would make NaN of an
+ * infinity); a key that is seen and holds NaN is not, however far it is. */
 int odit_attn_ruled(const void* q, const void* k, const void* v, void* o, int B, int Sq, int Sk, int H, int Hkv, int D,
                     const int64_t q_strides[3], const int64_t k_strides[3], const int64_t v_strides[3], const int64_t o_strides[3],
                     float scale, const odit_attn_rules* rules, int dtype, void* workspace, size_t workspace_bytes, void* stream);

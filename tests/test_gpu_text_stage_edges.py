@@ -1,11 +1,13 @@
 """A text stage's operators at the edges of their numbers."""
 
+import ctypes
+
 import pytest
 import torch
 
-from test_gpu_text_stage import BF16, F16, _bias, _paged_problem, _randn, _ruled
+from test_gpu_text_stage import BF16, F16, _all_tiles, _bias, _paged_problem, _randn, _ruled
 from text_stage import attention, seen_keys, within
-from vllm_omni_amd import kernels
+from vllm_omni_amd import _lib, kernels
 
 pytestmark = pytest.mark.gpu
 
@@ -180,6 +182,37 @@ def test_values_that_are_not_finite_in_cut_keys(gpu, Sq, Sk, D, dtype):
     want = _class_of(want, v[0], seen)
     for o in _ruled(q, k, v, 0.1, dict(causal=True), {}, 0.0):
         _same(o[0], want, tol)
+
+
+@pytest.mark.parametrize("Sq,Sk,causal", [(6200, 6200, True), (6144, 6144, False), (1030, 6145, True), (100, 300, True)])
+@pytest.mark.parametrize("D,dtype,H,Hkv", [(128, BF16, 8, 4), (64, F16, 40, 40)])
+def test_keys_that_are_no_numbers_reach_rows_behind_slopes_and_a_cap(gpu, Sq, Sk, causal, D, dtype, H, Hkv):
+    """However far they are; a key with infinities counts by the cap. The call without scratch visits all tiles."""
+    q, k, v = _randn(40, 1, Sq, H, D, dtype=dtype), _randn(41, 1, Sk, Hkv, D, dtype=dtype), _randn(42, 1, Sk, Hkv, D, dtype=dtype)
+    slopes = torch.tensor([4.0 * 2.0 ** (-12.0 * h / H) for h in range(H)], device="cuda:0")
+    group, clean = H // Hkv, kernels.attn_ruled(q, k, v, D ** -0.5, causal=causal, slopes=slopes, cap=5.0)
+    # (keys that are cut into ranges are summed in another order than those of a call without scratch)
+    whole = _lib.load().odit_attn_ruled_workspace_bytes(1, Sq, Sk, H, D, ctypes.byref(_lib.AttnRules(causal=int(causal), cap=5.0))) == 0
+    for what in (float("nan"), float("inf"), 1e30 if dtype == BF16 else 60000.0):
+        bad = k.clone()
+        bad[0, 3, 0, :7] = what
+        o = kernels.attn_ruled(q, bad, v, D ** -0.5, causal=causal, slopes=slopes, cap=5.0)
+        full = _all_tiles(q, bad, v, D ** -0.5, causal, None, 5.0, slopes)
+        assert torch.equal(o.isnan(), full.isnan())
+        assert torch.equal(o[:, :, group:], clean[:, :, group:])
+        sees = torch.arange(Sq, device="cuda:0") + Sk - Sq >= (3 if causal else 0)
+        if what != what:
+            assert o[0, sees, :group].isnan().all() and not o[0, ~sees].isnan().any()
+        if causal and whole:
+            assert torch.equal(o.nan_to_num(77.0), full.nan_to_num(77.0))
+    q[0, 70, 0, 0] = float("nan")  # (and a query that is none spoils its own row)
+    o = kernels.attn_ruled(q, k, v, D ** -0.5, causal=causal, slopes=slopes, cap=5.0)
+    assert o[0, 70, 0].isnan().all()
+    o[0, 70, 0] = clean[0, 70, 0]
+    if causal and whole:
+        assert torch.equal(o, clean)
+    else:
+        assert o.isfinite().all()
 
 
 def _us(call):

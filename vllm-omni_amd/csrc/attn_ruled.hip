@@ -39,8 +39,7 @@ struct RuledParams {
   Quotient by_blocks, by_units, by_heads, by_group;  // by n_qblocks * units, by the units of a row of blocks (of an XCD), by H, by group
   int bm;                // queries of a block
   int chunks;            // workgroups that share a query block's tiles; with more than one, their sums go to ws
-  bool cut;              // slopes: far tiles are left out whose probabilities are zero
-  const float* norms;    // [B][Hkv][kNormParts]: the largest squared length of a part's keys (with a cap: nullptr, not needed)
+  const float* norms;    // [B][Hkv][kNormParts]: the largest squared length of a part's keys, by which far tiles are left out (nullptr: none is)
   float* ws;             // [units][n_qblocks][chunks][bm][D] sums, then [...][bm] (maximum in units of scores, sum)
 };
 
@@ -302,36 +301,34 @@ void attn_ruled_kernel(const RuledParams p) {
     s2 = __builtin_amdgcn_readfirstlane(c0); n2 = __builtin_amdgcn_readfirstlane(c1 - c0);
   }
   if constexpr (BIAS == 1) {
-    // Slopes: no product exceeds |q| |k| in size (or the cap), a query's own key has no bias, so its maximum is at least -|q| |k|, and a key
+    // Slopes: no score exceeds |q| |k| in size, nor the cap, a query's own key has no bias, so its maximum is at least the negative of that, and a key
     // `reach` away has a probability of 2^-160 at most beside it, which is zero in 32 bits (2^-8 of that is what the running maximum may lag). Tiles
     // farther off than that from all queries are left out: of 16384 causal tokens, 16 heads with slopes of 2^-1/2 to 2^-8, more than half.
     const float steep = p.slopes[h] * kLog2e;
-    if (p.cut && steep > 0.f) {
-      float most = p.cap.out;
-      if constexpr (!CAP) {
-        float q2 = 0.f;
+    if (p.norms != nullptr && steep > 0.f) {
+      float q2 = 0.f;
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          const u32x4 x = __builtin_bit_cast(u32x4, qf[ks]);
+      for (int ks = 0; ks < KS; ++ks) {
+        const u32x4 x = __builtin_bit_cast(u32x4, qf[ks]);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) q2 = fmaf(Raw<T>::get(x, e), Raw<T>::get(x, e), q2);
-        }
-        q2 += __shfl_xor(q2, 32, 64);
-        float k2 = p.norms[(static_cast<int64_t>(b) * p.Hkv + hkv) * kNormParts + lane];
-#pragma unroll
-        for (int sft = 1; sft < 64; sft <<= 1) {  // (NaN stays NaN)
-          q2 = __builtin_elementwise_maximum(q2, __shfl_xor(q2, sft, 64));
-          k2 = __builtin_elementwise_maximum(k2, __shfl_xor(k2, sft, 64));
-        }
-        __shared__ float lengths[NW];
-        if (lane == 0) lengths[wave] = q2;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < NW; ++w) q2 = __builtin_elementwise_maximum(q2, lengths[w]);
-        most = p.scale_log2 * sqrtf(q2) * sqrtf(k2) * 1.001f;
+        for (int e = 0; e < 8; ++e) q2 = fmaf(Raw<T>::get(x, e), Raw<T>::get(x, e), q2);
       }
+      q2 += __shfl_xor(q2, 32, 64);
+      float k2 = p.norms[(static_cast<int64_t>(b) * p.Hkv + hkv) * kNormParts + lane];
+#pragma unroll
+      for (int sft = 1; sft < 64; sft <<= 1) {  // (NaN stays NaN)
+        q2 = __builtin_elementwise_maximum(q2, __shfl_xor(q2, sft, 64));
+        k2 = __builtin_elementwise_maximum(k2, __shfl_xor(k2, sft, 64));
+      }
+      __shared__ float lengths[NW];
+      if (lane == 0) lengths[wave] = q2;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < NW; ++w) q2 = __builtin_elementwise_maximum(q2, lengths[w]);
+      const float product = p.scale_log2 * sqrtf(q2) * sqrtf(k2) * 1.001f, most = CAP ? fminf(product, p.cap.out) : product;
       const float reach = (2.f * most + 160.f) / steep * 1.001f + 1.f;
-      const int far = __builtin_amdgcn_readfirstlane(reach < 1e9f ? static_cast<int>(reach) + 1 : -1);  // (-1 for NaN and infinities too)
+      // (-1: nothing is left out. NaN and infinities in queries or keys, behind a cap too: a score may then be NaN however far its key is)
+      const int far = __builtin_amdgcn_readfirstlane(product < INFINITY && reach < 1e9f ? static_cast<int>(reach) + 1 : -1);
       if (far >= 0) {
         const int row0 = qb * BM + p.Sk - p.Sq, row1 = min(qb * BM + BM, p.Sq) - 1 + p.Sk - p.Sq;
         const int from = max(row0 - far, 0) / BN, to = (row1 + far) / BN + 1;
@@ -913,17 +910,17 @@ __global__ __launch_bounds__(256) void attn_ruled_merge_kernel(const RuledParams
 //               S=1500 H=64 causal [768] 29.5 / 26.6    10 in S=4000 H=48 causal [1536] 46.0 / 47.6    23 in S=12007 H=32 causal [3008] 100 / 107
 // Where a call still has fewer workgroups than the GPU has room for, its tiles are cut into chunks, as many as cost least: the join is a launch
 // of 3 us and its sums' way to memory and back, 8 bytes a feature.
-// With slopes and no cap, a launch that reads all keys once gives the bound that far tiles are left out by. us, without / with it, causal, slopes from
-// 2^(-8/H) to 2^-8: 4 prompts of 2048, 16 heads of 128, 84 / 93; 4096, 24 of 64, 87 / 88; 6144, 32 of 128, 271 / 232; 8192, 32 on 8, 437 / 352; 16384, 16,
-// 860 / 645. A cap is a bound by itself: 16384, 16 heads, a cap of 30, 1255 / 775.
-struct RuledPlan { int halves, chunks; bool cut, norms; };
+// With slopes, a launch that reads all keys once gives the bound that far tiles are left out by (behind a cap too, which bounds scores by itself but does
+// not say whether keys are numbers). us, without / with it, causal, slopes from 2^(-8/H) to 2^-8, and the same with a cap of 30: 2048 tokens, 24 heads of
+// 128, 46.7 / 51.3, 53.4 / 57.0; 4096, 24, 116 / 116, 139 / 139; 4096, 16 of 64, 64.4 / 67.3, 81.5 / 84.2; 6144, 32 on 8 of 128, 260 / 217, 348 / 271;
+// 8192, 32 on 8, 436 / 339, 579 / 427; 16384, 16, 796 / 571, 1064 / 735.
+struct RuledPlan { int halves, chunks; bool norms; };
 static RuledPlan ruled_plan(int B, int Sq, int Sk, int H, int D, const odit_attn_rules& r) {
   const int docs = r.docs, window = r.window, causal = r.causal;
   const auto blocks = [&](int bm) { return static_cast<int64_t>((Sq + bm - 1) / bm) * H * B; };
   const int64_t few = docs > 0 ? (D == 128 ? 256 : 768) : causal ? 512 : 128;
-  RuledPlan plan{blocks(128) <= few ? 1 : 2, 1, r.slopes != nullptr && docs == 0 && Sk >= Sq, false};  // (cut: every query has a key at its own place)
-  plan.norms = plan.cut && r.cap == 0.f && Sq >= 1024 && Sk >= 6144;
-  plan.cut = plan.norms || (plan.cut && r.cap > 0.f);
+  // (slopes, and every query has a key at its own place)
+  RuledPlan plan{blocks(128) <= few ? 1 : 2, 1, r.slopes != nullptr && docs == 0 && Sk >= Sq && Sq >= 1024 && Sk >= 6144};
   const int64_t mine = blocks(64 * plan.halves), room = D == 128 ? 512 : 768;  // (1024 at halves of 64 features: 500 rows of 3000 keys 31.1 us, so 29.7)
   int64_t keys = docs > 0 ? 2 * (Sk / docs) + 64 : Sk;  // that a query block may see, about
   if (window > 0) {
@@ -1044,11 +1041,9 @@ extern "C" int odit_attn_ruled(const void* q, const void* k, const void* v, void
   RuledPlan plan = ruled_plan(B, Sq, Sk, H, D, r);
   if (workspace == nullptr || workspace_bytes < ruled_workspace_bytes(plan, B, Sq, H, D)) {
     plan.chunks = 1;
-    plan.cut = plan.cut && !plan.norms;
     plan.norms = false;
   }
   p.chunks = plan.chunks;
-  p.cut = plan.cut;
   p.norms = plan.norms ? static_cast<float*>(workspace) : nullptr;
   p.ws = static_cast<float*>(workspace) + ruled_norms_bytes(plan, B, H) / sizeof(float);
   p.cap = make_cap(r.cap, scale);

@@ -383,8 +383,8 @@ def attn_ruled(
     [N + 1], rising, on the GPU; every batch row is cut alike). A document's last query is at the place of its last key. ``causal`` hides the keys
     behind the query, ``window`` those with ``|away| >= window``; the first ``prefix[n]`` keys of document n (int32 [N], or [B] without
     documents) are seen in any case. A query that sees nothing, or is of no document, gets zeros; NaN and infinities in keys and values that
-    a query does not see do not reach it. (With slopes, a key so far away that its probability is zero in 32 bits may be left out.) Inference
-    only."""
+    a query does not see do not reach it. (With slopes or a table, the value of a key whose probability is zero in 32 bits may be left out,
+    whatever it holds.) Inference only."""
     out = (_nat or _load_native()).attn_ruled(q, k, v, scale, causal, window, prefix, q_starts, k_starts, cap, slopes, distance)
     if out is not None:
         return out
