@@ -913,14 +913,16 @@ __global__ __launch_bounds__(256) void attn_ruled_merge_kernel(const RuledParams
 // With slopes, a launch that reads all keys once gives the bound that far tiles are left out by (behind a cap too, which bounds scores by itself but does
 // not say whether keys are numbers). us, without / with it, causal, slopes from 2^(-8/H) to 2^-8, and the same with a cap of 30: 2048 tokens, 24 heads of
 // 128, 46.7 / 51.3, 53.4 / 57.0; 4096, 24, 116 / 116, 139 / 139; 4096, 16 of 64, 64.4 / 67.3, 81.5 / 84.2; 6144, 32 on 8 of 128, 260 / 217, 348 / 271;
-// 8192, 32 on 8, 436 / 339, 579 / 427; 16384, 16, 796 / 571, 1064 / 735.
+// 8192, 32 on 8, 436 / 339, 579 / 427; 16384, 16, 796 / 571, 1064 / 735. In a window, which leaves far tiles out by itself: 8192, 32 on 8, windows of 512,
+// 1024, 2048 and 4096, 103 / 111, 150 / 149, 230 / 209, 352 / 285; 16384, 16, windows of 2048 and 4096, 260 / 275, 414 / 358; 8192 of 64 features, 16, both ways,
+// 2048 and 4096, 162 / 167, 259 / 222.
 struct RuledPlan { int halves, chunks; bool norms; };
 static RuledPlan ruled_plan(int B, int Sq, int Sk, int H, int D, const odit_attn_rules& r) {
   const int docs = r.docs, window = r.window, causal = r.causal;
   const auto blocks = [&](int bm) { return static_cast<int64_t>((Sq + bm - 1) / bm) * H * B; };
   const int64_t few = docs > 0 ? (D == 128 ? 256 : 768) : causal ? 512 : 128;
   // (slopes, and every query has a key at its own place)
-  RuledPlan plan{blocks(128) <= few ? 1 : 2, 1, r.slopes != nullptr && docs == 0 && Sk >= Sq && Sq >= 1024 && Sk >= 6144};
+  RuledPlan plan{blocks(128) <= few ? 1 : 2, 1, r.slopes != nullptr && docs == 0 && Sk >= Sq && Sq >= 1024 && Sk >= 6144 && (window == 0 || window >= Sk / 4)};
   const int64_t mine = blocks(64 * plan.halves), room = D == 128 ? 512 : 768;  // (1024 at halves of 64 features: 500 rows of 3000 keys 31.1 us, so 29.7)
   int64_t keys = docs > 0 ? 2 * (Sk / docs) + 64 : Sk;  // that a query block may see, about
   if (window > 0) {
