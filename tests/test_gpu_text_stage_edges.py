@@ -254,3 +254,50 @@ def test_an_overflow_that_all_rows_see(gpu, S, H, Hkv, D, dtype):
     keep = torch.arange(D) != 5
     within(o[0, rows][..., keep.to("cuda:0")], want[..., keep], tol[..., keep])
     assert _us(call) < 20 * time + 1000
+
+
+# ------------------------------------------------------------------------------------------------ caps
+def _pairs(seed, n, D, step):
+    """Queries and pairs of keys whose products are exact in 32 bits, the two of a pair's up to 4 `step` apart."""
+    g = torch.Generator().manual_seed(seed)
+    q = torch.randint(-4, 5, (n, 1, D), generator=g).float()
+    k = torch.randint(-2, 3, (n, 1, D), generator=g).float() + q.sign() * torch.randint(0, 2, (n, 1, 1), generator=g)
+    other = k.clone()
+    other[:, :, 0] += step * torch.randint(-1, 2, (n, 1), generator=g)
+    return q.half(), torch.stack([k, other], dim=1).half()
+
+
+def _capped_pair(q, k, scale, cap, bias):
+    """(o, tolerance) of values 1 and -1. The larger probability is 1; the other one's rounding (below 1: 2^-12) and the result's (below 1/2, 2^-13, or
+    below 1, 2^-12) are halved by the sum; a score's own error is 2^-21 of it, and six roundings of what is added in 32 bits."""
+    s = (q.double()[:, None] * k.double()).sum(dim=-1)[..., 0] * scale
+    s = cap * torch.tanh(s / cap) + bias
+    p = torch.softmax(s, dim=1)
+    o = p[:, 0] - p[:, 1]
+    assert (p.min(dim=1).values > 0.05).all()
+    return o, 2.0 ** -13 + 2.0 ** -12 * o.abs().clamp_min(0.5) + 2.0 ** -21 * s.abs().amax(dim=1) + 6.0 * 2.0 ** -24 * s.abs().amax(dim=1)
+
+
+@pytest.mark.parametrize("kind", ["", "slopes", "table"])
+@pytest.mark.parametrize("cap", [30.0, 512.0, 513.0, 1000.0, 3000.0, 8192.0])
+@pytest.mark.parametrize("scale,step", [(0.125, 1.0), (4.0, 2.0 ** -5)])  # scores of tens, and up to a thousand
+@pytest.mark.parametrize("D", [64, 128])
+def test_scores_keep_their_digits_under_any_cap(gpu, cap, kind, scale, step, D):
+    """In fp16, whose probabilities tell scores apart that differ by 2^-11: whole prompts of two keys, and sequences of two."""
+    n = 3000
+    q, k = (t.to("cuda:0") for t in _pairs(50, n, D, step))
+    v = torch.ones_like(k)
+    v[:, 1] = -1.0
+    slope = 0.25
+    kw = dict(slopes=torch.full((1,), slope, device="cuda:0")) if kind == "slopes" else dict(distance=torch.full((1, 3), -slope, device="cuda:0")) if kind == "table" else {}
+    # away: the query stands at the second key
+    bias = torch.tensor([-slope, 0.0] if kind == "slopes" else [-slope, -slope] if kind else [0.0, 0.0], dtype=torch.float64)
+    want, tol = _capped_pair(q.cpu(), k.cpu(), scale, cap, bias)
+    if cap <= 512.0:
+        tol = tol + 2.0 * cap * 2.0 ** -21 / 2.0  # (both scores' errors, of the cap, of which half is the result's)
+    for o in (kernels.attn_ruled(q[:, None], k, v, scale, cap=cap, **kw)[:, 0],
+              kernels.attn_ruled(q[:, None].expand(n, 70, 1, D), k, v, scale, cap=cap, **kw)[:, -1],
+              kernels.attn_paged(q, k, v, torch.arange(n, dtype=torch.int32, device="cuda:0")[:, None], torch.full((n,), 2, dtype=torch.int32, device="cuda:0"),
+                                 scale, cap=cap, **kw)):
+        assert (o == o[..., :1]).all()
+        within(o[:, 0, 0], want, tol)

@@ -364,7 +364,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 4
     for (int e = 0; e < 4; ++e) {
       const int key = k0 + g * 4 + e;
       float x = s[e];
-      if constexpr (MADE) x = CAP ? p.cap(x) : x * p.scale_log2;
+      if constexpr (MADE) x = CAP ? p.cap.of_any(x) : x * p.scale_log2;
       if constexpr (BIAS == 1) x = fmaf(-slope, static_cast<float>(n - 1 - key), x);
       if constexpr (BIAS == 2) {
         if (near) x += in_units(dist[max(min(key, n - 1) - (n - 1), -p.radius)], kLog2e);

@@ -431,8 +431,9 @@ void attn_ruled_kernel(const RuledParams p) {
   };
   constexpr auto key_of = [](int e) { return (e >> 4) * 32 + ((e & 15) >> 2) * 8 + (e & 3); };  // of the lane's score e: t0 + 32 kt0 + key_of(e) + 4 hh
 
-  // biases of the lane's keys of the tile from t0 on
+  // biases of the lane's keys of the tile from t0 on: the scores' first values, or added to what a cap has made of them
   auto biases = [&](int t0, f32x16_v(&s)[KH]) __attribute__((always_inline)) {
+    const auto put = [&](int e, float bias) __attribute__((always_inline)) { s[e >> 4][e & 15] = CAP ? s[e >> 4][e & 15] + bias : bias; };
     const int pos = places[wave * 32 + l32], k0 = t0 + 32 * kt0, first = k0 + 4 * hh - pos;
     if constexpr (BIAS == 1) {
       const float at = static_cast<float>(first);
@@ -440,11 +441,11 @@ void attn_ruled_kernel(const RuledParams p) {
       if (before || behind) {  // (linear: one instruction each)
         const float sl = before ? slope : -slope, b0 = sl * at;
 #pragma unroll
-        for (int e = 0; e < NS; ++e) s[e >> 4][e & 15] = fmaf(sl, static_cast<float>(key_of(e)), b0);
+        for (int e = 0; e < NS; ++e) put(e, fmaf(sl, static_cast<float>(key_of(e)), b0));
       } else {
 #pragma unroll
         for (int e = 0; e < NS; ++e) {
-          s[e >> 4][e & 15] = -slope * fabsf(at + static_cast<float>(key_of(e)));
+          put(e, -slope * fabsf(at + static_cast<float>(key_of(e))));
           if (e % 8 == 7) __builtin_amdgcn_sched_barrier(0);
         }
       }
@@ -453,12 +454,12 @@ void attn_ruled_kernel(const RuledParams p) {
       if (before || behind) {
         const float far = table[before ? 0 : 2 * p.radius + 2 * kPad];
 #pragma unroll
-        for (int e = 0; e < NS; ++e) s[e >> 4][e & 15] = far;
+        for (int e = 0; e < NS; ++e) put(e, far);
       } else {
         const float* const from = table + clampi(first, -p.radius - kPad, p.radius) + p.radius + kPad;
 #pragma unroll
         for (int e = 0; e < NS; ++e) {
-          s[e >> 4][e & 15] = from[key_of(e)];
+          put(e, from[key_of(e)]);
           if (e % 8 == 7) __builtin_amdgcn_sched_barrier(0);  // (not all at once: there are no registers for it)
         }
       }
@@ -482,13 +483,24 @@ void attn_ruled_kernel(const RuledParams p) {
   // keys that some query does not see; returns the lane's maximum
   auto finish_scores = [&](int t0, bool all, f32x16_v(&s)[KH]) {
     if constexpr (CAP) {
-      f32x16_v add[KH];
-      if constexpr (BIAS != 0) biases(t0, add);
+      if (__builtin_expect(p.cap.large, 0)) {
 #pragma unroll
-      for (int e = 0; e < NS; ++e) {
-        s[e >> 4][e & 15] = p.cap(s[e >> 4][e & 15]) + (BIAS != 0 ? add[e >> 4][e & 15] : 0.f);
-        if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+        for (int e = 0; e < NS; ++e) {
+          float x = s[e >> 4][e & 15];
+          asm volatile("" : "+v"(x));  // (one after the other: there are no registers for more)
+          x = p.cap.of_large(x);
+          asm volatile("" : "+v"(x));
+          s[e >> 4][e & 15] = x;
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < NS; ++e) {
+          s[e >> 4][e & 15] = p.cap(s[e >> 4][e & 15]);
+          if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+        }
       }
+      if constexpr (BIAS != 0) biases(t0, s);
     }
     if (!all) {
       const int4 r = own();
@@ -669,192 +681,198 @@ void attn_ruled_kernel(const RuledParams p) {
   }
 
   // ---- epilogue ----
-  float l_tot = l_run + swapped(l_run);
-  if constexpr (KH == 1) {  // the upper halves' sums join the lower ones' (behind the loop's last barrier nothing is read from the tiles)
-    f32x4_v* const jo = reinterpret_cast<f32x4_v*>(lds) + (wave & 1) * (DT * 4 * 64);
-    float2* const jm = reinterpret_cast<float2*>(lds + 2 * DT * 4 * 64 * 16) + (wave & 1) * 64;
-    static_assert(2 * (DT * 4 * 64 * 16 + 64 * 8) <= 4 * TILEB, "the join fits the tiles' memory");
-    if (wave >= 2) {
+  {
+    // (what follows from the lane anew: the loop has no registers to hold it)
+    const int lane = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u)), l32 = lane & 31, hh = lane >> 5;
+    const int row = min(q0 + l32, p.Sq - 1);
+    auto swapped = [&](float x) __attribute__((always_inline)) {
+      const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+      return __uint_as_float(hh ? r[0] : r[1]);
+    };
+    float l_tot = l_run + swapped(l_run);
+    if constexpr (KH == 1) {  // the upper halves' sums join the lower ones' (behind the loop's last barrier nothing is read from the tiles)
+      f32x4_v* const jo = reinterpret_cast<f32x4_v*>(lds) + (wave & 1) * (DT * 4 * 64);
+      float2* const jm = reinterpret_cast<float2*>(lds + 2 * DT * 4 * 64 * 16) + (wave & 1) * 64;
+      static_assert(2 * (DT * 4 * 64 * 16 + 64 * 8) <= 4 * TILEB, "the join fits the tiles' memory");
+      if (wave >= 2) {
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
+        for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-        for (int g = 0; g < 4; ++g) jo[(dt * 4 + g) * 64 + lane] = f32x4_v{o[dt][g * 4], o[dt][g * 4 + 1], o[dt][g * 4 + 2], o[dt][g * 4 + 3]};
-      jm[lane] = make_float2(m_run, l_tot);
-    }
-    __syncthreads();
-    if (wave >= 2) return;
-    const float2 other = jm[lane];
-    const float m = fmaxf(m_run, other.x), m_safe = m == -INFINITY ? 0.f : m;
-    const float a = __builtin_amdgcn_exp2f((m_run - m_safe) * c), b = __builtin_amdgcn_exp2f((other.x - m_safe) * c);
-    m_run = m;
-    // (a side that saw nothing has a sum of zero, but what it multiplied by zero may be NaN)
-    l_tot = (l_tot == 0.f ? 0.f : l_tot * a) + (other.y == 0.f ? 0.f : other.y * b);
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x4_v x = jo[(dt * 4 + g) * 64 + lane];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[dt][g * 4 + e] = o[dt][g * 4 + e] * a + x[e] * b;
+          for (int g = 0; g < 4; ++g) jo[(dt * 4 + g) * 64 + lane] = f32x4_v{o[dt][g * 4], o[dt][g * 4 + 1], o[dt][g * 4 + 2], o[dt][g * 4 + 3]};
+        jm[lane] = make_float2(m_run, l_tot);
       }
-  }
-  const bool mine = q0 + l32 < p.Sq;
-  const int64_t part = (static_cast<int64_t>(unit) * p.n_qblocks + qb) * p.chunks + chunk;
-  float* const po = p.ws + part * BM * D;
-  float* const pml = p.ws + static_cast<int64_t>(p.units) * p.n_qblocks * p.chunks * BM * D + part * BM * 2;
-  T* const orow = static_cast<T*>(p.o) + b * p.os_b + h * p.os_h;
-  // stores the rows of the lanes that have one; returns the largest value in size, NaN once anything is
-  auto store = [&](bool mine) __attribute__((always_inline)) {
-    float probe = 0.f;
-    if (p.chunks > 1) {
+      __syncthreads();
+      if (wave >= 2) return;
+      const float2 other = jm[lane];
+      const float m = fmaxf(m_run, other.x), m_safe = m == -INFINITY ? 0.f : m;
+      const float a = __builtin_amdgcn_exp2f((m_run - m_safe) * c), b = __builtin_amdgcn_exp2f((other.x - m_safe) * c);
+      m_run = m;
+      // (a side that saw nothing has a sum of zero, but what it multiplied by zero may be NaN)
+      l_tot = (l_tot == 0.f ? 0.f : l_tot * a) + (other.y == 0.f ? 0.f : other.y * b);
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          f32x4_v x;
+          const f32x4_v x = jo[(dt * 4 + g) * 64 + lane];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            x[e] = l_tot == 0.f ? 0.f : o[dt][g * 4 + e];
-            if (e & 1) probe = __builtin_elementwise_maximum(__builtin_elementwise_maximum(probe, fabsf(x[e - 1])), fabsf(x[e]));
-          }
-          if (mine) *reinterpret_cast<f32x4_v*>(po + (q0 - qb * BM + l32) * D + dt * 32 + g * 8 + hh * 4) = x;
-        }
-      if (mine && hh == 0) *reinterpret_cast<float2*>(pml + (q0 - qb * BM + l32) * 2) = make_float2(m_run, l_tot);
-    } else {
-      const float inv = 1.f / l_tot;
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int g = 0; g < 4; g += 2) {
-          float x[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            x[e] = l_tot == 0.f ? 0.f : o[dt][g * 4 + e] * inv;
-            if (e & 1) probe = __builtin_elementwise_maximum(__builtin_elementwise_maximum(probe, fabsf(x[e - 1])), fabsf(x[e]));
-          }
-          auto pair = [&](int e) __attribute__((always_inline)) {
-            return __builtin_amdgcn_permlane32_swap(M::pack2(x[e], x[e + 1]), M::pack2(x[e + 4], x[e + 5]), false, false);
-          };
-          const auto lo = pair(0), hi = pair(2);
-          u32x4_v w;
-          w.x = lo[0]; w.y = hi[0]; w.z = lo[1]; w.w = hi[1];
-          if (mine) *reinterpret_cast<u32x4_v*>(orow + row * p.os_s + dt * 32 + g * 8 + hh * 8) = w;
+          for (int e = 0; e < 4; ++e) o[dt][g * 4 + e] = o[dt][g * 4 + e] * a + x[e] * b;
         }
     }
-    return probe;
-  };
-  const float probe = store(mine);
-  // rows with finite sums, but values that are not. (l_tot == 0: nothing was seen, zeros are right)
-  uint64_t bad = __ballot(mine && l_tot > 0.f && l_tot < INFINITY && !(probe < INFINITY));
-  bad = (bad | (bad >> 32)) & 0xffffffffull;
-  if (__builtin_expect(bad == 0, 1)) return;
-  int again = lane;
-  asm volatile("" : "+v"(again));  // (what follows from the lane is formed here, not held across the loop)
-  const int r32 = again & 31, rh = again >> 5;
-  const int4 its = ranges[wave * 32 + r32];
-  const auto see_some = [&](int k0, int n) { return __any((k0 < its.y && k0 + n > its.x) || (k0 < its.w && k0 + n > its.z)) != 0; };
-  const auto see_all = [&](int k0, int n) { return __all((k0 >= its.x && k0 + n <= its.y) || (k0 >= its.z && k0 + n <= its.w)) != 0; };
-  // Whether a value that is not finite lies in what was multiplied by a zero for some row: in keys of one product that not all rows see. Elsewhere
-  // such values are seen, and the rows are right as they are.
-  bool spoiled = false;
-  for (int i = 0; i < n_tiles && !spoiled; ++i)
-    for (int k0 = tile_at(i) * BN, n = 0; n < BN && !spoiled; n += WN, k0 += WN) {
-      if (!see_some(k0, WN) || see_all(k0, WN)) continue;
-      bool found = false;
-      for (int r = again / CPR; r < WN; r += RPI) {
-        const u32x4 x = load_raw(vbase + min(k0 + r, p.Sk - 1) * p.vs_s + again % CPR * 8);
+    const bool mine = q0 + l32 < p.Sq;
+    const int64_t part = (static_cast<int64_t>(unit) * p.n_qblocks + qb) * p.chunks + chunk;
+    float* const po = p.ws + part * BM * D;
+    float* const pml = p.ws + static_cast<int64_t>(p.units) * p.n_qblocks * p.chunks * BM * D + part * BM * 2;
+    T* const orow = static_cast<T*>(p.o) + b * p.os_b + h * p.os_h;
+    // stores the rows of the lanes that have one; returns the largest value in size, NaN once anything is
+    auto store = [&](bool mine) __attribute__((always_inline)) {
+      float probe = 0.f;
+      if (p.chunks > 1) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) found |= not_finite<T>(x[e]) || not_finite<T>(x[e] >> 16);
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            f32x4_v x;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              x[e] = l_tot == 0.f ? 0.f : o[dt][g * 4 + e];
+              if (e & 1) probe = __builtin_elementwise_maximum(__builtin_elementwise_maximum(probe, fabsf(x[e - 1])), fabsf(x[e]));
+            }
+            if (mine) *reinterpret_cast<f32x4_v*>(po + (q0 - qb * BM + l32) * D + dt * 32 + g * 8 + hh * 4) = x;
+          }
+        if (mine && hh == 0) *reinterpret_cast<float2*>(pml + (q0 - qb * BM + l32) * 2) = make_float2(m_run, l_tot);
+      } else {
+        const float inv = 1.f / l_tot;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int g = 0; g < 4; g += 2) {
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              x[e] = l_tot == 0.f ? 0.f : o[dt][g * 4 + e] * inv;
+              if (e & 1) probe = __builtin_elementwise_maximum(__builtin_elementwise_maximum(probe, fabsf(x[e - 1])), fabsf(x[e]));
+            }
+            auto pair = [&](int e) __attribute__((always_inline)) {
+              return __builtin_amdgcn_permlane32_swap(M::pack2(x[e], x[e + 1]), M::pack2(x[e + 4], x[e + 5]), false, false);
+            };
+            const auto lo = pair(0), hi = pair(2);
+            u32x4_v w;
+            w.x = lo[0]; w.y = hi[0]; w.z = lo[1]; w.w = hi[1];
+            if (mine) *reinterpret_cast<u32x4_v*>(orow + row * p.os_s + dt * 32 + g * 8 + hh * 8) = w;
+          }
       }
-      spoiled = __any(found) != 0;
-    }
-  if (!spoiled) return;
-  // The rows of the wavefront again, 32 keys at a time, straight from memory. A product takes the values that are finite, zeros for the others; where there
-  // are others, a second product counts for each feature and row those that the row sees, by kind (1, 64 and 4096 each, of 16 keys: its sum
-  // says how many of which), and they are added as what they are. us, 4096 causal tokens, 16 heads of 128 on 4: all finite 91, one infinite value at the
-  // head, which all rows see, 115, one NaN in the middle 250, a feature that is infinite at every key 846 (row by row, any of them took 20000).
-  l_run = 0.f;
-  m_run = -INFINITY;
+      return probe;
+    };
+    const float probe = store(mine);
+    // rows with finite sums, but values that are not. (l_tot == 0: nothing was seen, zeros are right)
+    uint64_t bad = __ballot(mine && l_tot > 0.f && l_tot < INFINITY && !(probe < INFINITY));
+    bad = (bad | (bad >> 32)) & 0xffffffffull;
+    if (__builtin_expect(bad == 0, 1)) return;
+    const int4 its = ranges[wave * 32 + l32];
+    const auto see_some = [&](int k0, int n) { return __any((k0 < its.y && k0 + n > its.x) || (k0 < its.w && k0 + n > its.z)) != 0; };
+    const auto see_all = [&](int k0, int n) { return __all((k0 >= its.x && k0 + n <= its.y) || (k0 >= its.z && k0 + n <= its.w)) != 0; };
+    // Whether a value that is not finite lies in what was multiplied by a zero for some row: in keys of one product that not all rows see. Elsewhere
+    // such values are seen, and the rows are right as they are.
+    bool spoiled = false;
+    for (int i = 0; i < n_tiles && !spoiled; ++i)
+      for (int k0 = tile_at(i) * BN, n = 0; n < BN && !spoiled; n += WN, k0 += WN) {
+        if (!see_some(k0, WN) || see_all(k0, WN)) continue;
+        bool found = false;
+        for (int r = lane / CPR; r < WN; r += RPI) {
+          const u32x4 x = load_raw(vbase + min(k0 + r, p.Sk - 1) * p.vs_s + lane % CPR * 8);
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-    for (int e = 0; e < 16; ++e) o[dt][e] = 0.f;
-  const int at = BIAS != 0 ? places[wave * 32 + r32] : 0;
-  const T* const qp = static_cast<const T*>(p.q) + b * p.qs_b + h * p.qs_h + min(q0 + r32, p.Sq - 1) * p.qs_s + rh * 8;
-  for (int i = 0; i < 2 * n_tiles; ++i) {
-    const int t0 = tile_at(i >> 1) * BN, k0 = t0 + (i & 1) * 32;
-    if (!see_some(k0, 32)) continue;
-    f32x16_v x;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) x[e] = 0.f;
-    const T* const kp = kbase + min(k0 + r32, p.Sk - 1) * p.ks_s + rh * 8;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {  // (the queries from memory too: their registers are needed here)
-      x = M::run(__builtin_bit_cast(frag, *reinterpret_cast<const u32x4_v*>(kp + ks * 16)), __builtin_bit_cast(frag, *reinterpret_cast<const u32x4_v*>(qp + ks * 16)), x);
-    }
-    const uint32_t sees = static_cast<uint32_t>((range_bits(its.x, its.y, t0) | range_bits(its.z, its.w, t0)) >> (32 * (i & 1))) >> (4 * rh);
-    float mx = -INFINITY;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const int away = k0 + key_of(e) + 4 * rh - at;
-      float bias = 0.f;
-      if constexpr (BIAS == 1) bias = -slope * fabsf(static_cast<float>(away));
-      if constexpr (BIAS == 2) bias = table[clampi(away, -p.radius, p.radius) + p.radius + kPad];
-      x[e] = (sees >> key_of(e)) & 1 ? (CAP ? p.cap(x[e]) : x[e]) + bias : -INFINITY;
-      mx = fmaxf(mx, x[e]);
-    }
-    const float m_new = fmaxf(m_run, fmaxf(mx, swapped(mx))), m_safe = m_new == -INFINITY ? 0.f : m_new;
-    const float alpha = __builtin_amdgcn_exp2f((m_run - m_safe) * c);
-    m_run = m_new;
-    l_run *= alpha;
+          for (int e = 0; e < 4; ++e) found |= not_finite<T>(x[e]) || not_finite<T>(x[e] >> 16);
+        }
+        spoiled = __any(found) != 0;
+      }
+    if (!spoiled) return;
+    // The rows of the wavefront lane, 32 keys at a time, straight from memory. A product takes the values that are finite, zeros for the others; where there
+    // are others, a second product counts for each feature and row those that the row sees, by kind (1, 64 and 4096 each, of 16 keys: its sum
+    // says how many of which), and they are added as what they are. us, 4096 causal tokens, 16 heads of 128 on 4: all finite 91, one infinite value at the
+    // head, which all rows see, 115, one NaN in the middle 250, a feature that is infinite at every key 846 (row by row, any of them took 20000).
+    l_run = 0.f;
+    m_run = -INFINITY;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) o[dt][e] = fabsf(o[dt][e]) < INFINITY ? o[dt][e] * alpha : o[dt][e];
-    u32x4_v weights[2], ones[2];
+      for (int e = 0; e < 16; ++e) o[dt][e] = 0.f;
+    const int at = BIAS != 0 ? places[wave * 32 + l32] : 0;
+    const T* const qp = static_cast<const T*>(p.q) + b * p.qs_b + h * p.qs_h + row * p.qs_s + hh * 8;
+    for (int i = 0; i < 2 * n_tiles; ++i) {
+      const int t0 = tile_at(i >> 1) * BN, k0 = t0 + (i & 1) * 32;
+      if (!see_some(k0, 32)) continue;
+      f32x16_v x;
 #pragma unroll
-    for (int e = 0; e < 16; e += 2) {
-      const float p0 = __builtin_amdgcn_exp2f((x[e] - m_safe) * c), p1 = __builtin_amdgcn_exp2f((x[e + 1] - m_safe) * c);
-      l_run += p0 + p1;
-      weights[e >> 3][(e & 7) >> 1] = M::pack2(p0, p1);
-      ones[e >> 3][(e & 7) >> 1] = M::pack2((sees >> key_of(e)) & 1 ? 1.f : 0.f, (sees >> key_of(e + 1)) & 1 ? 1.f : 0.f);
-    }
+      for (int e = 0; e < 16; ++e) x[e] = 0.f;
+      const T* const kp = kbase + min(k0 + l32, p.Sk - 1) * p.ks_s + hh * 8;
 #pragma unroll
-    for (int g = 0; g < 2; ++g)
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        uint32_t v[8];
-        bool others = false;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int key = min(k0 + g * 16 + (j >> 2) * 8 + 4 * rh + (j & 3), p.Sk - 1);
-          v[j] = *reinterpret_cast<const uint16_t*>(vbase + key * p.vs_s + dt * 32 + r32);
-          others |= not_finite<T>(v[j]);
-        }
-        u32x4_v clean;
-#pragma unroll
-        for (int j = 0; j < 8; j += 2) clean[j >> 1] = (not_finite<T>(v[j]) ? 0u : v[j]) | (not_finite<T>(v[j + 1]) ? 0u : v[j + 1] << 16);
-        o[dt] = M::run(__builtin_bit_cast(frag, clean), __builtin_bit_cast(frag, weights[g]), o[dt]);
-        if (!__any(others)) continue;
-        const auto kind = [](uint32_t u) { return !not_finite<T>(u) ? 0.f : is_nan<T>(u) ? 4096.f : (u & 0x8000u) ? 64.f : 1.f; };
-        u32x4_v kinds;
-        f32x16_v found;
-#pragma unroll
-        for (int j = 0; j < 8; j += 2) kinds[j >> 1] = M::pack2(kind(v[j]), kind(v[j + 1]));
-#pragma unroll
-        for (int e = 0; e < 16; ++e) found[e] = 0.f;
-        found = M::run(__builtin_bit_cast(frag, kinds), __builtin_bit_cast(frag, ones[g]), found);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int n = static_cast<int>(found[e]);
-          if (n >= 4096) o[dt][e] = NAN;
-          if (n & 63) o[dt][e] += INFINITY;
-          if (n & 4032) o[dt][e] -= INFINITY;
-        }
+      for (int ks = 0; ks < KS; ++ks) {  // (the queries from memory too: their registers are needed here)
+        x = M::run(__builtin_bit_cast(frag, *reinterpret_cast<const u32x4_v*>(kp + ks * 16)), __builtin_bit_cast(frag, *reinterpret_cast<const u32x4_v*>(qp + ks * 16)), x);
       }
+      const uint32_t sees = static_cast<uint32_t>((range_bits(its.x, its.y, t0) | range_bits(its.z, its.w, t0)) >> (32 * (i & 1))) >> (4 * hh);
+      float mx = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int away = k0 + key_of(e) + 4 * hh - at;
+        float bias = 0.f;
+        if constexpr (BIAS == 1) bias = -slope * fabsf(static_cast<float>(away));
+        if constexpr (BIAS == 2) bias = table[clampi(away, -p.radius, p.radius) + p.radius + kPad];
+        x[e] = (sees >> key_of(e)) & 1 ? (CAP ? p.cap.of_any(x[e]) : x[e]) + bias : -INFINITY;
+        mx = fmaxf(mx, x[e]);
+      }
+      const float m_new = fmaxf(m_run, fmaxf(mx, swapped(mx))), m_safe = m_new == -INFINITY ? 0.f : m_new;
+      const float alpha = __builtin_amdgcn_exp2f((m_run - m_safe) * c);
+      m_run = m_new;
+      l_run *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[dt][e] = fabsf(o[dt][e]) < INFINITY ? o[dt][e] * alpha : o[dt][e];
+      u32x4_v weights[2], ones[2];
+#pragma unroll
+      for (int e = 0; e < 16; e += 2) {
+        const float p0 = __builtin_amdgcn_exp2f((x[e] - m_safe) * c), p1 = __builtin_amdgcn_exp2f((x[e + 1] - m_safe) * c);
+        l_run += p0 + p1;
+        weights[e >> 3][(e & 7) >> 1] = M::pack2(p0, p1);
+        ones[e >> 3][(e & 7) >> 1] = M::pack2((sees >> key_of(e)) & 1 ? 1.f : 0.f, (sees >> key_of(e + 1)) & 1 ? 1.f : 0.f);
+      }
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          uint32_t v[8];
+          bool others = false;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int key = min(k0 + g * 16 + (j >> 2) * 8 + 4 * hh + (j & 3), p.Sk - 1);
+            v[j] = *reinterpret_cast<const uint16_t*>(vbase + key * p.vs_s + dt * 32 + l32);
+            others |= not_finite<T>(v[j]);
+          }
+          u32x4_v clean;
+#pragma unroll
+          for (int j = 0; j < 8; j += 2) clean[j >> 1] = (not_finite<T>(v[j]) ? 0u : v[j]) | (not_finite<T>(v[j + 1]) ? 0u : v[j + 1] << 16);
+          o[dt] = M::run(__builtin_bit_cast(frag, clean), __builtin_bit_cast(frag, weights[g]), o[dt]);
+          if (!__any(others)) continue;
+          const auto kind = [](uint32_t u) { return !not_finite<T>(u) ? 0.f : is_nan<T>(u) ? 4096.f : (u & 0x8000u) ? 64.f : 1.f; };
+          u32x4_v kinds;
+          f32x16_v found;
+#pragma unroll
+          for (int j = 0; j < 8; j += 2) kinds[j >> 1] = M::pack2(kind(v[j]), kind(v[j + 1]));
+#pragma unroll
+          for (int e = 0; e < 16; ++e) found[e] = 0.f;
+          found = M::run(__builtin_bit_cast(frag, kinds), __builtin_bit_cast(frag, ones[g]), found);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int n = static_cast<int>(found[e]);
+            if (n >= 4096) o[dt][e] = NAN;
+            if (n & 63) o[dt][e] += INFINITY;
+            if (n & 4032) o[dt][e] -= INFINITY;
+          }
+        }
+    }
+    l_tot = l_run + swapped(l_run);
+    store(mine && ((bad >> l32) & 1) != 0);
   }
-  l_tot = l_run + swapped(l_run);
-  store(mine && ((bad >> l32) & 1) != 0);
 }
 
 // Joins the chunks' sums, a wavefront for each row: o = sum_c 2^(m_c - m) o_c / sum_c 2^(m_c - m) l_c, m = max_c m_c. Lane c has chunk c's
