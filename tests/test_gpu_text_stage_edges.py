@@ -301,3 +301,27 @@ def test_scores_keep_their_digits_under_any_cap(gpu, cap, kind, scale, step, D):
                                  scale, cap=cap, **kw)):
         assert (o == o[..., :1]).all()
         within(o[:, 0, 0], want, tol)
+
+
+# ------------------------------------------------------------------------------------------------ derivatives
+def test_tangents_are_refused(gpu):
+    """Forward-mode derivatives, like gradients: not dropped without a word. Inference mode is for calls that want none."""
+    q, kv, slopes = _randn(60, 1, 8, 4, 64), _randn(61, 1, 8, 2, 64), torch.ones(4, device="cuda:0")
+    table, lengths, at = (torch.zeros(8, 1, dtype=torch.int32, device="cuda:0"), torch.full((8,), 3, dtype=torch.int32, device="cuda:0"), torch.arange(8, device="cuda:0"))
+    turns = torch.rand(32, dtype=torch.float64, device="cuda:0")
+    calls = {"attn_ruled": (lambda q, kv, s: kernels.attn_ruled(q, kv, kv, 0.1, slopes=s)),
+             "attn_paged": (lambda q, kv, s: kernels.attn_paged(q[0], kv, kv, table, lengths, 0.1, slopes=s)),
+             "rope_append": (lambda q, kv, s: kernels.rope_append(q[0], kv[0], None, at, turns * s[0]))}
+    dual = torch.autograd.forward_ad
+    for name, call in calls.items():
+        call(q, kv, slopes)
+        with dual.dual_level():
+            call(q, kv, slopes)
+            for i, t in enumerate((q, kv, slopes)):
+                args = [q, kv, slopes]
+                args[i] = dual.make_dual(t, torch.ones_like(t))
+                for grad in (True, False):
+                    with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match=name):
+                        call(*args)
+                with torch.inference_mode():
+                    call(*args)

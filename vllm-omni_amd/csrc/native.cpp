@@ -20,6 +20,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/hip/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
@@ -593,11 +594,11 @@ PyObject* py_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // ------------------------------------------------------------------------------------- a text stage's operators
-// whether a gradient would be asked of the result: kernels.py refuses that
+// whether a gradient would be asked of the result, or a tangent has come in: kernels.py refuses that
 bool wants_grad(std::initializer_list<const Tensor*> ts) {
-  if (!c10::GradMode::is_enabled()) return false;
+  const bool backward = c10::GradMode::is_enabled(), forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
   for (const Tensor* t : ts)
-    if (t && t->requires_grad()) return true;
+    if (t && ((backward && t->requires_grad()) || (forward && t->_fw_grad(0).defined()))) return true;
   return false;
 }
 

@@ -315,8 +315,11 @@ def _attn_scratch(device: int, stream: int, need: int) -> torch.Tensor:
 
 # ------------------------------------------------------------------------- a text stage: prompts, and one token at a time
 def _inference_only(name: str, *tensors: torch.Tensor | None) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    held = [t for t in tensors if t is not None]
+    if torch.is_grad_enabled() and any(t.requires_grad for t in held):
         raise RuntimeError(f"{name} has no backward pass: call it under torch.inference_mode() or torch.no_grad()")
+    if not torch.is_inference_mode_enabled() and any(torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in held):
+        raise RuntimeError(f"{name} has no forward-mode derivative: call it without tangents or under torch.inference_mode()")
 
 
 def _strided8(t: torch.Tensor) -> torch.Tensor:
