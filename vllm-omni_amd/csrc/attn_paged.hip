@@ -9,9 +9,11 @@
 //
 // The sequences' keys are cut into chunks, a workgroup each; a chunk's tiles of 16 keys go round its 4 wavefronts. A wavefront has two stages
 // of LDS of its own and fills one, 16 bytes a lane straight from global memory, while it computes the other: no barrier in the loop. The page
-// numbers of the chunk wait in LDS, so nothing else is loaded there. (Tiles of 32 keys leave room for one workgroup of head size 128 on a compute
-// unit, and nothing runs while it begins and ends: 8 sequences of 4096 keys 37 to 51 us, so 31.) The wavefronts' sums are joined in LDS, the
-// chunks' by the last workgroup of a sequence to be done, or by a second launch.
+// numbers of the chunk wait in LDS, so nothing else is loaded there but, of a table of biases, those of keys within its radius: the wait for them
+// is one for the tile on its way too (32 sequences, 24 heads of 64, window of 1024: 36.4 us without a table, 37.7 with a radius of 128, 44.5 with
+// 1024). (Tiles of 32 keys leave room for one workgroup of head size 128 on a compute unit, and nothing runs while it begins and ends: 8 sequences
+// of 4096 keys 37 to 51 us, so 31.) The wavefronts' sums are joined in LDS, the chunks' by the last workgroup of a sequence to be done, or by a
+// second launch.
 //
 // Rows behind a sequence's last key are never read, as a page may hold anything there: the tile's rest is the last key again, with no
 // weight and values of zero.

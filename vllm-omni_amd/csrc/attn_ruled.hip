@@ -163,8 +163,8 @@ void attn_ruled_kernel(const RuledParams p) {
   // the last query blocks, which see most under a causal order, begin first; where the heads divide over the XCDs, an XCD keeps its heads
   // (steep slopes leave a head little to do: with slopes the heads go round the XCDs and back again, so that each has steep and shallow ones, and an XCD
   // begins its rows of blocks with each of its heads in turn: it hands workgroups to its shader engines in a fixed order, so that those which
-  // would get steep heads alone stood empty while the others were full. us of 16384 causal tokens, 16 heads of 128: 1040 with neighbours on an XCD, 929 going
-  // round, 910 there and back; with far tiles left out 860, and 645 with the heads in turn)
+  // would get steep heads alone stood empty while the others were full. us of 16384 causal tokens, 16 heads of 128: while all tiles were visited, 1040 with
+  // neighbours on an XCD, 929 going round, 910 there and back; with far tiles left out 828, and 632 with the heads in turn on the same box, 435 and 360 of 8192, 32 on 8)
   const int chunk = p.chunks > 1 ? p.by_blocks(blockIdx.x) : 0, block = blockIdx.x - chunk * (p.units * p.n_qblocks);
   int unit, qb;
   if (BIAS != 1 && p.units % kNumXcd == 0) {
