@@ -164,7 +164,7 @@ void attn_ruled_kernel(const RuledParams p) {
   // (steep slopes leave a head little to do: with slopes the heads go round the XCDs and back again, so that each has steep and shallow ones, and an XCD
   // begins its rows of blocks with each of its heads in turn: it hands workgroups to its shader engines in a fixed order, so that those which
   // would get steep heads alone stood empty while the others were full. us of 16384 causal tokens, 16 heads of 128: while all tiles were visited, 1040 with
-  // neighbours on an XCD, 929 going round, 910 there and back; with far tiles left out 828, and 632 with the heads in turn on the same box, 435 and 360 of 8192, 32 on 8)
+  // neighbours on an XCD, 929 going round, 910 there and back; with far tiles left out 828, and 632 with the heads in turn on the same card, 435 and 360 of 8192, 32 on 8)
   const int chunk = p.chunks > 1 ? p.by_blocks(blockIdx.x) : 0, block = blockIdx.x - chunk * (p.units * p.n_qblocks);
   int unit, qb;
   if (BIAS != 1 && p.units % kNumXcd == 0) {
@@ -786,7 +786,7 @@ void attn_ruled_kernel(const RuledParams p) {
         spoiled = __any(found) != 0;
       }
     if (!spoiled) return;
-    // The rows of the wavefront lane, 32 keys at a time, straight from memory. A product takes the values that are finite, zeros for the others; where there
+    // The rows of the wavefront once more, 32 keys at a time, straight from memory. A product takes the values that are finite, zeros for the others; where there
     // are others, a second product counts for each feature and row those that the row sees, by kind (1, 64 and 4096 each, of 16 keys: its sum
     // says how many of which), and they are added as what they are. us, 4096 causal tokens, 16 heads of 128 on 4: all finite 91, one infinite value at the
     // head, which all rows see, 115, one NaN in the middle 250, a feature that is infinite at every key 846 (row by row, any of them took 20000).
